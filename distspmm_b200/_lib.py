@@ -66,6 +66,23 @@ class dsp_rank_stats(ctypes.Structure):
         (n, ctypes.c_float) for n in ("model_rows_ms", "model_split_ms", "model_groups_ms")]
 
 
+class dsp_pattern_info(ctypes.Structure):
+    _fields_ = [(n, c_i64) for n in ("rows", "cols", "nnz", "flags", "chunk_units", "chunks", "split_rows",
+                                     "max_row_len", "device_bytes")]
+
+
+class dsp_act_desc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("act", c_int), ("N", c_int), ("values", c_vp), ("B", c_vp), ("ldb", c_i64),
+                ("bias", c_vp), ("residual", c_vp), ("ldr", c_i64), ("out", c_vp), ("ldo", c_i64), ("pre", c_vp),
+                ("ldp", c_i64)]
+
+
+class dsp_act_grad_desc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("act", c_int), ("N", c_int), ("values", c_vp), ("B", c_vp), ("ldb", c_i64),
+                ("pre", c_vp), ("ldp", c_i64), ("dout", c_vp), ("lddo", c_i64), ("dB", c_vp), ("lddb", c_i64),
+                ("dvalues", c_vp), ("dbias", c_vp)]
+
+
 class dsp_args(ctypes.Structure):
     _fields_ = [("file", ctypes.c_char_p), ("matrix", P(dsp_csr)), ("dims", c_int), ("task_dist", c_int),
                 ("comm_type", c_int), ("n_rolls", c_int), ("repeat", c_int), ("n_streams", c_int),
@@ -125,6 +142,13 @@ PROTOTYPES = {
     "dsp_spmm_check_error": (c_int, [c_vp]),
     "dsp_spmm_csr_f32_noalloc": (c_int, [c_vp, c_vp, c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_int,
                                          c_int, c_vp]),
+    "dsp_pattern_create": (c_int, [c_int, P(dsp_csr), c_int, P(c_vp)]),
+    "dsp_pattern_destroy": (None, [c_vp]),
+    "dsp_pattern_info_get": (c_int, [c_vp, P(dsp_pattern_info)]),
+    "dsp_spmm_act_workspace": (c_i64, [c_vp, c_int]),
+    "dsp_spmm_act": (c_int, [c_vp, P(dsp_act_desc), c_vp, c_i64, c_vp]),
+    "dsp_spmm_act_grad_workspace": (c_i64, [c_vp, P(dsp_act_grad_desc)]),
+    "dsp_spmm_act_grad": (c_int, [c_vp, P(dsp_act_grad_desc), c_vp, c_i64, c_vp]),
     "dsp_rank_create": (c_int, [P(dsp_rank_desc), P(c_vp)]),
     "dsp_rank_destroy": (None, [c_vp]),
     "dsp_rank_stats_get": (c_int, [c_vp, P(dsp_rank_stats)]),

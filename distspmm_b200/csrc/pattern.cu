@@ -1,0 +1,206 @@
+// pattern.cu — dsp_pattern: a CSR matrix prepared once for the fused product (act.cu) and for attention (attn.cu).
+#include <string.h>
+
+#include <algorithm>
+#include <new>
+
+#include "pattern.h"
+
+namespace dsp {
+
+int32_t pattern_chunk_units(int64_t units) {
+  int64_t l = (units + 148 * 48 - 1) / (148 * 48);
+  l = (l + 31) / 32 * 32;
+  return (int32_t)std::min<int64_t>(512, std::max<int64_t>(64, l));
+}
+
+void pattern_chunks(int32_t n, HostDir *d) {
+  const int64_t nnz = d->ptr[n], units = n + nnz;
+  d->L = pattern_chunk_units(units);
+  d->n_chunks = (int32_t)((units + d->L - 1) / d->L);
+  d->row_of.resize(nnz);
+  d->row0.resize(d->n_chunks + 1);
+  d->nz0.resize(d->n_chunks + 1);
+  parallel_for(n, [&](int64_t b, int64_t e) {
+    for (int64_t r = b; r < e; ++r)
+      for (int32_t p = d->ptr[r]; p < d->ptr[r + 1]; ++p) d->row_of[p] = (int32_t)r;
+  });
+  parallel_for(d->n_chunks + 1, [&](int64_t b, int64_t e) {
+    for (int64_t c = b; c < e; ++c) {
+      const int64_t x = std::min<int64_t>(c * d->L, units);
+      // rows ended before unit x: the row r whose units r + ptr[r] .. r + ptr[r+1] hold x
+      int64_t lo = 0, hi = n;
+      while (lo < hi) {
+        const int64_t m = (lo + hi) / 2;
+        if (m + d->ptr[m + 1] < x) lo = m + 1;
+        else hi = m;
+      }
+      d->row0[c] = (int32_t)lo;
+      d->nz0[c] = (int32_t)(x - lo);
+    }
+  });
+  d->split_row.clear();
+  for (int32_t r = 0; r < n; ++r)
+    if (((int64_t)r + d->ptr[r]) / d->L != ((int64_t)r + d->ptr[r + 1]) / d->L) d->split_row.push_back(r);
+}
+
+namespace {
+
+template <class V>
+int put(dsp_pattern *p, const std::vector<V> &h, V **out) {
+  *out = nullptr;
+  const size_t bytes = std::max<size_t>(h.size(), 1) * sizeof(V) + 16;  // vector loads may read past the last entry
+  void *d = nullptr;
+  cudaError_t e = cudaMalloc(&d, bytes);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(DSP_ERR_NOMEM, "dsp_pattern_create: %zu bytes: %s", bytes, cudaGetErrorString(e));
+  }
+  p->allocs.push_back(d);
+  p->device_bytes += (int64_t)bytes;
+  if (!h.empty() && (e = cudaMemcpy(d, h.data(), h.size() * sizeof(V), cudaMemcpyHostToDevice)) != cudaSuccess)
+    return fail(DSP_ERR_CUDA, "dsp_pattern_create: %s", cudaGetErrorString(e));
+  *out = (V *)d;
+  return DSP_OK;
+}
+
+int put_dir(dsp_pattern *p, int32_t n, const HostDir &h, PatternDir *d) {
+  d->n = n;
+  d->L = h.L;
+  d->n_chunks = h.n_chunks;
+  d->n_split = (int32_t)h.split_row.size();
+  int rc;
+  if ((rc = put(p, h.ptr, &d->ptr)) || (rc = put(p, h.row_of, &d->row_of)) || (rc = put(p, h.cols, &d->cols)) ||
+      (rc = put(p, h.row0, &d->row0)) || (rc = put(p, h.nz0, &d->nz0)) || (rc = put(p, h.split_row, &d->split_row)))
+    return rc;
+  if (!h.perm.empty() && (rc = put(p, h.perm, &d->perm))) return rc;
+  return DSP_OK;
+}
+
+// A row that lists a column twice, or -1.
+int64_t repeated_column(const dsp_csr *a) {
+  std::atomic<int64_t> bad{-1};
+  std::atomic<bool> no_memory{false};
+  parallel_for(a->num_rows, [&](int64_t b, int64_t e) {
+    for (int64_t r = b; r < e && bad.load() < 0; ++r) {
+      const int64_t *x = a->indices + a->indptr[r], *y = a->indices + a->indptr[r + 1];
+      bool rising = true;
+      for (const int64_t *q = x; q + 1 < y; ++q) rising &= q[0] < q[1];
+      if (rising) continue;
+      try {  // an exception must not leave the worker thread
+        std::vector<int64_t> s(x, y);
+        std::sort(s.begin(), s.end());
+        if (std::adjacent_find(s.begin(), s.end()) != s.end()) bad.store(r);
+      } catch (const std::bad_alloc &) {
+        no_memory.store(true);
+      }
+    }
+  }, 1024);
+  if (no_memory.load()) throw std::bad_alloc();
+  return bad.load();
+}
+
+int create(int device, const dsp_csr *a, int flags, dsp_pattern *p) {
+  const int32_t M = (int32_t)a->num_rows, K = (int32_t)a->num_cols;
+  p->device = device;
+  p->flags = flags;
+  p->rows = M;
+  p->cols = K;
+  p->nnz = a->nnz;
+  HostDir h;
+  h.ptr.resize(M + 1);
+  h.cols.resize(a->nnz);
+  for (int32_t r = 0; r <= M; ++r) h.ptr[r] = (int32_t)a->indptr[r];
+  for (int32_t r = 0; r < M; ++r) p->max_row_len = std::max<int64_t>(p->max_row_len, h.ptr[r + 1] - h.ptr[r]);
+  parallel_for(a->nnz, [&](int64_t b, int64_t e) {
+    for (int64_t i = b; i < e; ++i) h.cols[i] = (int32_t)a->indices[i];
+  });
+  pattern_chunks(M, &h);
+  HostDir t;
+  if (flags & DSP_PATTERN_GRAD) {  // counting sort by column: entries of a column in row order
+    t.ptr.assign(K + 1, 0);
+    t.cols.resize(a->nnz);
+    t.perm.resize(a->nnz);
+    for (int64_t i = 0; i < a->nnz; ++i) ++t.ptr[h.cols[i] + 1];
+    for (int32_t c = 0; c < K; ++c) t.ptr[c + 1] += t.ptr[c];
+    std::vector<int32_t> at(t.ptr.begin(), t.ptr.end() - 1);
+    for (int64_t i = 0; i < a->nnz; ++i) {
+      const int32_t q = at[h.cols[i]]++;
+      t.cols[q] = h.row_of[i];
+      t.perm[q] = (int32_t)i;
+    }
+    pattern_chunks(K, &t);
+  }
+  DeviceGuard g(device);
+  if (g.err != cudaSuccess) return fail(DSP_ERR_CUDA, "cudaSetDevice(%d): %s", device, cudaGetErrorString(g.err));
+  cudaError_t e = cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, device);
+  if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_pattern_create: %s", cudaGetErrorString(e));
+  int rc = put_dir(p, M, h, &p->a);
+  if (!rc && (flags & DSP_PATTERN_GRAD)) rc = put_dir(p, K, t, &p->t);
+  return rc;
+}
+
+}  // namespace
+}  // namespace dsp
+
+using namespace dsp;
+
+extern "C" int dsp_pattern_create(int device, const dsp_csr *a, int flags, dsp_pattern **out) {
+  DSP_TRY_ARG(a && out && a->indptr, "dsp_pattern_create: null argument");
+  *out = nullptr;
+  DSP_TRY_ARG((flags & ~(DSP_PATTERN_GRAD | DSP_PATTERN_ATTENTION)) == 0, "dsp_pattern_create: flags %d", flags);
+  DSP_TRY_ARG(a->num_rows >= 0 && a->num_cols >= 0 && a->nnz >= 0, "dsp_pattern_create: negative size");
+  DSP_TRY_ARG(a->nnz == 0 || a->indices, "dsp_pattern_create: null indices");
+  if (a->num_rows >= INT32_MAX || a->num_cols >= INT32_MAX || a->nnz >= INT32_MAX)
+    return fail(DSP_ERR_UNSUPPORTED, "dsp_pattern_create: %lld x %lld with %lld entries: ids are 32-bit",
+                (long long)a->num_rows, (long long)a->num_cols, (long long)a->nnz);
+  dsp_pattern *p = nullptr;
+  try {
+    int rc = dsp_csr_validate(a);
+    if (rc) return rc;
+    if (flags & DSP_PATTERN_ATTENTION) {
+      const int64_t r = repeated_column(a);
+      if (r >= 0)
+        return fail(DSP_ERR_FORMAT, "dsp_pattern_create: row %lld lists a column twice (attention needs distinct keys)",
+                    (long long)r);
+    }
+    p = new dsp_pattern();
+    rc = create(device, a, flags, p);
+    if (rc) {
+      dsp_pattern_destroy(p);
+      return rc;
+    }
+  } catch (const std::bad_alloc &) {
+    dsp_pattern_destroy(p);
+    return fail(DSP_ERR_NOMEM, "dsp_pattern_create: out of host memory");
+  } catch (const std::exception &e) {
+    dsp_pattern_destroy(p);
+    return fail(DSP_ERR_STATE, "dsp_pattern_create: %s", e.what());
+  }
+  *out = p;
+  return DSP_OK;
+}
+
+extern "C" void dsp_pattern_destroy(dsp_pattern *p) {
+  if (!p) return;
+  {
+    DeviceGuard g(p->device);
+    for (void *d : p->allocs) cudaFree(d);
+  }
+  delete p;
+}
+
+extern "C" int dsp_pattern_info_get(const dsp_pattern *p, dsp_pattern_info *info) {
+  DSP_TRY_ARG(p && info, "dsp_pattern_info_get: null argument");
+  memset(info, 0, sizeof *info);
+  info->rows = p->rows;
+  info->cols = p->cols;
+  info->nnz = p->nnz;
+  info->flags = p->flags;
+  info->chunk_units = p->a.L;
+  info->chunks = p->a.n_chunks;
+  info->split_rows = p->a.n_split;
+  info->max_row_len = p->max_row_len;
+  info->device_bytes = p->device_bytes;
+  return DSP_OK;
+}

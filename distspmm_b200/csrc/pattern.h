@@ -1,0 +1,79 @@
+// pattern.h — the device-resident CSR pattern shared by the fused product and the attention kernels.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <vector>
+
+#include "internal.h"
+
+namespace dsp {
+
+// One orientation of the pattern (A, or A transposed), with its balanced work chunks.
+//
+// The work of one orientation is a path of n + nnz units: the entries of row 0, the end of row 0, the entries of row 1,
+// its end, ... (merge path). Chunk c holds the units [c L, (c + 1) L): the row ends row0[c] .. row0[c+1] - 1 and the
+// entries nz0[c] .. nz0[c+1] - 1, so rows of any length and rows without entries cost the same for the same number of
+// units. Row r spans the units r + ptr[r] .. r + ptr[r+1]; it is cut when these lie in different chunks, and then leaves
+// one partial in each of them: in slot 2c + 1 of the chunk it starts in, in slot 2c of every later one. The list of
+// cut rows is split_row.
+struct PatternDir {
+  int32_t n = 0;          // rows of this orientation
+  int32_t n_chunks = 0;
+  int32_t L = 0;          // units of a chunk
+  int32_t n_split = 0;
+  int32_t *ptr = nullptr;        // [n + 1]
+  int32_t *row_of = nullptr;     // [nnz]
+  int32_t *cols = nullptr;       // [nnz]
+  int32_t *perm = nullptr;       // [nnz] place of the entry in A's own order (transposed orientation only)
+  int32_t *row0 = nullptr;       // [n_chunks + 1]
+  int32_t *nz0 = nullptr;        // [n_chunks + 1]
+  int32_t *split_row = nullptr;  // [n_split]
+};
+
+// Kernel-side view (passed by value).
+struct DirView {
+  int32_t n, n_chunks, L, n_split;
+  const int32_t *ptr, *row_of, *cols, *perm, *row0, *nz0, *split_row;
+};
+
+inline DirView view(const PatternDir &d) {
+  return {d.n, d.n_chunks, d.L, d.n_split, d.ptr, d.row_of, d.cols, d.perm, d.row0, d.nz0, d.split_row};
+}
+
+// Host form of one orientation.
+struct HostDir {
+  std::vector<int32_t> ptr, row_of, cols, perm, row0, nz0, split_row;
+  int32_t L = 0, n_chunks = 0;
+};
+
+// Units of a chunk: enough chunks to give every SM some 48 warps' worth, 64 to 512 units each.
+int32_t pattern_chunk_units(int64_t units);
+// Fill row_of, chunks and cut rows from ptr.
+void pattern_chunks(int32_t n, HostDir *d);
+
+// Restores the caller's current device on scope exit.
+struct DeviceGuard {
+  int before = -1;
+  cudaError_t err;
+  explicit DeviceGuard(int device) {
+    err = cudaGetDevice(&before);
+    if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+  }
+  ~DeviceGuard() {
+    if (before >= 0) cudaSetDevice(before);
+  }
+};
+
+}  // namespace dsp
+
+struct dsp_pattern {
+  int device = 0;
+  int sms = 0;
+  int flags = 0;
+  int64_t rows = 0, cols = 0, nnz = 0, max_row_len = 0;
+  dsp::PatternDir a;  // A
+  dsp::PatternDir t;  // A transposed (DSP_PATTERN_GRAD)
+  int64_t device_bytes = 0;
+  std::vector<void *> allocs;
+};

@@ -295,6 +295,94 @@ int dsp_spmm_csr_f32_noalloc(const int64_t *indptr, const int64_t *indices, cons
                              int64_t rows, int64_t cols, int64_t nnz, const float *B, int64_t ldb,
                              float *C, int64_t ldc, int N, int accumulate, void *stream);
 
+/* ---------------------------------------------------------------- sparse layers: pattern */
+/* Element types of the dense operands below (products and sums are fp32 in every case). */
+#define DSP_F32 0
+#define DSP_BF16 1
+#define DSP_F16 2
+
+/* A CSR matrix prepared on one device for dsp_spmm_act and dsp_attn: 32-bit ids, chunks of equal work (entries and row
+ * ends), and, on request, the transposed lists that the gradients need. The matrix's values are not kept: dsp_spmm_act
+ * takes them with each call (they may be trained), attention uses the pattern alone. Read-only after creation: any number
+ * of calls, streams, host threads and captured graphs may use one pattern at a time (each call brings its own
+ * workspace). Not in the reference. */
+typedef struct dsp_pattern dsp_pattern;
+#define DSP_PATTERN_GRAD 1      /* transposed lists, for dsp_spmm_act_grad and dsp_attn_grad          */
+#define DSP_PATTERN_ATTENTION 2 /* for dsp_attn: refuses a row that lists a column twice (FORMAT)     */
+
+typedef struct dsp_pattern_info {
+  int64_t rows, cols, nnz;
+  int64_t flags;
+  int64_t chunk_units;  /* entries + row ends of a work chunk                    */
+  int64_t chunks;
+  int64_t split_rows;   /* rows cut across chunks                                 */
+  int64_t max_row_len;
+  int64_t device_bytes; /* all device memory the pattern holds                    */
+} dsp_pattern_info;
+
+/* rows, cols and nnz < 2^31 - 1 (UNSUPPORTED otherwise); the matrix is validated (FORMAT). Synchronous. Columns need no
+ * order; columns listed twice in a row add up in dsp_spmm_act. a->values may be NULL. */
+int dsp_pattern_create(int device, const dsp_csr *a, int flags, dsp_pattern **out);
+/* No call that uses the pattern may still be running on the device. */
+void dsp_pattern_destroy(dsp_pattern *p);
+int dsp_pattern_info_get(const dsp_pattern *p, dsp_pattern_info *info);
+
+/* ---------------------------------------------------------------- sparse layers: product with an epilogue */
+#define DSP_ACT_NONE 0
+#define DSP_ACT_RELU 1
+#define DSP_ACT_SILU 2
+#define DSP_ACT_GELU 3 /* z * Phi(z), the erf form */
+
+/* out = act(A*B + bias) + residual, row by row:
+ *   values    [nnz] fp32, device, in A's CSR order
+ *   B         cols x N, dtype, leading dimension ldb (elements)
+ *   bias      [N] fp32, or NULL
+ *   residual  rows x N, dtype, ldr, or NULL; may be `out` itself (the same address and ldr = ldo)
+ *   out       rows x N, dtype, ldo; no overlap with B. Rows of A without entries give act(bias) + residual.
+ *   pre       rows x N fp32, ldp, or NULL: receives z = A*B + bias, which dsp_spmm_act_grad needs unless act is NONE
+ * workspace: device memory of at least dsp_spmm_act_workspace(p, N) bytes, 256-byte aligned, not shared by calls that
+ * may overlap. Enqueued on `stream`, on the pattern's device, whatever the current device is; results do not depend on
+ * timing (no atomics). */
+typedef struct dsp_act_desc {
+  int dtype, act, N;
+  const float *values;
+  const void *B;
+  int64_t ldb;
+  const float *bias;
+  const void *residual;
+  int64_t ldr;
+  void *out;
+  int64_t ldo;
+  float *pre;
+  int64_t ldp;
+} dsp_act_desc;
+int64_t dsp_spmm_act_workspace(const dsp_pattern *p, int N);
+int dsp_spmm_act(const dsp_pattern *p, const dsp_act_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Gradients of dsp_spmm_act for the gradient `dout` (rows x N, dtype, lddo) of `out`; each result may be NULL:
+ *   dB       cols x N, dtype, lddb: every row is written (0 where a column has no entry)
+ *   dvalues  [nnz] fp32, A's CSR order
+ *   dbias    [N] fp32
+ * The residual's gradient is dout itself. pre: as written by dsp_spmm_act (may be NULL for DSP_ACT_NONE). Needs a pattern
+ * with DSP_PATTERN_GRAD when dB is given (STATE otherwise). dtype, act, N, values, B, ldb, pre, ldp as in the forward. */
+typedef struct dsp_act_grad_desc {
+  int dtype, act, N;
+  const float *values;
+  const void *B;
+  int64_t ldb;
+  const float *pre;
+  int64_t ldp;
+  const void *dout;
+  int64_t lddo;
+  void *dB;
+  int64_t lddb;
+  float *dvalues;
+  float *dbias;
+} dsp_act_grad_desc;
+int64_t dsp_spmm_act_grad_workspace(const dsp_pattern *p, const dsp_act_grad_desc *d);
+int dsp_spmm_act_grad(const dsp_pattern *p, const dsp_act_grad_desc *d, void *workspace, int64_t workspace_bytes,
+                      void *stream);
+
 /* ---------------------------------------------------------------- distributed rank */
 /* One GPU's share of the distributed SpMM: the local rows of A cut into segments by the
  * owner of each column tile (own tiles first, then peers in ring order (me+k)%P as in
