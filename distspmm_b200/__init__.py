@@ -4,8 +4,9 @@ Layers
   include/distspmm.h        C ABI (the drop-in boundary)
   libdistspmm_b200.so       native library: loader, planner, sm_100a kernels, rank runtime
   bin/dist_spmm_node        reference-compatible CLI
-  pattern / act             sparse layers on one GPU: the product with bias, activation and
-                            residual, with gradients
+  pattern / act / attention sparse layers on one GPU: the product with bias, activation and
+                            residual, attention masked by a matrix's entries (with gradients),
+                            and attention of single tokens over a cache
   matrix / planner / spmm / dist   Python face of the C ABI (ctypes; torch only supplies
                             device memory, streams and torch.distributed)
   comm_test / fit_comm_model       the bulk-vs-sparse fetch microbenchmark and the
@@ -33,6 +34,9 @@ def __getattr__(name):
     if name in ("spmm_act", "spmm_act_forward", "spmm_act_backward"):
         from . import act
         return getattr(act, name)
+    if name in ("sparse_attention", "sparse_attention_forward", "sparse_attention_backward", "sparse_attention_decode"):
+        from . import attention
+        return getattr(attention, name)
     if name in ("Rank", "build_local_group", "TorchComm", "distributed_plan", "connect_peers", "make_rank",
                 "global_plan", "fetch_view"):
         from . import dist

@@ -83,6 +83,22 @@ class dsp_act_grad_desc(ctypes.Structure):
                 ("dvalues", c_vp), ("dbias", c_vp)]
 
 
+class dsp_attn_desc(ctypes.Structure):
+    _fields_ = [("dtype", c_int), ("heads", c_int), ("kv_heads", c_int), ("dim", c_int), ("scale", c_f32),
+                ("softcap", c_f32), ("slopes", c_vp), ("row_offset", c_i64)] + [
+        f for x in ("q", "k", "v", "out") for f in ((x, c_vp), (x + "_row", c_i64), (x + "_head", c_i64))] + [("lse", c_vp)]
+
+
+class dsp_attn_grad_desc(ctypes.Structure):
+    _fields_ = [("fwd", dsp_attn_desc)] + [
+        f for x in ("dout", "dq", "dk", "dv") for f in ((x, c_vp), (x + "_row", c_i64), (x + "_head", c_i64))]
+
+
+class dsp_attn_decode_desc(ctypes.Structure):
+    _fields_ = [("fwd", dsp_attn_desc), ("rows", c_i64), ("nnz", c_i64), ("keys", c_i64), ("indptr", c_vp),
+                ("indices", c_vp)]
+
+
 class dsp_args(ctypes.Structure):
     _fields_ = [("file", ctypes.c_char_p), ("matrix", P(dsp_csr)), ("dims", c_int), ("task_dist", c_int),
                 ("comm_type", c_int), ("n_rolls", c_int), ("repeat", c_int), ("n_streams", c_int),
@@ -149,6 +165,12 @@ PROTOTYPES = {
     "dsp_spmm_act": (c_int, [c_vp, P(dsp_act_desc), c_vp, c_i64, c_vp]),
     "dsp_spmm_act_grad_workspace": (c_i64, [c_vp, P(dsp_act_grad_desc)]),
     "dsp_spmm_act_grad": (c_int, [c_vp, P(dsp_act_grad_desc), c_vp, c_i64, c_vp]),
+    "dsp_attn_workspace": (c_i64, [c_vp, P(dsp_attn_desc)]),
+    "dsp_attn": (c_int, [c_vp, P(dsp_attn_desc), c_vp, c_i64, c_vp]),
+    "dsp_attn_grad_workspace": (c_i64, [c_vp, P(dsp_attn_desc)]),
+    "dsp_attn_grad": (c_int, [c_vp, P(dsp_attn_grad_desc), c_vp, c_i64, c_vp]),
+    "dsp_attn_decode_workspace": (c_i64, [P(dsp_attn_decode_desc)]),
+    "dsp_attn_decode": (c_int, [P(dsp_attn_decode_desc), c_vp, c_i64, c_vp]),
     "dsp_rank_create": (c_int, [P(dsp_rank_desc), P(c_vp)]),
     "dsp_rank_destroy": (None, [c_vp]),
     "dsp_rank_stats_get": (c_int, [c_vp, P(dsp_rank_stats)]),

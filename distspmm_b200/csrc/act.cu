@@ -52,27 +52,32 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   return 1.f;
 }
 
-// The epilogue of VE columns of one row: sum -> z -> pre, out.
+// The epilogue of VE columns of one row: sum -> z -> pre, out. r: the residual's vector (zero where there is none).
 template <class T, int VE>
-__device__ __forceinline__ void finish(const ActArgs &a, int64_t row, int col, float (&z)[VE], const float (&bias)[VE]) {
+__device__ __forceinline__ void finish(const ActArgs &a, int64_t row, int col, float (&z)[VE], const float (&bias)[VE],
+                                       typename RowVec<T, VE>::Raw res) {
   using V = RowVec<T, VE>;
 #pragma unroll
   for (int i = 0; i < VE; ++i) z[i] += bias[i];
   if (a.pre) st_f32<VE>(a.pre + row * a.ldp + col, z);
-  float r[VE];
-  if (a.residual) V::widen(V::ld((const T *)a.residual + row * a.ldr + col), r);
+  if (a.act != DSP_ACT_NONE) {
 #pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    z[i] = act_of(z[i], a.act);
-    if (a.residual) z[i] += r[i];
+    for (int i = 0; i < VE; ++i) z[i] = act_of(z[i], a.act);
+  }
+  if (a.residual) {
+    float r[VE];
+    V::widen(res, r);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) z[i] += r[i];
   }
   V::st_stream((T *)a.out + row * a.ldo + col, z);
 }
 
 // One chunk per group of LPR lanes, walked in steps of U entries: the U rows of B are requested together, whatever rows of A
-// they belong to, then added to the running row; a finished row goes through the epilogue, a cut one to its slot.
-template <class T, int VE, int LPR, int VPL, int U, bool PERM>
-__global__ void __launch_bounds__(kThreads) act_product_kernel(const DirView d, const ActArgs a) {
+// they belong to, then added to the running row; a finished row goes through the epilogue, a cut one to its slot. The
+// residual of the running row is requested when the row begins, so that a row's end does not wait for it.
+template <class T, int VE, int LPR, int VPL, int U, int MINB, bool PERM>
+__global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirView d, const ActArgs a) {
   using V = RowVec<T, VE>;
   const int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LPR;
   if (chunk >= d.n_chunks) return;
@@ -81,15 +86,27 @@ __global__ void __launch_bounds__(kThreads) act_product_kernel(const DirView d, 
   const int32_t p0 = __ldg(d.nz0 + chunk), p1 = __ldg(d.nz0 + chunk + 1);
   const bool head_cut = p0 > __ldg(d.ptr + r0);
   float acc[VPL][VE], bias[VPL][VE];
+  typename V::Raw res[VPL];
+  int32_t row = r0;
+  auto begin_row = [&]() {
 #pragma unroll
-  for (int w = 0; w < VPL; ++w)
+    for (int w = 0; w < VPL; ++w) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[w][i] = 0.f;
+      const int col = col0 + w * LPR * VE;
+      if (a.residual && row < r1 && col < a.N) res[w] = V::ld((const T *)a.residual + (int64_t)row * a.ldr + col);
+    }
+  };
+#pragma unroll
+  for (int w = 0; w < VPL; ++w) {
+    res[w] = V::zero();
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
       const int col = col0 + w * LPR * VE + i;
-      acc[w][i] = 0.f;
       bias[w][i] = a.bias && col < a.N ? __ldg(a.bias + col) : 0.f;
     }
-  int32_t row = r0;
+  }
+  begin_row();
   auto store_slot = [&](int64_t slot) {
 #pragma unroll
     for (int w = 0; w < VPL; ++w) {
@@ -97,94 +114,121 @@ __global__ void __launch_bounds__(kThreads) act_product_kernel(const DirView d, 
       if (col < a.N) st_f32<VE>(a.slots + slot * a.N + col, acc[w]);
     }
   };
-  auto end_row = [&]() {  // the row's last unit is in this chunk
-    if (row == r0 && head_cut) {
-      store_slot(2 * chunk);
-    } else {
+  auto end_rows = [&](int32_t to) {  // rows row .. to - 1 end in this chunk
+#pragma unroll 1
+    while (row < to) {
+      if (row == r0 && head_cut) {
+        store_slot(2 * chunk);
+        ++row;
+        begin_row();
+        continue;
+      }
+      typename V::Raw now[VPL];
+      float z[VPL][VE];
+#pragma unroll
+      for (int w = 0; w < VPL; ++w) {
+        now[w] = res[w];
+#pragma unroll
+        for (int i = 0; i < VE; ++i) z[w][i] = acc[w][i];
+      }
+      const int64_t at = row++;
+      begin_row();
 #pragma unroll
       for (int w = 0; w < VPL; ++w) {
         const int col = col0 + w * LPR * VE;
-        if (col < a.N) finish<T, VE>(a, row, col, acc[w], bias[w]);
+        if (col < a.N) finish<T, VE>(a, at, col, z[w], bias[w], now[w]);
       }
     }
-    ++row;
-#pragma unroll
-    for (int w = 0; w < VPL; ++w)
-#pragma unroll
-      for (int i = 0; i < VE; ++i) acc[w][i] = 0.f;
   };
   const T *B = (const T *)a.B + col0;
-  auto add = [&](float v, const typename V::Raw(&b)[VPL]) {
-#pragma unroll
-    for (int w = 0; w < VPL; ++w) {
-      float f[VE];
-      V::widen(b[w], f);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) acc[w][i] = fmaf(v, f[i], acc[w][i]);
-    }
-  };
-  auto fetch = [&](int32_t c, typename V::Raw(&b)[VPL]) {
-    const T *src = B + (int64_t)c * a.ldb;
-#pragma unroll
-    for (int w = 0; w < VPL; ++w) b[w] = col0 + w * LPR * VE < a.N ? V::ldg(src + w * LPR * VE) : V::zero();
-  };
-  auto one = [&](int32_t p) {
-    typename V::Raw b[VPL];
-    fetch(__ldg(d.cols + p), b);
-    const float v = __ldg(a.values + (PERM ? __ldg(d.perm + p) : p));
-    const int32_t r = __ldg(d.row_of + p);
-    while (row < r) end_row();
-    add(v, b);
-  };
-  int32_t p = p0;
-  for (; p < p1 && (p & 3); ++p) one(p);
-  for (; p + U <= p1; p += U) {  // p is a multiple of 4 here: ids and values come four to a load
-    int32_t c[U], r[U];
+  // entries come in aligned groups of 4 (the id lists are padded); those outside [p0, p1) are masked
+#pragma unroll 1
+  for (int32_t p = p0 & ~3; p < p1; p += U) {
+    int32_t c[U];
     float v[U];
 #pragma unroll
     for (int q = 0; q < U / 4; ++q) {
       const int4 c4 = __ldg(reinterpret_cast<const int4 *>(d.cols + p) + q);
-      const int4 r4 = __ldg(reinterpret_cast<const int4 *>(d.row_of + p) + q);
       c[4 * q] = c4.x, c[4 * q + 1] = c4.y, c[4 * q + 2] = c4.z, c[4 * q + 3] = c4.w;
-      r[4 * q] = r4.x, r[4 * q + 1] = r4.y, r[4 * q + 2] = r4.z, r[4 * q + 3] = r4.w;
-      if (PERM) {
-        const int4 x = __ldg(reinterpret_cast<const int4 *>(d.perm + p) + q);
-        v[4 * q] = __ldg(a.values + x.x), v[4 * q + 1] = __ldg(a.values + x.y);
-        v[4 * q + 2] = __ldg(a.values + x.z), v[4 * q + 3] = __ldg(a.values + x.w);
-      } else {
+    }
+    const bool whole = p >= p0 && p + U <= p1;
+    const int32_t last = __ldg(d.row_of + (p + U <= p1 ? p + U : p1) - 1);
+    if (PERM) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * q + i] = __ldg(a.values + p + 4 * q + i);
+      for (int q = 0; q < U / 4; ++q) {
+        const int4 x = __ldg(reinterpret_cast<const int4 *>(d.perm + p) + q);
+        const int32_t at = p + 4 * q;
+        v[4 * q] = at >= p0 && at < p1 ? __ldg(a.values + x.x) : 0.f;
+        v[4 * q + 1] = at + 1 >= p0 && at + 1 < p1 ? __ldg(a.values + x.y) : 0.f;
+        v[4 * q + 2] = at + 2 >= p0 && at + 2 < p1 ? __ldg(a.values + x.z) : 0.f;
+        v[4 * q + 3] = at + 3 >= p0 && at + 3 < p1 ? __ldg(a.values + x.w) : 0.f;
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = p + u >= p0 && p + u < p1 ? __ldg(a.values + p + u) : 0.f;
     }
     typename V::Raw b[U][VPL];
 #pragma unroll
-    for (int u = 0; u < U; ++u) fetch(c[u], b[u]);
-    if (r[U - 1] == row) {  // rows are in order: the whole step belongs to the running row
+    for (int u = 0; u < U; ++u) {
+      const bool in = whole || (p + u >= p0 && p + u < p1);
+      const T *src = B + (int64_t)c[u] * a.ldb;
 #pragma unroll
-      for (int u = 0; u < U; ++u) add(v[u], b[u]);
+      for (int w = 0; w < VPL; ++w) b[u][w] = in && col0 + w * LPR * VE < a.N ? V::ldg(src + w * LPR * VE) : V::zero();
+    }
+    auto add = [&](int u) {
+#pragma unroll
+      for (int w = 0; w < VPL; ++w) {
+        float f[VE];
+        V::widen(b[u][w], f);
+#pragma unroll
+        for (int i = 0; i < VE; ++i) acc[w][i] = fmaf(v[u], f[i], acc[w][i]);
+      }
+    };
+    if (whole && last == row) {  // rows are in order: the whole step belongs to the running row
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(u);
     } else {
+      int32_t r[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        while (row < r[u]) end_row();
-        add(v[u], b[u]);
+      for (int u = 0; u < U; ++u) r[u] = p + u < p0 ? -1 : p + u < p1 ? __ldg(d.row_of + p + u) : INT32_MAX;
+#pragma unroll 1
+      while (true) {
+        int32_t next = last;  // the first listed row after the running one
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (r[u] == row) add(u);
+          if (r[u] > row) next = min(next, r[u]);
+        }
+        if (row >= last) break;
+        end_rows(next);
       }
     }
   }
-  for (; p < p1; ++p) one(p);
-  while (row < r1) end_row();
+  end_rows(r1);
   if (p1 > max(p0, __ldg(d.ptr + r1))) store_slot(r1 == r0 && head_cut ? 2 * chunk : 2 * chunk + 1);
 }
 
-// Rows cut across chunks: their partials, added in chunk order (eight interleaved sums, then those eight in order), go
-// through the epilogue. One block per cut row and 128 columns.
+// Rows cut across chunks: their partials go through the epilogue, added in chunk order: by one warp where there are few, in
+// eight interleaved sums and then those eight in order where there are many (the first n_long of the list, a block each).
 template <class T>
 __global__ void __launch_bounds__(kThreads) act_join_kernel(const DirView d, const ActArgs a) {
   __shared__ float part[8][128];
-  const int32_t r = __ldg(d.split_row + blockIdx.x);
-  const int64_t c0 = ((int64_t)r + __ldg(d.ptr + r)) / d.L, c1 = ((int64_t)r + __ldg(d.ptr + r + 1)) / d.L;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool wide = (int)blockIdx.x < d.n_long;
+  const int32_t at = wide ? (int)blockIdx.x : d.n_long + ((int)blockIdx.x - d.n_long) * 8 + warp;
+  if (at >= d.n_split) return;  // whole warps of a narrow block: no barrier there
+  const int32_t r = __ldg(d.split_row + at);
+  const int64_t c0 = row_start(r, __ldg(d.ptr + r)) / d.L, c1 = row_start(r, __ldg(d.ptr + r + 1)) / d.L;
   float s[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t c = c0 + warp; c <= c1; c += 8) {
+  typename RowVec<T, 1>::Raw res[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int col = blockIdx.y * 128 + lane + 32 * k;
+    res[k] = RowVec<T, 1>::zero();
+    if (a.residual && col < a.N) res[k] = RowVec<T, 1>::ld((const T *)a.residual + (int64_t)r * a.ldr + col);
+  }
+#pragma unroll 4
+  for (int64_t c = c0 + (wide ? warp : 0); c <= c1; c += wide ? 8 : 1) {
     const float *src = a.slots + (c == c0 ? 2 * c + 1 : 2 * c) * a.N;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -192,15 +236,25 @@ __global__ void __launch_bounds__(kThreads) act_join_kernel(const DirView d, con
       if (col < a.N) s[k] += src[col];
     }
   }
+  if (wide) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) part[warp][lane + 32 * k] = s[k];
-  __syncthreads();
-  const int col = blockIdx.y * 128 + threadIdx.x;
-  if (threadIdx.x < 128 && col < a.N) {
-    float z[1] = {0.f}, b[1] = {a.bias ? __ldg(a.bias + col) : 0.f};
+    for (int k = 0; k < 4; ++k) part[warp][lane + 32 * k] = s[k];
+    __syncthreads();
+    if (warp > 0) return;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) z[0] += part[w][threadIdx.x];
-    finish<T, 1>(a, r, col, z, b);
+    for (int k = 0; k < 4; ++k) {
+      s[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) s[k] += part[w][lane + 32 * k];
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int col = blockIdx.y * 128 + lane + 32 * k;
+    if (col < a.N) {
+      float z[1] = {s[k]}, b[1] = {a.bias ? __ldg(a.bias + col) : 0.f};
+      finish<T, 1>(a, r, col, z, b, res[k]);
+    }
   }
 }
 
@@ -384,10 +438,15 @@ Shape shape_of(int N, int ve, int size) {
 
 template <class T, int VE, int LPR, int VPL, bool PERM>
 void run_product(const DirView &d, const ActArgs &a, cudaStream_t s) {
-  constexpr int U = VE * VPL >= 8 ? 4 : 8;
+#ifndef ACT_U
+#define ACT_U 4
+#define ACT_B 4
+#endif
+  constexpr int U = VE * VPL >= 8 ? 4 : ACT_U;
   const dim3 grid((unsigned)(((int64_t)d.n_chunks * LPR + kThreads - 1) / kThreads),
                   (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL)));
-  act_product_kernel<T, VE, LPR, VPL, U, PERM><<<grid, kThreads, 0, s>>>(d, a);
+  constexpr int minb = VE * VPL >= 16 ? 2 : VE * VPL == 8 ? ACT_B - 1 : ACT_B;
+  act_product_kernel<T, VE, LPR, VPL, U, minb, PERM><<<grid, kThreads, 0, s>>>(d, a);
 }
 
 template <class T, bool PERM>
@@ -409,7 +468,8 @@ int product(const DirView &d, const ActArgs &a, bool transposed, int ve, cudaStr
     if (transposed) pick_product<T, true>(h, d, a, s);
     else pick_product<T, false>(h, d, a, s);
   }
-  if (d.n_split > 0) act_join_kernel<T><<<dim3((unsigned)d.n_split, (unsigned)((a.N + 127) / 128)), kThreads, 0, s>>>(d, a);
+  if (d.n_split > 0)
+    act_join_kernel<T><<<dim3((unsigned)join_blocks(d), (unsigned)((a.N + 127) / 128)), kThreads, 0, s>>>(d, a);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_spmm_act: %s", cudaGetErrorString(e));
 }

@@ -1,0 +1,47 @@
+// attn.h — arguments shared by the attention kernels.
+#pragma once
+#include "pattern.h"
+
+namespace dsp {
+
+// Strides are in elements; a head's dim values are contiguous.
+struct Heads {
+  const void *p;
+  int64_t row, head;
+};
+struct HeadsOut {
+  void *p;
+  int64_t row, head;
+};
+
+struct AttnArgs {
+  int heads, group, dim;  // group: query heads of one key/value head
+  float scale, cap;       // cap = 0: none
+  const float *slopes;    // [heads] or nullptr
+  int64_t row_offset;
+  Heads q, k, v, dout, o;
+  HeadsOut out, dq, dk, dv;
+  float *lse;        // [rows][heads]
+  float *delta;      // [rows][heads] dout . out
+  float *slots;      // partials of cut rows: [2 n_chunks][heads][width]
+  float *slot_ml;    // [2 n_chunks][heads][2] running maximum and sum (forward)
+};
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// cap tanh(s / cap) through one exponential: tanh x = 1 - 2 / (e^2x + 1), which is within 2^-22 absolutely for every x
+// (tanh.approx is within 2^-11 of the value: a cap of 50 would shift scores by 0.02). th: tanh itself, for the gradient.
+__device__ __forceinline__ float capped(float s, float cap, float inv_cap2, float &th) {
+  th = 1.f - __fdividef(2.f, exp2_approx(s * inv_cap2) + 1.f);  // 2 / inf = 0
+  return cap * th;
+}
+
+int check_attn(const char *who, const dsp_attn_desc *d, int64_t rows, int64_t keys);
+
+}  // namespace dsp

@@ -8,15 +8,16 @@
 
 namespace dsp {
 
-int32_t pattern_chunk_units(int64_t units) {
-  int64_t l = (units + 148 * 48 - 1) / (148 * 48);
+// Units of a chunk: enough chunks for some 32 warps on every SM, 64 to 512 units each.
+static int32_t chunk_units(int64_t units) {
+  int64_t l = (units + 148 * 32 - 1) / (148 * 32);
   l = (l + 31) / 32 * 32;
   return (int32_t)std::min<int64_t>(512, std::max<int64_t>(64, l));
 }
 
 void pattern_chunks(int32_t n, HostDir *d) {
-  const int64_t nnz = d->ptr[n], units = n + nnz;
-  d->L = pattern_chunk_units(units);
+  const int64_t nnz = d->ptr[n], units = row_start(n, nnz);
+  d->L = chunk_units(units);
   d->n_chunks = (int32_t)((units + d->L - 1) / d->L);
   d->row_of.resize(nnz);
   d->row0.resize(d->n_chunks + 1);
@@ -28,20 +29,25 @@ void pattern_chunks(int32_t n, HostDir *d) {
   parallel_for(d->n_chunks + 1, [&](int64_t b, int64_t e) {
     for (int64_t c = b; c < e; ++c) {
       const int64_t x = std::min<int64_t>(c * d->L, units);
-      // rows ended before unit x: the row r whose units r + ptr[r] .. r + ptr[r+1] hold x
-      int64_t lo = 0, hi = n;
+      int64_t lo = 0, hi = n;  // the first row whose end is at x or behind
       while (lo < hi) {
         const int64_t m = (lo + hi) / 2;
-        if (m + d->ptr[m + 1] < x) lo = m + 1;
+        if (row_start(m, d->ptr[m + 1]) < x) lo = m + 1;
         else hi = m;
       }
       d->row0[c] = (int32_t)lo;
-      d->nz0[c] = (int32_t)(x - lo);
+      d->nz0[c] = (int32_t)std::max<int64_t>(x - row_start(lo, 0), d->ptr[lo]);  // x may lie inside the end of row lo - 1
     }
   });
   d->split_row.clear();
-  for (int32_t r = 0; r < n; ++r)
-    if (((int64_t)r + d->ptr[r]) / d->L != ((int64_t)r + d->ptr[r + 1]) / d->L) d->split_row.push_back(r);
+  std::vector<int32_t> few;
+  for (int32_t r = 0; r < n; ++r) {
+    const int64_t cuts = row_start(r, d->ptr[r + 1]) / d->L - row_start(r, d->ptr[r]) / d->L;
+    if (cuts > kLongSlots) d->split_row.push_back(r);
+    else if (cuts > 0) few.push_back(r);
+  }
+  d->n_long = (int32_t)d->split_row.size();
+  d->split_row.insert(d->split_row.end(), few.begin(), few.end());
 }
 
 namespace {
@@ -49,7 +55,7 @@ namespace {
 template <class V>
 int put(dsp_pattern *p, const std::vector<V> &h, V **out) {
   *out = nullptr;
-  const size_t bytes = std::max<size_t>(h.size(), 1) * sizeof(V) + 16;  // vector loads may read past the last entry
+  const size_t bytes = std::max<size_t>(h.size(), 1) * sizeof(V) + 64;  // id lists are read in aligned steps of up to 8
   void *d = nullptr;
   cudaError_t e = cudaMalloc(&d, bytes);
   if (e != cudaSuccess) {
@@ -69,6 +75,7 @@ int put_dir(dsp_pattern *p, int32_t n, const HostDir &h, PatternDir *d) {
   d->L = h.L;
   d->n_chunks = h.n_chunks;
   d->n_split = (int32_t)h.split_row.size();
+  d->n_long = h.n_long;
   int rc;
   if ((rc = put(p, h.ptr, &d->ptr)) || (rc = put(p, h.row_of, &d->row_of)) || (rc = put(p, h.cols, &d->cols)) ||
       (rc = put(p, h.row0, &d->row0)) || (rc = put(p, h.nz0, &d->nz0)) || (rc = put(p, h.split_row, &d->split_row)))

@@ -11,17 +11,22 @@ namespace dsp {
 
 // One orientation of the pattern (A, or A transposed), with its balanced work chunks.
 //
-// The work of one orientation is a path of n + nnz units: the entries of row 0, the end of row 0, the entries of row 1,
-// its end, ... (merge path). Chunk c holds the units [c L, (c + 1) L): the row ends row0[c] .. row0[c+1] - 1 and the
-// entries nz0[c] .. nz0[c+1] - 1, so rows of any length and rows without entries cost the same for the same number of
-// units. Row r spans the units r + ptr[r] .. r + ptr[r+1]; it is cut when these lie in different chunks, and then leaves
-// one partial in each of them: in slot 2c + 1 of the chunk it starts in, in slot 2c of every later one. The list of
-// cut rows is split_row.
+// The work of one orientation is a path of units: the entries of row 0 (a unit each), the end of row 0 (kRowUnits units: it
+// costs an epilogue, not a gathered row), the entries of row 1, its end, ... (merge path). Chunk c holds what begins in the
+// units [c L, (c + 1) L): the row ends row0[c] .. row0[c+1] - 1 and the entries nz0[c] .. nz0[c+1] - 1, so rows of any length
+// and runs of rows without entries are spread evenly. Row r begins at row_start(r, ptr[r]) and its end is at
+// row_start(r, ptr[r+1]); it is cut when these lie in different chunks, and then leaves one partial in each of them: in slot
+// 2c + 1 of the chunk it starts in, in slot 2c of every later one. split_row lists the cut rows, those of more than
+// kLongSlots partials first (n_long of them).
+constexpr int kRowUnits = 8;
+constexpr int kLongSlots = 16;
+DSP_HD int64_t row_start(int64_t r, int64_t p) { return r * kRowUnits + p; }
+
 struct PatternDir {
   int32_t n = 0;          // rows of this orientation
   int32_t n_chunks = 0;
   int32_t L = 0;          // units of a chunk
-  int32_t n_split = 0;
+  int32_t n_split = 0, n_long = 0;
   int32_t *ptr = nullptr;        // [n + 1]
   int32_t *row_of = nullptr;     // [nnz]
   int32_t *cols = nullptr;       // [nnz]
@@ -33,22 +38,23 @@ struct PatternDir {
 
 // Kernel-side view (passed by value).
 struct DirView {
-  int32_t n, n_chunks, L, n_split;
+  int32_t n, n_chunks, L, n_split, n_long;
   const int32_t *ptr, *row_of, *cols, *perm, *row0, *nz0, *split_row;
 };
 
 inline DirView view(const PatternDir &d) {
-  return {d.n, d.n_chunks, d.L, d.n_split, d.ptr, d.row_of, d.cols, d.perm, d.row0, d.nz0, d.split_row};
+  return {d.n, d.n_chunks, d.L, d.n_split, d.n_long, d.ptr, d.row_of, d.cols, d.perm, d.row0, d.nz0, d.split_row};
 }
+
+// Blocks of 8 warps that join the cut rows: a block for each long one, a warp for each other.
+inline int64_t join_blocks(const DirView &d) { return d.n_long + (d.n_split - d.n_long + 7) / 8; }
 
 // Host form of one orientation.
 struct HostDir {
   std::vector<int32_t> ptr, row_of, cols, perm, row0, nz0, split_row;
-  int32_t L = 0, n_chunks = 0;
+  int32_t L = 0, n_chunks = 0, n_long = 0;
 };
 
-// Units of a chunk: enough chunks to give every SM some 48 warps' worth, 64 to 512 units each.
-int32_t pattern_chunk_units(int64_t units);
 // Fill row_of, chunks and cut rows from ptr.
 void pattern_chunks(int32_t n, HostDir *d);
 

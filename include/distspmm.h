@@ -383,6 +383,67 @@ int64_t dsp_spmm_act_grad_workspace(const dsp_pattern *p, const dsp_act_grad_des
 int dsp_spmm_act_grad(const dsp_pattern *p, const dsp_act_grad_desc *d, void *workspace, int64_t workspace_bytes,
                       void *stream);
 
+/* ---------------------------------------------------------------- sparse layers: attention */
+/* Attention whose mask is a pattern: query row i attends to the key rows j that row i of A lists (sliding window, packed
+ * documents, prefix, the edges of a graph), for each query head h (key/value head h / (heads / kv_heads)):
+ *   u_ij = softcap * tanh(scale * q_i.k_j / softcap) - slopes[h] * |i + row_offset - j|
+ *   out_i = sum_j exp(u_ij - lse_i) v_j,   lse_i = log sum_j exp(u_ij)   (natural logarithm)
+ * softcap = 0: no cap. slopes [heads] fp32 (device) or NULL: no distance bias. row_offset: the position of row 0 (a rank's
+ * first row, say). Rows without entries give out = 0, lse = -infinity. Entries that A does not list are not part of a row,
+ * whatever k and v hold there.
+ * q, out: rows x heads x dim; k, v: cols x kv_heads x dim; dtype; strides in elements (row, head), dim contiguous; addresses
+ * and strides multiples of 16 bytes (INVALID otherwise). dim: a multiple of 8 up to 256 (UNSUPPORTED otherwise). lse: rows x
+ * heads fp32, contiguous, or NULL. No output may overlap an input. Workspace, device, stream and order of sums as for
+ * dsp_spmm_act. The pattern needs DSP_PATTERN_ATTENTION, for gradients DSP_PATTERN_GRAD too (STATE otherwise). */
+typedef struct dsp_attn_desc {
+  int dtype, heads, kv_heads, dim;
+  float scale, softcap;
+  const float *slopes;
+  int64_t row_offset;
+  const void *q;
+  int64_t q_row, q_head;
+  const void *k;
+  int64_t k_row, k_head;
+  const void *v;
+  int64_t v_row, v_head;
+  void *out;
+  int64_t out_row, out_head;
+  float *lse;
+} dsp_attn_desc;
+int64_t dsp_attn_workspace(const dsp_pattern *p, const dsp_attn_desc *d);
+int dsp_attn(const dsp_pattern *p, const dsp_attn_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* dq, dk, dv for the gradient `dout` of `out`; fwd: the forward's operands, with the out and lse that it wrote (read only
+ * here). Every row is written (0 where a row or column has no entry). slopes are constants: no gradient. */
+typedef struct dsp_attn_grad_desc {
+  dsp_attn_desc fwd;
+  const void *dout;
+  int64_t dout_row, dout_head;
+  void *dq;
+  int64_t dq_row, dq_head;
+  void *dk;
+  int64_t dk_row, dk_head;
+  void *dv;
+  int64_t dv_row, dv_head;
+} dsp_attn_grad_desc;
+int64_t dsp_attn_grad_workspace(const dsp_pattern *p, const dsp_attn_desc *d);
+int dsp_attn_grad(const dsp_pattern *p, const dsp_attn_grad_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* The form for single query tokens over a cache, without a pattern: the mask is a CSR already in device memory (int64
+ * indptr[rows + 1] from 0 to nnz, int64 indices[nnz]), which may change with every call. Row r is the newest token of a
+ * sequence; indices[indptr[r] .. indptr[r+1]) are the rows of k and v (of `keys` rows) that hold its tokens, oldest first: a
+ * page table with pages of one row. Entry t of n is at distance n - 1 - t (for slopes); fwd.row_offset is not used. The
+ * lists are not validated on the host; an entry outside [0, keys) makes its row of out and lse NaN and nothing is read there.
+ * An entry listed twice counts twice. Runs on the current device. rows <= 2^24, nnz < 2^31 - 1. */
+typedef struct dsp_attn_decode_desc {
+  dsp_attn_desc fwd; /* q, out: rows x heads x dim; k, v: keys x kv_heads x dim */
+  int64_t rows, nnz, keys;
+  const int64_t *indptr;
+  const int64_t *indices;
+} dsp_attn_decode_desc;
+int64_t dsp_attn_decode_workspace(const dsp_attn_decode_desc *d);
+int dsp_attn_decode(const dsp_attn_decode_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
+
 /* ---------------------------------------------------------------- distributed rank */
 /* One GPU's share of the distributed SpMM: the local rows of A cut into segments by the
  * owner of each column tile (own tiles first, then peers in ring order (me+k)%P as in

@@ -49,3 +49,33 @@ def test_python_refuses_what_is_no_pattern():
         d.spmm_act("A", torch.ones(2, 2))
     with pytest.raises(ValueError, match="act must be"):
         d.spmm_act_forward("A", torch.ones(2, 2), act="swish")
+
+
+def test_attention_null_arguments():
+    from distspmm_b200._lib import dsp_attn_decode_desc, dsp_attn_desc, dsp_attn_grad_desc
+    assert status("dsp_attn", None, ctypes.byref(dsp_attn_desc()), None, 0, None) == -1
+    assert status("dsp_attn_grad", None, ctypes.byref(dsp_attn_grad_desc()), None, 0, None) == -1
+    assert status("dsp_attn_decode", None, None, 0, None) == -1
+    assert d.lib().dsp_attn_workspace(None, None) == 0
+    assert d.lib().dsp_attn_grad_workspace(None, None) == 0
+    assert d.lib().dsp_attn_decode_workspace(None) == 0
+
+
+def decode_desc(**kw):
+    from distspmm_b200._lib import dsp_attn_decode_desc, dsp_attn_desc
+    f = dict(dtype=1, heads=4, kv_heads=2, dim=64, scale=0.125, softcap=0.0, slopes=None, row_offset=0, q=1 << 12, q_row=256, q_head=64,
+             k=1 << 13, k_row=128, k_head=64, v=1 << 14, v_row=128, v_head=64, out=1 << 15, out_row=256, out_head=64, lse=None)
+    g = dict(rows=1, nnz=5, keys=5, indptr=1 << 16, indices=1 << 17)
+    for k, v in kw.items():
+        (f if k in f else g)[k] = v
+    return dsp_attn_decode_desc(dsp_attn_desc(*f.values()), *g.values())
+
+
+@pytest.mark.parametrize("bad,code", [
+    (dict(dtype=3), -1), (dict(heads=0), -1), (dict(kv_heads=3), -1), (dict(kv_heads=0), -1), (dict(dim=0), -6), (dict(dim=20), -6),
+    (dict(dim=264), -6), (dict(softcap=-1.0), -1), (dict(softcap=float("inf")), -1), (dict(scale=float("nan")), -1), (dict(q=None), -1),
+    (dict(q=(1 << 12) + 2), -1), (dict(k_row=129), -1), (dict(out=None), -1), (dict(indptr=None), -1), (dict(indices=None), -1),
+    (dict(rows=-1), -1), (dict(nnz=-1), -1), (dict(rows=1 << 25), -6), (dict(nnz=1 << 31), -6), (dict(), -1)])
+def test_decode_refuses(bad, code):
+    """Bad arguments, and (last) a missing workspace: all refused before anything reaches a device."""
+    assert status("dsp_attn_decode", ctypes.byref(decode_desc(**bad)), None, 0, None) == code
