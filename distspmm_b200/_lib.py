@@ -68,7 +68,7 @@ class dsp_rank_stats(ctypes.Structure):
 
 class dsp_pattern_info(ctypes.Structure):
     _fields_ = [(n, c_i64) for n in ("rows", "cols", "nnz", "flags", "chunk_units", "chunks", "split_rows",
-                                     "max_row_len", "device_bytes")]
+                                     "max_row_len", "tiles", "device_bytes")]
 
 
 class dsp_act_desc(ctypes.Structure):
@@ -161,6 +161,7 @@ PROTOTYPES = {
     "dsp_pattern_create": (c_int, [c_int, P(dsp_csr), c_int, P(c_vp)]),
     "dsp_pattern_destroy": (None, [c_vp]),
     "dsp_pattern_info_get": (c_int, [c_vp, P(dsp_pattern_info)]),
+    "dsp_pattern_check_error": (c_int, [c_vp]),
     "dsp_spmm_act_workspace": (c_i64, [c_vp, c_int]),
     "dsp_spmm_act": (c_int, [c_vp, P(dsp_act_desc), c_vp, c_i64, c_vp]),
     "dsp_spmm_act_grad_workspace": (c_i64, [c_vp, P(dsp_act_grad_desc)]),

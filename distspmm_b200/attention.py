@@ -16,11 +16,11 @@ from .pattern import DTYPES, SparsePattern, need, on_device, ptr, workspace
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels can read it in place (dim contiguous, address and strides multiples of 16 bytes), else a
-    contiguous copy."""
+    """t itself where the kernels can read it in place (dim contiguous, address and strides multiples of 16 bytes, no axis
+    expanded), else a contiguous copy."""
     e = t.element_size()
     ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or (s * e) % 16 == 0 for n, s in zip(t.shape[:2], t.stride()[:2]))
+        n <= 1 or (s > 0 and (s * e) % 16 == 0) for n, s in zip(t.shape[:2], t.stride()[:2]))
     return t if ok else t.contiguous()
 
 

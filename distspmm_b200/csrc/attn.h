@@ -19,6 +19,7 @@ struct AttnArgs {
   float scale, cap;       // cap = 0: none
   const float *slopes;    // [heads] or nullptr
   int64_t row_offset;
+  int64_t n_queries;      // rows of q (tile form of dk, dv)
   Heads q, k, v, dout, o;
   HeadsOut out, dq, dk, dv;
   float *lse;        // [rows][heads]

@@ -1,0 +1,748 @@
+// attn_tile.cu — attention over the tile form of a pattern, on the 5th-generation tensor cores (bf16, fp16; dim 64 or 128).
+//
+// One kernel in three roles, each a stationary tile of 128 rows against a stream of tiles of 64 rows (the tiles the pattern
+// lists), with products of 128 x 64 x dim and 128 x dim x 64 per tile:
+//
+//             stationary   stream    first products            weights (16-bit, in tensor memory)   second products
+//   forward   Q            K, V      S = Q K^T                 P = exp(u - m)                       O += P V
+//   dq        Q, dO        K, V      S = Q K^T, R = dO V^T     dS = P (R - delta) c                 dQ += dS K
+//   dk, dv    K, V         Q, dO     S^T = K Q^T, R^T = V dO^T P^T, dS^T                            dV += P^T dO, dK += dS^T Q
+//
+// A CTA: four warps of weights (a thread owns one of the 128 rows: the running maximum, sum and all masks are its own
+// registers, no shuffles), one warp of TMA loads, one that issues the products. Scores arrive in tensor memory, weights go
+// back into the same columns as the A operand of the second product, so neither passes through shared memory; the stream's
+// tiles serve both products from one swizzled image (K-major in the first, N-major in the second). The sums over keys stay in
+// tensor memory; the forward pass rescales its own only when a row's maximum grew by more than 2^8 (kSlack), which leaves
+// the result the same (weights and their sum share the stale maximum).
+//
+// Rounding: weights enter the second product in the operands' 16-bit type (half a step each; the sum l is of unrounded
+// weights). fp16 has few exponents: weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is
+// scaled by a power of two that brings the largest |dout| near 16; both come off in the epilogue.
+//
+// Masks and values that are not finite: an entry that is not listed has weight 0, but 0 x NaN in the product is NaN. So a row
+// whose result is not finite is computed again by attn_row.cuh's gather, which reads listed entries only. A NaN that belongs
+// there stays, one that leaked in does not.
+//
+// Bounds: the first and second products of a tile take 128 x 64 x dim x 2 / 8192 cycles each on the tensor cores (256 for
+// dim 128), the exponentials 128 x 64 / 16 = 512 on the special function units, which bound the forward pass; two CTAs on an
+// SM overlap one's weights with the other's products. Measured figures are beside the launches at the end of the file.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_row.cuh"
+#include "attn_tile.h"
+#include "tcgen05.cuh"
+
+namespace dsp {
+namespace {
+
+enum Mode { kFwd, kDq, kDkv };
+constexpr int kThreads = 192, kWeightThreads = 128;
+constexpr float kSlack = 8.f;
+
+struct TileView {
+  const int32_t *ptr, *col, *mask, *order;
+  const uint64_t *words;
+};
+
+struct TileArgs {
+  TileView t;
+  AttnArgs a;
+  PlanRows rows;        // the gather form of the same orientation
+  int n_heads;          // heads of the grid (query heads, or key/value heads for dk, dv)
+  int splits;           // pieces of a row tile's list (forward)
+  float *part, *part_ml;  // their partial results: [splits][rows][heads][dim], [splits][rows][heads][2]
+  const uint32_t *dout_max;  // bits of the largest finite |dout| (fp16 gradients)
+  int *err;
+};
+
+template <int D, Mode M>
+struct Cfg {
+  static constexpr int kStatic = M == kFwd ? 1 : 2;            // stationary operands
+  static constexpr int kScores = M == kFwd ? 1 : 2;            // score tiles of 64 columns
+  static constexpr int NB = M == kFwd && D == 128 ? 2 : M != kFwd && D == 128 ? 2 : 1;  // score buffers
+  static constexpr int ST = 2;                                 // stages of each streamed operand
+  static constexpr int kAcc = kScores * NB * 64;               // first accumulator column
+  static constexpr int kUsed = kAcc + (M == kDkv ? 2 : 1) * D;
+  static constexpr int kCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+  static constexpr int kStaticBytes = 128 * D * 2, kStreamBytes = 64 * D * 2;
+  static constexpr int kSmemUsed = kStatic * kStaticBytes + 2 * ST * kStreamBytes + 1024;
+  // no more CTAs on an SM than tensor memory has room for: an allocation never waits for another CTA's end
+  static constexpr int kCtas = 512 / kCols;
+  static constexpr int kSmemLeast = 232448 / (kCtas + 1) + 1024;
+  static constexpr int kSmem = kSmemUsed > kSmemLeast ? kSmemUsed : kSmemLeast;
+};
+
+// Bounded wait; gives up at once where another thread of the CTA has.
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *dead, int *err, int code) {
+  const long long t0 = clock64();
+  while (true) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (*dead) return false;
+    if (clock64() - t0 > kMbarWaitCycles) {
+      *dead = 1;
+      atomicExch(err, code);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *dead, int *err, int code) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done ? true : wait_slow(bar, parity, dead, err, code);
+}
+
+// The same by a whole warp, which leaves it together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *dead, int *err, int code) {
+  return __all_sync(0xffffffffu, wait(bar, parity, dead, err, code));
+}
+
+// The last of n phases. When a thread has seen the last scores, the phase n - 3 is over, n - 2 perhaps not: a wait for n - 1
+// alone would take the parity of n - 3 for it.
+__device__ __forceinline__ bool wait_last(uint32_t bar, int n, volatile int *dead, int *err, int code) {
+  return (n < 2 || warp_wait(bar, n & 1, dead, err, code)) && warp_wait(bar, (n - 1) & 1, dead, err, code);
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&x);
+  } else {
+    const __half2 x = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&x);
+  }
+}
+
+// Rows of a warp whose result is not finite (bits of `bad`), again by gather.
+template <class T, int D, Mode M>
+__device__ __noinline__ void redo(const TileArgs &x, int64_t row0, int head, uint32_t bad) {
+  using H = HeadRow<T, 8, D / 8, 1>;
+  const int lane = threadIdx.x % (D / 8), g = (threadIdx.x & 31) / (D / 8);
+  while (bad) {
+    const int64_t row = row0 + __ffs(bad) - 1;
+    bad &= bad - 1;
+    const int64_t p = x.rows.ptr(row), pe = x.rows.ptr(row + 1);
+    float y[1][8], z[1][8], m, l;
+    if constexpr (M == kFwd) {
+      attend<H, D / 8>(x.rows, x.a, row, head, p, pe, pe, m, l, y);
+      put_row<H, D / 8>(x.a, row, head, m, l, y);
+    } else if constexpr (M == kDq) {
+      attend_dq<H, D / 8>(x.rows, x.a, row, head, p, pe, m, y, z);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[0][i] = (y[0][i] - m * z[0][i]) * x.a.scale;
+      if (g == 0) H::store(x.a.dq, row, head, lane, D, y);
+    } else {
+      attend_dkv<H, D / 8>(x.rows, x.a, row, head, p, pe, y, z);
+      if (g == 0) {
+        H::store(x.a.dk, row, head, lane, D, y);
+        H::store(x.a.dv, row, head, lane, D, z);
+      }
+    }
+  }
+}
+
+// D columns of this thread's row at `addr`, times f, to the row's place in global memory; whether all were finite.
+template <class T, int D>
+__device__ __forceinline__ bool put_acc(uint32_t addr, float f, const HeadsOut &o, int64_t row, int head, bool store) {
+  bool fine = true;
+  T *dst = (T *)o.p + row * o.row + (int64_t)head * o.head;
+#pragma unroll 1
+  for (int c = 0; c < D; c += 32) {
+    uint32_t r[32];
+    tmem_ld32(addr + c, r);
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 32; i += 8) {
+      uint4 w;
+      uint32_t *w4 = &w.x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float lo = __uint_as_float(r[i + 2 * j]) * f, hi = __uint_as_float(r[i + 2 * j + 1]) * f;
+        fine &= isfinite(lo) && isfinite(hi);
+        w4[j] = pack2<T>(lo, hi);
+      }
+      if (store) *reinterpret_cast<uint4 *>(dst + c + i) = w;
+    }
+  }
+  return fine;
+}
+
+template <class T, int D, Mode M>
+__global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>::kCtas)
+    attn_tile_kernel(const __grid_constant__ CUtensorMap map_a0, const __grid_constant__ CUtensorMap map_a1,
+                     const __grid_constant__ CUtensorMap map_x0, const __grid_constant__ CUtensorMap map_x1,
+                     const __grid_constant__ TileArgs x) {
+  using C = Cfg<D, M>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int NB = C::NB, ST = C::ST;
+  extern __shared__ uint8_t raw_smem[];
+  __shared__ uint64_t bars[1 + 4 * ST + 2 * NB + 2];
+  __shared__ uint32_t tmem_result;
+  __shared__ int dead_flag;
+  __shared__ float2 row_stats[2][64];  // dk, dv: lse (base 2) and delta of the streamed rows
+  volatile int *dead = &dead_flag;
+
+  const int warp = threadIdx.x >> 5;
+  const int head = blockIdx.x % x.n_heads, rt = __ldg(x.t.order + blockIdx.x / x.n_heads);
+  int t0 = __ldg(x.t.ptr + rt), t1 = __ldg(x.t.ptr + rt + 1);
+  if (M == kFwd && x.splits > 1) {
+    const int n = t1 - t0, z = blockIdx.y;
+    t1 = t0 + (int)((int64_t)n * (z + 1) / x.splits);
+    t0 = t0 + (int)((int64_t)n * z / x.splits);
+  }
+  const int nt = t1 - t0, iters = M == kDkv ? nt * x.a.group : nt;
+  const int head_a = M == kDkv ? head : head;                      // head of the stationary operands
+  const int64_t row0 = (int64_t)rt * kTileRows;
+
+  const uint32_t sm = (smem_addr(raw_smem) + 1023u) & ~1023u;
+  const uint32_t sm_a0 = sm, sm_a1 = sm + C::kStaticBytes * (C::kStatic - 1);
+  const uint32_t sm_x0 = sm + C::kStatic * C::kStaticBytes, sm_x1 = sm_x0 + ST * C::kStreamBytes;
+  const uint32_t b0 = smem_addr(bars);
+  const uint32_t bar_static = b0, bar_x0_full = b0 + 8, bar_x0_free = bar_x0_full + 8 * ST, bar_x1_full = bar_x0_free + 8 * ST,
+                 bar_x1_free = bar_x1_full + 8 * ST, bar_scores = bar_x1_free + 8 * ST, bar_weights = bar_scores + 8 * NB,
+                 bar_acc = bar_weights + 8 * NB, bar_stats = bar_acc + 8;
+
+  if (iters > 0 && warp == 5) tmem_alloc(smem_addr(&tmem_result), C::kCols);
+  if (threadIdx.x == 0) {
+    dead_flag = 0;
+    mbar_init(bar_static, 1);
+    for (int i = 0; i < ST; ++i) {
+      mbar_init(bar_x0_full + 8 * i, 1);
+      mbar_init(bar_x0_free + 8 * i, 1);
+      mbar_init(bar_x1_full + 8 * i, 1);
+      mbar_init(bar_x1_free + 8 * i, 1);
+    }
+    for (int i = 0; i < NB; ++i) {
+      mbar_init(bar_scores + 8 * i, 1);
+      mbar_init(bar_weights + 8 * i, kWeightThreads);
+    }
+    mbar_init(bar_acc, 1);
+    mbar_init(bar_stats, kWeightThreads);
+    mbar_fence_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = iters > 0 ? tmem_result : 0;
+  const uint32_t tm_s = tm, tm_r = tm + NB * 64, tm_acc0 = tm + C::kAcc, tm_acc1 = tm_acc0 + D;
+
+  if (warp == 4) {  // ------------------------------------------------------------------ loads
+    if ((threadIdx.x & 31) == 0 && iters > 0) {
+      mbar_arrive_expect_tx(bar_static, C::kStatic * C::kStaticBytes);
+      for (int c = 0; c < D / 64; ++c) {
+        tma_load3(sm_a0 + c * 16384, &map_a0, c * 64, head_a, (int)row0, bar_static);
+        if (C::kStatic == 2) tma_load3(sm_a1 + c * 16384, &map_a1, c * 64, head_a, (int)row0, bar_static);
+      }
+      for (int it = 0; it < iters; ++it) {
+        const int s = it % ST, col = __ldg(x.t.col + t0 + it % nt) * kTileCols;
+        const uint32_t parity = ((it / ST) & 1) ^ 1;
+        const int hx = M == kDkv ? head * x.a.group + it / nt : head / x.a.group;
+        if (!wait(bar_x0_free + 8 * s, parity, dead, x.err, 1)) break;
+        mbar_arrive_expect_tx(bar_x0_full + 8 * s, C::kStreamBytes);
+        for (int c = 0; c < D / 64; ++c)
+          tma_load3(sm_x0 + s * C::kStreamBytes + c * 8192, &map_x0, c * 64, hx, col, bar_x0_full + 8 * s);
+        if (!wait(bar_x1_free + 8 * s, parity, dead, x.err, 2)) break;
+        mbar_arrive_expect_tx(bar_x1_full + 8 * s, C::kStreamBytes);
+        for (int c = 0; c < D / 64; ++c)
+          tma_load3(sm_x1 + s * C::kStreamBytes + c * 8192, &map_x1, c * 64, hx, col, bar_x1_full + 8 * s);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 5) {  // ----------------------------------------------------------- products
+    if ((threadIdx.x & 31) == 0 && iters > 0) {
+      constexpr uint32_t id_first = mma_desc(kBf16, 128, 64, false), id_second = mma_desc(kBf16, 128, D, true);
+      // scores of iteration it
+      auto first = [&](int it) {
+        const int s = it % ST, b = it % NB;
+        const uint32_t parity = (it / ST) & 1;
+        if (!wait(bar_x0_full + 8 * s, parity, dead, x.err, 3)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t half = k / 4, off = (k % 4) * 32;
+          mma_ss(tm_s + b * 64, desc_k_major(sm_a0 + half * 16384 + off),
+                 desc_k_major(sm_x0 + s * C::kStreamBytes + half * 8192 + off), id_first, k > 0);
+        }
+        if (M == kFwd) mma_commit(bar_x0_free + 8 * s);  // K is not needed again
+        if (M != kFwd) {
+          if (!wait(bar_x1_full + 8 * s, parity, dead, x.err, 4)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t half = k / 4, off = (k % 4) * 32;
+            mma_ss(tm_r + b * 64, desc_k_major(sm_a1 + half * 16384 + off),
+                   desc_k_major(sm_x1 + s * C::kStreamBytes + half * 8192 + off), id_first, k > 0);
+          }
+          if (M == kDq) mma_commit(bar_x1_free + 8 * s);  // nor is V
+        }
+        mma_commit(bar_scores + 8 * b);
+        return true;
+      };
+      auto second = [&](int it) {
+        const int s = it % ST, b = it % NB;
+        if (!wait(bar_weights + 8 * b, (it / NB) & 1, dead, x.err, 5)) return false;
+        if (M == kFwd && !wait(bar_x1_full + 8 * s, (it / ST) & 1, dead, x.err, 6)) return false;
+        tc_fence_after();
+        const uint32_t x0 = sm_x0 + s * C::kStreamBytes, x1 = sm_x1 + s * C::kStreamBytes;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // 16 streamed rows each: 8 columns of weights, 2048 bytes of the stream's image
+          mma_ts(tm_acc0, tm_s + b * 64 + k * 8, desc_mn_major((M == kDq ? x0 : x1) + k * 2048, 8192), id_second, it > 0 || k > 0);
+        if (M == kDkv) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_ts(tm_acc1, tm_r + b * 64 + k * 8, desc_mn_major(x0 + k * 2048, 8192), id_second, it > 0 || k > 0);
+        }
+        if (M != kFwd) mma_commit(bar_x0_free + 8 * s);
+        if (M != kDq) mma_commit(bar_x1_free + 8 * s);
+        mma_commit(bar_acc);
+        return true;
+      };
+      bool ok = wait(bar_static, 0, dead, x.err, 7);
+      tc_fence_after();
+      ok = ok && first(0);
+      for (int it = 0; ok && it < iters; ++it) {
+        // with two score buffers the next scores are computed while this iteration's weights are
+        if (NB == 2 && it + 1 < iters) ok = first(it + 1);
+        ok = ok && second(it);
+        if (NB == 1 && ok && it + 1 < iters) ok = first(it + 1);
+      }
+    }
+    __syncwarp();
+  } else {  // -------------------------------------------------------------------------- weights
+    const int r = threadIdx.x;  // row of the tile
+    const int64_t row = row0 + r;
+    const int64_t n_rows = x.rows.d.n;
+    const uint32_t lanes = (uint32_t)warp << 21;  // lane 32 * warp
+    const float cap = x.a.cap, inv_cap2 = cap > 0.f ? 2.f * kLog2e / cap : 0.f;
+    const float scale2 = x.a.scale * kLog2e;
+    bool ok = true;
+    // the score of streamed row c of the tile, base 2; d0 + c * step: the signed distance
+    auto score = [&](float dot, float slope2, float dist, float &th) {
+      float u;
+      if (cap > 0.f) u = capped(dot * x.a.scale, cap, inv_cap2, th) * kLog2e;
+      else u = dot * scale2;
+      return fmaf(-slope2, fabsf(dist), u);
+    };
+    if constexpr (M == kFwd) {
+      constexpr float kUp = kBf16 ? 0.f : 6.f;
+      const float slope2 = x.a.slopes ? __ldg(x.a.slopes + head) * kLog2e : 0.f;
+      float m = -INFINITY, l = 0.f;  // weights are exp2(u - m); m lies kUp below a maximum of the row
+      for (int it = 0; it < iters; ++it) {
+        const int b = it % NB, t = t0 + it, mi = __ldg(x.t.mask + t);
+        const uint64_t bits = mi < 0 ? ~0ull : __ldg(x.t.words + (int64_t)mi * kTileRows + r);
+        const float d0 = (float)(row + x.a.row_offset - (int64_t)__ldg(x.t.col + t) * kTileCols);
+        if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x.err, 8))) break;
+        tc_fence_after();
+        float u[64];
+        {
+          uint32_t lo[32], hi[32];
+          tmem_ld32(tm_s + lanes + b * 64, lo);
+          tmem_ld32(tm_s + lanes + b * 64 + 32, hi);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) u[c] = __uint_as_float(lo[c]), u[c + 32] = __uint_as_float(hi[c]);
+        }
+        if (cap > 0.f || slope2 != 0.f) {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) {
+            float th;
+            u[c] = score(u[c], slope2, d0 - (float)c, th);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 64; ++c) u[c] *= scale2;
+        }
+        if (mi >= 0) {
+          const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            u[c] = lo & (1u << c) ? u[c] : -INFINITY;
+            u[c + 32] = hi & (1u << c) ? u[c + 32] : -INFINITY;
+          }
+        }
+        float top[4] = {u[0], u[1], u[2], u[3]};
+#pragma unroll
+        for (int c = 4; c < 64; ++c) top[c & 3] = fmaxf(top[c & 3], u[c]);
+        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) - kUp;
+        const bool grow = mt > m + kSlack || (m == -INFINITY && mt > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float m2 = grow ? mt : m, f = grow ? exp2_approx(m - m2) : 1.f;
+          m = m2;
+          l *= f;
+          if (it > 0) {  // the sum so far, once the previous product has been added to it
+            if (!(ok = warp_wait(bar_acc, (it - 1) & 1, dead, x.err, 9))) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t w[32];
+              tmem_ld32(tm_acc0 + lanes + c, w);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+              tmem_st32(tm_acc0 + lanes + c, w);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float p0 = exp2_approx(u[2 * c] - base), p1 = exp2_approx(u[2 * c + 1] - base);
+          sum[c & 3] += p0 + p1;
+          w[c] = pack2<T>(p0, p1);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st32(tm_s + lanes + b * 64, w);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_weights + 8 * b);
+      }
+      if (ok && iters > 0) ok = wait_last(bar_acc, iters, dead, x.err, 10);
+      tc_fence_after();
+      const bool live = row < n_rows;
+      if (ok && x.splits > 1) {
+        const int64_t at = ((int64_t)blockIdx.y * n_rows + row) * x.a.heads + head;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t w[32];
+          if (iters > 0) {
+            tmem_ld32(tm_acc0 + lanes + c, w);
+            tmem_wait_ld();
+          }
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              *reinterpret_cast<uint4 *>(x.part + at * D + c + i) =
+                  iters > 0 ? make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]) : make_uint4(0, 0, 0, 0);
+          }
+        }
+        if (live) x.part_ml[2 * at] = m, x.part_ml[2 * at + 1] = l;
+      } else if (ok && iters > 0) {
+        const bool fine = put_acc<T, D>(tm_acc0 + lanes, l == 0.f ? 0.f : 1.f / l, x.a.out, row, head, live);
+        if (live && x.a.lse) x.a.lse[row * x.a.heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        const uint32_t bad = __ballot_sync(0xffffffffu, live && !(fine && l == l));
+        if (bad) redo<T, D, M>(x, row0 + 32 * warp, head, bad);
+      } else if (ok && live) {  // no tile: no entry
+        T *dst = (T *)x.a.out.p + row * x.a.out.row + (int64_t)head * x.a.out.head;
+        for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
+        if (x.a.lse) x.a.lse[row * x.a.heads + head] = -INFINITY;
+      }
+    } else {
+      // fp16: dS carries a power of two that brings the largest |dout| near 16
+      float up = 1.f;
+      if (!kBf16) {
+        const int e = (int)(__ldg(x.dout_max) >> 23);  // biased exponent; 255: not finite
+        if (e > 0 && e < 255) up = __uint_as_float((uint32_t)min(max(127 + 4 - (e - 127), 1), 254) << 23);
+      }
+      constexpr float kUp = kBf16 ? 0.f : 12.f;
+      const bool live = row < n_rows;
+      float lse2 = INFINITY, delta = 0.f;
+      if (M == kDq && live) {
+        lse2 = x.a.lse[row * x.a.heads + head] * kLog2e;
+        if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without entries: weights of 0
+        delta = x.a.delta[row * x.a.heads + head];
+      }
+      for (int it = 0; it < iters; ++it) {
+        const int b = it % NB, t = t0 + it % nt, mi = __ldg(x.t.mask + t);
+        const uint64_t bits = mi < 0 ? ~0ull : __ldg(x.t.words + (int64_t)mi * kTileRows + r);
+        const int64_t col = (int64_t)__ldg(x.t.col + t) * kTileCols;
+        const int h = M == kDkv ? head * x.a.group + it / nt : head;
+        const float slope2 = x.a.slopes ? __ldg(x.a.slopes + h) * kLog2e : 0.f;
+        // query position - key position; along the columns it falls (dq: columns are keys) or rises (dk, dv: queries)
+        const float d0 = M == kDq ? (float)(row + x.a.row_offset - col) : (float)(col + x.a.row_offset - row);
+        if (M == kDkv) {
+          if (r < 64) {
+            const int64_t q = col + r;
+            float2 st = make_float2(INFINITY, 0.f);
+            if (q < x.a.n_queries) {
+              st.x = x.a.lse[q * x.a.heads + h] * kLog2e;
+              if (st.x == -INFINITY) st.x = INFINITY;
+              st.x -= kUp;
+              st.y = x.a.delta[q * x.a.heads + h];
+            }
+            row_stats[it & 1][r] = st;
+          }
+          mbar_arrive(bar_stats);
+          if (!(ok = warp_wait(bar_stats, it & 1, dead, x.err, 13))) break;
+        }
+        if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x.err, 11))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t s[32], e[32];
+          tmem_ld32(tm_s + lanes + b * 64 + half * 32, s);
+          tmem_ld32(tm_r + lanes + b * 64 + half * 32, e);
+          tmem_wait_ld();
+          const uint32_t bit = half ? (uint32_t)(bits >> 32) : (uint32_t)bits;
+          uint32_t w[16], v[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float p[2], g[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int cc = half * 32 + c + k;
+              float th = 0.f, lse_c = lse2, delta_c = delta;
+              if (M == kDkv) {
+                const float2 st = row_stats[it & 1][cc];
+                lse_c = st.x, delta_c = st.y;
+              }
+              float u = score(__uint_as_float(s[c + k]), slope2, M == kDq ? d0 - (float)cc : d0 + (float)cc, th);
+              p[k] = exp2_approx(u - lse_c);
+              g[k] = p[k] * (__uint_as_float(e[c + k]) - delta_c) * up;
+              if (cap > 0.f) g[k] *= 1.f - th * th;
+              if (M == kDkv && !kBf16) g[k] *= 0x1p-12f;
+              if (!(bit & (1u << (c + k)))) p[k] = g[k] = 0.f;
+            }
+            if (M == kDkv) w[c / 2] = pack2<T>(p[0], p[1]);
+            v[c / 2] = pack2<T>(g[0], g[1]);
+          }
+          if (M == kDkv) {
+            tmem_st16(tm_s + lanes + b * 64 + half * 16, w);
+            tmem_st16(tm_r + lanes + b * 64 + half * 16, v);
+          } else {
+            tmem_st16(tm_s + lanes + b * 64 + half * 16, v);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(bar_weights + 8 * b);
+      }
+      if (ok && iters > 0) ok = wait_last(bar_acc, iters, dead, x.err, 12);
+      tc_fence_after();
+      const float f = x.a.scale / up;
+      if (ok && iters > 0) {
+        bool fine;
+        if constexpr (M == kDq) {
+          fine = put_acc<T, D>(tm_acc0 + lanes, f, x.a.dq, row, head, live);
+        } else {
+          fine = put_acc<T, D>(tm_acc0 + lanes, kBf16 ? 1.f : 0x1p-12f, x.a.dv, row, head, live);
+          fine = put_acc<T, D>(tm_acc1 + lanes, f, x.a.dk, row, head, live) && fine;
+        }
+        const uint32_t bad = __ballot_sync(0xffffffffu, live && !fine);
+        if (bad) redo<T, D, M>(x, row0 + 32 * warp, head, bad);
+      } else if (ok && live) {
+        for (int c = 0; c < D; c += 8) {
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+          if (M == kDq) {
+            *reinterpret_cast<uint4 *>((T *)x.a.dq.p + row * x.a.dq.row + (int64_t)head * x.a.dq.head + c) = zero;
+          } else {
+            *reinterpret_cast<uint4 *>((T *)x.a.dk.p + row * x.a.dk.row + (int64_t)head * x.a.dk.head + c) = zero;
+            *reinterpret_cast<uint4 *>((T *)x.a.dv.p + row * x.a.dv.row + (int64_t)head * x.a.dv.head + c) = zero;
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*dead)  // a wait gave up: copies and products in flight land before memory is given back
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+  tc_fence_after();
+  if (iters > 0 && warp == 5) tmem_free(tm, C::kCols);
+}
+
+// Splits of the forward pass, joined: a warp per row and head.
+template <class T, int D>
+__global__ void __launch_bounds__(256) attn_tile_join_kernel(const __grid_constant__ TileArgs x) {
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5, n = x.rows.d.n * (int64_t)x.a.heads;
+  if (item >= n) return;
+  const int64_t row = item / x.a.heads;
+  const int h = (int)(item - row * x.a.heads), lane = threadIdx.x & 31;
+  float m = -INFINITY, l = 0.f, acc[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
+  for (int z = 0; z < x.splits; ++z) {
+    const int64_t at = z * n + item;
+    const float m2 = x.part_ml[2 * at], l2 = x.part_ml[2 * at + 1];
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+    const float f1 = exp2_approx(m - base), f2 = exp2_approx(m2 - base);
+    l = l * f1 + l2 * f2;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * f1 + x.part[at * D + lane + 32 * i] * f2;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  bool fine = l == l;
+  T *dst = (T *)x.a.out.p + row * x.a.out.row + (int64_t)h * x.a.out.head;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const float o = acc[i] * inv;
+    fine &= isfinite(o);
+    dst[lane + 32 * i] = T(o);
+  }
+  if (x.a.lse && lane == 0) x.a.lse[item] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (__any_sync(0xffffffffu, !fine)) redo<T, D, kFwd>(x, row, h, 1u);
+}
+
+// delta_i = dout_i . out_i of each row and head, a warp each (fp16: and the largest finite |dout|).
+template <class T, int D>
+__global__ void __launch_bounds__(256) attn_delta_kernel(int64_t rows, const AttnArgs a, uint32_t *dout_max) {
+  const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int64_t row = item / a.heads;
+  const int h = (int)(item - row * a.heads), lane = threadIdx.x & 31;
+  if (row >= rows) return;
+  const T *p = (const T *)a.dout.p + row * a.dout.row + h * a.dout.head, *y = (const T *)a.o.p + row * a.o.row + h * a.o.head;
+  float s = 0.f, top = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) {
+    float f[2], g[2];
+    RowVec<T, 2>::widen(RowVec<T, 2>::ldg(p + 2 * (lane + 32 * i)), f);
+    RowVec<T, 2>::widen(RowVec<T, 2>::ldg(y + 2 * (lane + 32 * i)), g);
+    s = fmaf(f[0], g[0], fmaf(f[1], g[1], s));
+    if (isfinite(f[0])) top = fmaxf(top, fabsf(f[0]));
+    if (isfinite(f[1])) top = fmaxf(top, fabsf(f[1]));
+  }
+  s = group_sum<32>(s);
+  if (lane == 0) a.delta[item] = s;
+  if (std::is_same<T, __half>::value) {
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+    if (lane == 0 && bits > *(volatile uint32_t *)dout_max) atomicMax(dout_max, bits);  // a maximum does not depend on the order
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ launches
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                   const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return (EncodeTiledFn) nullptr;
+    }
+    return (EncodeTiledFn)p;
+  }();
+  return fn;
+}
+
+// rows x heads x dim of a 16-bit type; boxes of 64 elements of one head, `box_rows` rows.
+bool encode(CUtensorMap *map, const Heads &x, int64_t rows, int heads, int dim, bool bf16, int box_rows) {
+  EncodeTiledFn fn = encode_tiled();
+  if (!fn) return false;
+  const cuuint64_t size[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)rows};
+  // the stride of an axis of length one is free
+  const cuuint64_t stride[2] = {(cuuint64_t)(heads > 1 ? x.head : dim) * 2, (cuuint64_t)(rows > 1 ? x.row : (int64_t)dim * heads) * 2};
+  const cuuint32_t box[3] = {64, 1, (cuuint32_t)box_rows}, step[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void *)x.p, size, stride, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+TileView view(const PatternTiles &t) { return {t.ptr, t.col, t.mask, t.order, t.words}; }
+
+int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
+
+template <class T, int D, Mode M>
+int launch(const dsp_pattern *p, TileArgs x, cudaStream_t s) {
+  using C = Cfg<D, M>;
+  constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+  const PatternTiles &t = M == kDkv ? p->tt : p->at;
+  if (t.n == 0) return DSP_OK;
+  const int kv_heads = x.a.heads / x.a.group;
+  x.t = view(t);
+  x.rows = {view(M == kDkv ? p->t : p->a)};
+  x.n_heads = M == kDkv ? kv_heads : x.a.heads;
+  x.err = p->d_err;
+  // an operand without rows is never loaded: any valid map will do
+  const Heads q = x.a.q, k = p->cols ? x.a.k : q, v = p->cols ? x.a.v : q, o = M == kFwd ? q : x.a.dout;
+  const int64_t nq = p->rows, nk = p->cols ? p->cols : p->rows;
+  const int hk = p->cols ? kv_heads : x.a.heads;
+  CUtensorMap a0, a1, x0, x1;
+  bool ok;
+  if (M == kDkv)
+    ok = encode(&a0, k, nk, hk, D, bf16, 128) && encode(&a1, v, nk, hk, D, bf16, 128) &&
+         (nq == 0 || (encode(&x0, q, nq, x.a.heads, D, bf16, 64) && encode(&x1, o, nq, x.a.heads, D, bf16, 64)));
+  else
+    ok = encode(&a0, q, nq, x.a.heads, D, bf16, 128) && encode(&a1, o, nq, x.a.heads, D, bf16, 128) &&
+         encode(&x0, k, nk, hk, D, bf16, 64) && encode(&x1, v, nk, hk, D, bf16, 64);
+  if (!ok) return fail(DSP_ERR_CUDA, "dsp_attn: a tensor map was refused");
+  const cudaError_t e = cudaFuncSetAttribute((const void *)attn_tile_kernel<T, D, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+  if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_attn: %s", cudaGetErrorString(e));
+  attn_tile_kernel<T, D, M><<<dim3((unsigned)((int64_t)t.n * x.n_heads), (unsigned)std::max(1, x.splits)), kThreads, C::kSmem, s>>>(
+      a0, a1, x0, x1, x);
+  const cudaError_t l = cudaGetLastError();
+  return l == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_attn: %s", cudaGetErrorString(l));
+}
+
+template <class T, int D>
+int forward(const dsp_pattern *p, TileArgs x, cudaStream_t s) {
+  int rc = launch<T, D, kFwd>(p, x, s);
+  if (rc || x.splits == 1) return rc;
+  x.rows = {view(p->a)};
+  attn_tile_join_kernel<T, D><<<(unsigned)((p->rows * x.a.heads + 7) / 8), 256, 0, s>>>(x);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_attn: %s", cudaGetErrorString(e));
+}
+
+template <class T, int D>
+int gradients(const dsp_pattern *p, TileArgs x, uint32_t *dout_max, cudaStream_t s) {
+  cudaError_t e = cudaSuccess;
+  if (std::is_same<T, __half>::value) e = cudaMemsetAsync(dout_max, 0, 4, s);
+  if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_attn_grad: %s", cudaGetErrorString(e));
+  attn_delta_kernel<T, D><<<(unsigned)((p->rows * x.a.heads + 7) / 8), 256, 0, s>>>(p->rows, x.a, dout_max);
+  x.dout_max = dout_max;
+  const int rc = launch<T, D, kDq>(p, x, s);
+  return rc ? rc : launch<T, D, kDkv>(p, x, s);
+}
+
+// Pieces that a row tile's list is cut into: enough CTAs for two on every SM where there are few row tiles and heads, each
+// with four tiles at least.
+int splits_of(const dsp_pattern *p, int heads) {
+  const int64_t ctas = (int64_t)p->at.n * heads;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({2ll * p->sms / std::max<int64_t>(ctas, 1), p->at.max_tiles / 4, 64}));
+}
+
+}  // namespace
+
+bool tile_form(const dsp_pattern *p, const dsp_attn_desc *d) {
+  return p->tiled && p->rows > 0 && p->cols > 0 && (d->dtype == DSP_BF16 || d->dtype == DSP_F16) && (d->dim == 64 || d->dim == 128) &&
+         (p->rows == 1 || d->q_row > 0) && (d->heads == 1 || d->q_head > 0) &&
+         (p->cols == 1 || (d->k_row > 0 && d->v_row > 0)) && (d->kv_heads == 1 || (d->k_head > 0 && d->v_head > 0));
+}
+
+int64_t tile_forward_bytes(const dsp_pattern *p, const dsp_attn_desc *d) {
+  const int s = splits_of(p, d->heads);
+  return s == 1 ? 0 : up256(4 * s * p->rows * d->heads * d->dim) + up256(8 * s * p->rows * d->heads);
+}
+
+int tile_forward(const dsp_pattern *p, const AttnArgs &a, int dtype, void *ws, cudaStream_t s) {
+  TileArgs x = {};
+  x.a = a;
+  x.splits = splits_of(p, a.heads);
+  x.part = (float *)ws;
+  x.part_ml = (float *)((char *)ws + up256(4 * x.splits * p->rows * a.heads * a.dim));
+  if (dtype == DSP_BF16) return a.dim == 64 ? forward<__nv_bfloat16, 64>(p, x, s) : forward<__nv_bfloat16, 128>(p, x, s);
+  return a.dim == 64 ? forward<__half, 64>(p, x, s) : forward<__half, 128>(p, x, s);
+}
+
+int64_t tile_grad_bytes(const dsp_pattern *p, const dsp_attn_desc *d) { return up256(4 * p->rows * d->heads) + 256; }
+
+int tile_gradients(const dsp_pattern *p, const AttnArgs &a, int dtype, void *ws, cudaStream_t s) {
+  TileArgs x = {};
+  x.a = a;
+  x.a.delta = (float *)ws;
+  x.a.n_queries = p->rows;
+  x.splits = 1;
+  uint32_t *dout_max = (uint32_t *)((char *)ws + up256(4 * p->rows * a.heads));
+  if (dtype == DSP_BF16) return a.dim == 64 ? gradients<__nv_bfloat16, 64>(p, x, dout_max, s) : gradients<__nv_bfloat16, 128>(p, x, dout_max, s);
+  return a.dim == 64 ? gradients<__half, 64>(p, x, dout_max, s) : gradients<__half, 128>(p, x, dout_max, s);
+}
+
+}  // namespace dsp

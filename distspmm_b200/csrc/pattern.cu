@@ -50,6 +50,83 @@ void pattern_chunks(int32_t n, HostDir *d) {
   d->split_row.insert(d->split_row.end(), few.begin(), few.end());
 }
 
+bool build_tiles(int32_t n, int32_t n_cols, const HostDir &d, bool always, HostTiles *out) {
+  const int32_t nt = (n + kTileRows - 1) / kTileRows, nc = (n_cols + kTileCols - 1) / kTileCols;
+  std::vector<int32_t> ptr(nt + 1, 0);
+  std::atomic<bool> no_memory{false};
+  // tiles of each row tile: stamp[c] = the last row tile that touched column tile c
+  parallel_for(nt, [&](int64_t b, int64_t e) {
+    try {
+      std::vector<int32_t> stamp(nc, -1);
+      for (int64_t t = b; t < e; ++t) {
+        int32_t k = 0;
+        const int32_t hi = d.ptr[std::min<int64_t>(n, (t + 1) * kTileRows)];
+        for (int32_t p = d.ptr[t * kTileRows]; p < hi; ++p) {
+          int32_t &s = stamp[d.cols[p] / kTileCols];
+          k += s != (int32_t)t;
+          s = (int32_t)t;
+        }
+        ptr[t + 1] = k;
+      }
+    } catch (const std::bad_alloc &) {
+      no_memory.store(true);
+    }
+  }, 8);
+  if (no_memory.load()) throw std::bad_alloc();
+  int64_t count = 0;
+  for (int32_t t = 0; t < nt; ++t) count += ptr[t + 1];
+  if (!always && (d.ptr[n] == 0 || (int64_t)d.ptr[n] < count * kTileFill)) return false;
+  HostTiles &o = *out;
+  for (int32_t t = 0; t < nt; ++t) {
+    o.max_tiles = std::max(o.max_tiles, ptr[t + 1]);
+    ptr[t + 1] += ptr[t];
+  }
+  o.ptr = std::move(ptr);
+  o.col.resize(count);
+  o.mask.resize(count);
+  std::vector<uint64_t> words((size_t)count * kTileRows, 0);
+  parallel_for(nt, [&](int64_t b, int64_t e) {
+    try {
+      std::vector<int32_t> at(nc, -1);
+      for (int64_t t = b; t < e; ++t) {
+        const int32_t r0 = (int32_t)(t * kTileRows), r1 = std::min(n, r0 + kTileRows), first = o.ptr[t], last = o.ptr[t + 1];
+        int32_t k = first;
+        for (int32_t p = d.ptr[r0]; p < d.ptr[r1]; ++p) {
+          const int32_t c = d.cols[p] / kTileCols;
+          if (at[c] < 0) at[c] = 0, o.col[k++] = c;
+        }
+        std::sort(o.col.begin() + first, o.col.begin() + last);
+        for (k = first; k < last; ++k) at[o.col[k]] = k;
+        for (int32_t r = r0; r < r1; ++r)
+          for (int32_t p = d.ptr[r]; p < d.ptr[r + 1]; ++p)
+            words[(size_t)at[d.cols[p] / kTileCols] * kTileRows + (r - r0)] |= 1ull << (d.cols[p] % kTileCols);
+        for (k = first; k < last; ++k) at[o.col[k]] = -1;
+      }
+    } catch (const std::bad_alloc &) {
+      no_memory.store(true);
+    }
+  }, 8);
+  if (no_memory.load()) throw std::bad_alloc();
+  int32_t masks = 0;
+  for (int64_t k = 0; k < count; ++k) {
+    const uint64_t *w = &words[(size_t)k * kTileRows];
+    bool full = true;
+    for (int r = 0; r < kTileRows; ++r) full &= w[r] == ~0ull;
+    o.mask[k] = full ? -1 : masks;
+    if (!full) {
+      if (masks != k) std::copy(w, w + kTileRows, &words[(size_t)masks * kTileRows]);
+      ++masks;
+    }
+  }
+  words.resize((size_t)masks * kTileRows);
+  o.words = std::move(words);
+  o.order.resize(nt);
+  for (int32_t t = 0; t < nt; ++t) o.order[t] = t;
+  std::stable_sort(o.order.begin(), o.order.end(),
+                   [&](int32_t x, int32_t y) { return o.ptr[x + 1] - o.ptr[x] > o.ptr[y + 1] - o.ptr[y]; });
+  return true;
+}
+
 namespace {
 
 template <class V>
@@ -81,6 +158,17 @@ int put_dir(dsp_pattern *p, int32_t n, const HostDir &h, PatternDir *d) {
       (rc = put(p, h.row0, &d->row0)) || (rc = put(p, h.nz0, &d->nz0)) || (rc = put(p, h.split_row, &d->split_row)))
     return rc;
   if (!h.perm.empty() && (rc = put(p, h.perm, &d->perm))) return rc;
+  return DSP_OK;
+}
+
+int put_tiles(dsp_pattern *p, const HostTiles &h, PatternTiles *t) {
+  t->n = (int32_t)h.order.size();
+  t->max_tiles = h.max_tiles;
+  t->count = (int64_t)h.col.size();
+  int rc;
+  if ((rc = put(p, h.ptr, &t->ptr)) || (rc = put(p, h.col, &t->col)) || (rc = put(p, h.mask, &t->mask)) ||
+      (rc = put(p, h.order, &t->order)) || (rc = put(p, h.words, &t->words)))
+    return rc;
   return DSP_OK;
 }
 
@@ -138,12 +226,20 @@ int create(int device, const dsp_csr *a, int flags, dsp_pattern *p) {
     }
     pattern_chunks(K, &t);
   }
+  HostTiles ta, tt;
+  if (flags & DSP_PATTERN_ATTENTION) {
+    p->tiled = build_tiles(M, K, h, false, &ta);
+    if (p->tiled && (flags & DSP_PATTERN_GRAD)) build_tiles(K, M, t, true, &tt);
+  }
   DeviceGuard g(device);
   if (g.err != cudaSuccess) return fail(DSP_ERR_CUDA, "cudaSetDevice(%d): %s", device, cudaGetErrorString(g.err));
   cudaError_t e = cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, device);
   if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_pattern_create: %s", cudaGetErrorString(e));
   int rc = put_dir(p, M, h, &p->a);
   if (!rc && (flags & DSP_PATTERN_GRAD)) rc = put_dir(p, K, t, &p->t);
+  if (!rc && p->tiled) rc = put_tiles(p, ta, &p->at);
+  if (!rc && p->tiled && (flags & DSP_PATTERN_GRAD)) rc = put_tiles(p, tt, &p->tt);
+  if (!rc) rc = put(p, std::vector<int>(1, 0), &p->d_err);
   return rc;
 }
 
@@ -197,6 +293,18 @@ extern "C" void dsp_pattern_destroy(dsp_pattern *p) {
   delete p;
 }
 
+extern "C" int dsp_pattern_check_error(dsp_pattern *p) {
+  DSP_TRY_ARG(p, "dsp_pattern_check_error: null pattern");
+  DeviceGuard g(p->device);
+  int flag = 0;
+  cudaError_t e = g.err;
+  if (e == cudaSuccess) e = cudaMemcpy(&flag, p->d_err, sizeof flag, cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && flag != 0) e = cudaMemset(p->d_err, 0, sizeof(int));
+  if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_pattern_check_error: %s", cudaGetErrorString(e));
+  if (flag == 0) return DSP_OK;
+  return fail(DSP_ERR_TIMEOUT, "attention: a bounded wait gave up (code %d); results are incomplete", flag);
+}
+
 extern "C" int dsp_pattern_info_get(const dsp_pattern *p, dsp_pattern_info *info) {
   DSP_TRY_ARG(p && info, "dsp_pattern_info_get: null argument");
   memset(info, 0, sizeof *info);
@@ -208,6 +316,7 @@ extern "C" int dsp_pattern_info_get(const dsp_pattern *p, dsp_pattern_info *info
   info->chunks = p->a.n_chunks;
   info->split_rows = p->a.n_split;
   info->max_row_len = p->max_row_len;
+  info->tiles = p->tiled ? p->at.count : 0;
   info->device_bytes = p->device_bytes;
   return DSP_OK;
 }

@@ -58,6 +58,28 @@ struct HostDir {
 // Fill row_of, chunks and cut rows from ptr.
 void pattern_chunks(int32_t n, HostDir *d);
 
+// The tile form: tiles of kTileRows x kTileCols entries that hold at least one entry, by row tiles, columns rising. A tile
+// with gaps has a 64-bit word of presence bits for each of its rows; a full one (mask = -1) has none.
+constexpr int kTileRows = 128, kTileCols = 64;
+struct PatternTiles {
+  int32_t n = 0, max_tiles = 0;  // row tiles; tiles of the longest one
+  int64_t count = 0;
+  int32_t *ptr = nullptr;     // [n + 1]
+  int32_t *col = nullptr;     // [count] column tile
+  int32_t *mask = nullptr;    // [count] words + 128 * mask, or -1
+  int32_t *order = nullptr;   // [n] row tiles, longest first
+  uint64_t *words = nullptr;
+};
+struct HostTiles {
+  std::vector<int32_t> ptr, col, mask, order;
+  std::vector<uint64_t> words;
+  int32_t max_tiles = 0;
+};
+// Entries per tile from which the tile form is built and used (see tiles_pay in pattern.cu).
+constexpr int64_t kTileFill = 192;
+// False (and out untouched) where tiles would hold fewer than kTileFill entries on average.
+bool build_tiles(int32_t n, int32_t n_cols, const HostDir &d, bool always, HostTiles *out);
+
 // Restores the caller's current device on scope exit.
 struct DeviceGuard {
   int before = -1;
@@ -80,6 +102,9 @@ struct dsp_pattern {
   int64_t rows = 0, cols = 0, nnz = 0, max_row_len = 0;
   dsp::PatternDir a;  // A
   dsp::PatternDir t;  // A transposed (DSP_PATTERN_GRAD)
+  bool tiled = false;  // the tile form of a (and of t) exists
+  dsp::PatternTiles at, tt;
+  int *d_err = nullptr;  // set by a kernel whose bounded wait gave up
   int64_t device_bytes = 0;
   std::vector<void *> allocs;
 };

@@ -50,6 +50,11 @@ class SparsePattern:
         call("dsp_pattern_info_get", self._h, ctypes.byref(i))
         return {k: int(getattr(i, k)) for k, _ in dsp_pattern_info._fields_}
 
+    def check_error(self) -> None:
+        """After the streams were synchronised: raise DspError if an attention kernel's bounded wait
+        gave up (the flag is cleared)."""
+        call("dsp_pattern_check_error", self._h)
+
     def close(self) -> None:
         """Free the device memory; no call that uses the pattern may still be running."""
         if getattr(self, "_h", None):

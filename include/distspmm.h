@@ -317,6 +317,7 @@ typedef struct dsp_pattern_info {
   int64_t chunks;
   int64_t split_rows;   /* rows cut across chunks                                 */
   int64_t max_row_len;
+  int64_t tiles;        /* tiles of the tile form, 0 where the pattern is too thin for it */
   int64_t device_bytes; /* all device memory the pattern holds                    */
 } dsp_pattern_info;
 
@@ -326,6 +327,9 @@ int dsp_pattern_create(int device, const dsp_csr *a, int flags, dsp_pattern **ou
 /* No call that uses the pattern may still be running on the device. */
 void dsp_pattern_destroy(dsp_pattern *p);
 int dsp_pattern_info_get(const dsp_pattern *p, dsp_pattern_info *info);
+/* After the streams of earlier calls were synchronised: DSP_OK, or DSP_ERR_TIMEOUT if an attention kernel's bounded wait on
+ * its own copies or products gave up; the flag is cleared. */
+int dsp_pattern_check_error(dsp_pattern *p);
 
 /* ---------------------------------------------------------------- sparse layers: product with an epilogue */
 #define DSP_ACT_NONE 0
@@ -414,7 +418,7 @@ int64_t dsp_attn_workspace(const dsp_pattern *p, const dsp_attn_desc *d);
 int dsp_attn(const dsp_pattern *p, const dsp_attn_desc *d, void *workspace, int64_t workspace_bytes, void *stream);
 
 /* dq, dk, dv for the gradient `dout` of `out`; fwd: the forward's operands, with the out and lse that it wrote (read only
- * here). Every row is written (0 where a row or column has no entry). slopes are constants: no gradient. */
+ * here); dout's strides are positive. Every row is written (0 where a row or column has no entry). slopes are constants: no gradient. */
 typedef struct dsp_attn_grad_desc {
   dsp_attn_desc fwd;
   const void *dout;

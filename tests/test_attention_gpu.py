@@ -126,17 +126,30 @@ def test_unlisted_keys_never_count(gpu, kind, t):
     kb[bad[2:]] = float("inf")
     vb[bad[:3]] = float("inf")
     vb[bad[3:]] = float("nan")
-    want = d.sparse_attention(p, q.cuda(), k.cuda(), v.cuda()).cpu()
     got, lse = (x.cpu() for x in d.sparse_attention(p, q.cuda(), kb.cuda(), vb.cuda(), return_lse=True))
-    assert torch.equal(got[~hit], want[~hit])
-    assert not torch.isfinite(got[hit]).all(-1).any() and torch.isfinite(lse[~hit & mask.any(1)]).all()
-    # gradients: zero where nothing flows; the rows that see a bad key, and the keys that such rows see, are spoiled
+    want, tol = want64(mask, q, k, v, dout)
+    near(got[~hit], want["out"][~hit], tol["out"][~hit], "out")
+    near(lse[~hit], want["lse"][~hit], tol["lse"][~hit], "lse")
+    assert not torch.isfinite(got[hit]).all(-1).any()
+    # gradients: the rows that see a bad key, and the keys that such rows see, are spoiled
     spoiled = mask[hit].any(0)
-    dq0, dk0, dv0 = (x.cpu() for x in backward(p, dout, q, k, v))
     dq, dk, dv = (x.cpu() for x in backward(p, dout, q, kb, vb))
     clean = ~spoiled & ~torch.isin(torch.arange(n), bad)
-    assert torch.equal(dq[~hit], dq0[~hit])
-    assert clean.any() and torch.equal(dk[clean], dk0[clean]) and torch.equal(dv[clean], dv0[clean])
+    assert clean.any()
+    near(dq[~hit], want["dq"][~hit], tol["dq"][~hit], "dq")
+    near(dk[clean], want["dk"][clean], tol["dk"][clean], "dk")
+    near(dv[clean], want["dv"][clean], tol["dv"][clean], "dv")
+
+
+def want64(mask, q, k, v, dout):
+    """Results and tolerances for these inputs."""
+    w = [x.double().requires_grad_() for x in (q, k, v)]
+    scale = q.shape[2] ** -0.5
+    o, l, p = attention64(mask, *w, scale)
+    grads = torch.autograd.grad(o, w, dout.double())
+    args = [x.detach() for x in (*w, o, l, p)]
+    tol = attention_tolerances(mask, *args, q.dtype, scale, dout=dout.double(), grads=grads)
+    return dict(out=args[3], lse=args[4], dq=grads[0], dk=grads[1], dv=grads[2]), tol
 
 
 def backward(p, dout, q, k, v):
@@ -151,15 +164,59 @@ def test_bad_query_rows_stay_alone(gpu, t):
     a = positional("window", 260, window=50)
     p = d.SparsePattern(a, grad=True, attention=True)
     q, k, v, dout = inputs(260, 260, 2, 2, 64, t, 4)
-    dq0, dk0, dv0 = (x.cpu() for x in backward(p, dout, q, k, v))
     qb, db = q.clone(), dout.clone()
     qb[130] = float("nan")
     db[131] = float("inf")
     dq, dk, dv = (x.cpu() for x in backward(p, db, qb, k, v))
+    mask = mask_of(a)
     rows = torch.ones(260, dtype=torch.bool)
     rows[130:132] = False
-    keys = ~mask_of(a)[130:132].any(0)
-    assert torch.equal(dq[rows], dq0[rows]) and torch.equal(dk[keys], dk0[keys]) and torch.equal(dv[keys], dv0[keys])
+    keys = ~mask[130:132].any(0)
+    want, tol = want64(mask, q, k, v, dout)
+    near(dq[rows], want["dq"][rows], tol["dq"][rows], "dq")
+    near(dk[keys], want["dk"][keys], tol["dk"][keys], "dk")
+    near(dv[keys], want["dv"][keys], tol["dv"][keys], "dv")
+
+
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -10, 2.0 ** 9])
+def test_fp16_gradients_of_any_size(gpu, size):
+    """Small and large gradients in fp16: what the type cannot hold in between is scaled, results keep the tolerance."""
+    a = positional("window", 400, window=220)
+    p = d.SparsePattern(a, grad=True, attention=True)
+    q, k, v, dout = inputs(400, 400, 2, 1, 64, F16, 11)
+    dout = (dout.float() * size).to(F16)
+    dq, dk, dv = (x.cpu() for x in backward(p, dout, q, k, v))
+    want, tol = want64(mask_of(a), q, k, v, dout)
+    for name, x in (("dq", dq), ("dk", dk), ("dv", dv)):
+        near(x, want[name], tol[name], name)
+
+
+def test_split_rows(gpu):
+    """One row tile over many keys, few heads: its list is cut into pieces that are joined; NaN in unlisted keys stays out."""
+    rows, keys = 100, 4000
+    a = csr_of([[j for j in range(keys) if j % 7 or j < i * 30] for i in range(rows)], keys)
+    p = d.SparsePattern(a, attention=True)
+    for t, dim in ((BF16, 128), (F16, 64)):
+        q, k, v, _ = inputs(rows, keys, 2, 1, dim, t, 12)
+        mask = mask_of(a)
+        w = [x.double() for x in (q, k, v)]
+        o, l, pr = attention64(mask, *w, dim ** -0.5)
+        tol = attention_tolerances(mask, *w, o, l, pr, t, dim ** -0.5)
+        out, lse = d.sparse_attention_forward(p, q.cuda(), k.cuda(), v.cuda())
+        near(out, o, tol["out"], "out")
+        near(lse, l, tol["lse"], "lse")
+        v[3500] = float("nan")  # 3500 is a multiple of 7: row 0 does not list it
+        out = d.sparse_attention(p, q.cuda(), k.cuda(), v.cuda()).cpu()
+        free = ~mask[:, 3500]
+        assert free.all()
+        near(out, o, tol["out"], "out")
+
+
+def test_forms_are_chosen_by_fill(gpu):
+    assert d.SparsePattern(positional("window", 600, window=300), attention=True).info()["tiles"] > 0
+    assert d.SparsePattern(d.gen_uniform(4096, 8, seed=1), attention=True).info()["tiles"] == 0
+    assert d.SparsePattern(positional("window", 600, window=300)).info()["tiles"] == 0  # not asked for
+    d.SparsePattern(matrix("one")).check_error()
 
 
 def test_autograd_and_differences(gpu):
