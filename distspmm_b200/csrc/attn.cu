@@ -14,41 +14,13 @@
 #include <type_traits>
 
 #include "attn_row.cuh"
+#include "attn_decode.h"
 #include "attn_tile.h"
 
 namespace dsp {
 namespace {
 
 constexpr int kThreads = 256;
-
-// Rows listed by a CSR in device memory that nothing has validated: every value read from it is bounded before it is used,
-// so that no list can make the kernel leave its operands.
-struct ListRows {
-  const int64_t *indptr, *indices;
-  int64_t rows, nnz, keys;
-  int32_t n_chunks, L;
-  __device__ int64_t chunks() const { return n_chunks; }
-  __device__ int64_t n() const { return rows; }
-  __device__ int64_t ptr(int64_t r) const { return min(max(__ldg(indptr + r), (int64_t)0), nnz); }
-  __device__ void at(int64_t x, int64_t &r, int64_t &p) const {
-    int64_t lo = 0, hi = rows;
-    while (lo < hi) {
-      const int64_t m = (lo + hi) / 2;
-      if (row_start(m, ptr(m + 1)) < x) lo = m + 1;
-      else hi = m;
-    }
-    r = lo;
-    p = lo < rows ? min(max(x - row_start(lo, 0), ptr(lo)), nnz) : ptr(rows);  // no entry behind the last row's end
-  }
-  __device__ void chunk(int64_t c, int64_t &r0, int64_t &r1, int64_t &p0, int64_t &p1) const {
-    at(c * L, r0, p0);
-    at(min((c + 1) * L, row_start(rows, nnz)), r1, p1);
-  }
-  __device__ int64_t col(int64_t p) const { return __ldg(indices + p); }
-  __device__ float distance(const AttnArgs &, int64_t, int64_t end, int64_t p, int64_t) const { return (float)(end - 1 - p); }
-  __device__ bool in_range(int64_t c) const { return c >= 0 && c < keys; }
-  __device__ int32_t units() const { return L; }
-};
 
 template <class Rows, class T, int VE, int LPR, int VPL>
 __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const Rows d, const AttnArgs a) {
@@ -150,15 +122,13 @@ __global__ void __launch_bounds__(kThreads) attn_dkv_kernel(const PlanRows d, co
 }
 
 // Partials of cut rows (forward): merged in chunk order. blockIdx.y: head. Lane l holds columns l, l + 32, ...
-template <class Rows, class T>
-__global__ void __launch_bounds__(kThreads) attn_join_kernel(const Rows d, const int32_t *split_row, int n_split, const AttnArgs a) {
+template <class T>
+__global__ void __launch_bounds__(kThreads) attn_join_kernel(const DirView d, const AttnArgs a) {
   const int lane = threadIdx.x & 31, h = blockIdx.y;
   const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (at >= n_split) return;
-  const int64_t r = split_row ? __ldg(split_row + at) : at;
-  const int64_t L = d.units(), last = d.chunks() - 1;
-  const int64_t c0 = row_start(r, d.ptr(r)) / L, c1 = min(row_start(r, d.ptr(r + 1)) / L, last);
-  if (c0 >= c1) return;  // not cut
+  if (at >= d.n_split) return;
+  const int64_t r = __ldg(d.split_row + at);
+  const int64_t c0 = row_start(r, __ldg(d.ptr + r)) / d.L, c1 = row_start(r, __ldg(d.ptr + r + 1)) / d.L;
   float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
@@ -299,8 +269,7 @@ int forward(const dsp_pattern *p, const dsp_attn_desc *d, char *ws, cudaStream_t
   const PlanRows rows = {view(p->a)};
   launch_pass<PlanRows, T>(kForward, rows, a, p->a.n_chunks, s);
   if (p->a.n_split)
-    attn_join_kernel<PlanRows, T>
-        <<<dim3((unsigned)((p->a.n_split + 7) / 8), (unsigned)d->heads), kThreads, 0, s>>>(rows, p->a.split_row, p->a.n_split, a);
+    attn_join_kernel<T><<<dim3((unsigned)((p->a.n_split + 7) / 8), (unsigned)d->heads), kThreads, 0, s>>>(rows.d, a);
   return status("dsp_attn");
 }
 
@@ -332,25 +301,19 @@ int gradients(const dsp_pattern *p, const dsp_attn_grad_desc *g, char *ws, cudaS
   return status("dsp_attn_grad");
 }
 
-// Units of a chunk for a list of nnz entries: some 16 warps for every SM over all heads.
-int32_t list_units(int64_t rows, int64_t nnz, int heads) {
-  const int64_t l = (row_start(rows, nnz) * heads + 148 * 16 - 1) / (148 * 16);
-  return (int32_t)std::min<int64_t>(1024, std::max<int64_t>(64, (l + 31) / 32 * 32));
-}
-
 template <class T>
 int decode(const dsp_attn_decode_desc *g, char *ws, cudaStream_t s) {
   const dsp_attn_desc *d = &g->fwd;
   AttnArgs a = args_of(d);
-  ListRows rows = {g->indptr, g->indices, g->rows, g->nnz, g->keys, 0, list_units(g->rows, g->nnz, d->heads)};
+  const bool tensor = decode_on_tensor_cores(d->dtype, d->dim);
+  ListRows rows = {g->indptr, g->indices, g->rows, g->nnz, g->keys, 0, decode_units(g->rows, g->nnz, d->heads, d->kv_heads, tensor)};
   rows.n_chunks = (int32_t)((row_start(g->rows, g->nnz) + rows.L - 1) / rows.L);
   const ForwardPlan f = forward_plan(rows.n_chunks, true, d->heads, d->dim);
   a.slots = (float *)ws;
   a.slot_ml = (float *)(ws + f.ml);
+  if (tensor) return decode_tensor(rows, a, d->dtype, s);
   launch_pass<ListRows, T>(kForward, rows, a, rows.n_chunks, s);
-  attn_join_kernel<ListRows, T>
-      <<<dim3((unsigned)((g->rows + 7) / 8), (unsigned)d->heads), kThreads, 0, s>>>(rows, nullptr, (int)g->rows, a);
-  return status("dsp_attn_decode");
+  return decode_join(rows, a, d->dtype, s);
 }
 
 int check_heads(const char *who, const char *name, const void *p, int64_t row, int64_t head, int dtype) {
@@ -457,7 +420,7 @@ extern "C" int dsp_attn_grad(const dsp_pattern *p, const dsp_attn_grad_desc *g, 
 
 extern "C" int64_t dsp_attn_decode_workspace(const dsp_attn_decode_desc *g) {
   if (!g || !usable(&g->fwd) || g->rows < 0 || g->nnz < 0) return 0;
-  const int64_t L = list_units(g->rows, g->nnz, g->fwd.heads);
+  const int64_t L = decode_units(g->rows, g->nnz, g->fwd.heads, g->fwd.kv_heads, decode_on_tensor_cores(g->fwd.dtype, g->fwd.dim));
   return forward_plan((row_start(g->rows, g->nnz) + L - 1) / L, true, g->fwd.heads, g->fwd.dim).total;
 }
 
@@ -465,7 +428,8 @@ extern "C" int dsp_attn_decode(const dsp_attn_decode_desc *g, void *workspace, i
   const char *who = "dsp_attn_decode";
   DSP_TRY_ARG(g, "%s: null argument", who);
   DSP_TRY_ARG(g->rows >= 0 && g->nnz >= 0 && g->keys >= 0, "%s: negative size", who);
-  if (g->rows > (1 << 24) || g->nnz >= INT32_MAX) return fail(DSP_ERR_UNSUPPORTED, "%s: %lld rows, %lld entries", who, (long long)g->rows, (long long)g->nnz);
+  if (g->rows > (1 << 24) || g->nnz >= INT32_MAX || g->keys > INT32_MAX)
+    return fail(DSP_ERR_UNSUPPORTED, "%s: %lld rows, %lld entries, %lld keys", who, (long long)g->rows, (long long)g->nnz, (long long)g->keys);
   int rc = check_attn(who, &g->fwd, g->rows, g->keys);
   if (rc) return rc;
   if (g->rows == 0) return DSP_OK;

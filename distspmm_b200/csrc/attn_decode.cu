@@ -1,0 +1,337 @@
+// attn_decode.cu — single query tokens over listed cache rows, 16-bit caches of dim 64 or 128.
+//
+// Every listed key and value row is read once for all query heads of its group, so the cache's bytes bound the kernel (16
+// query heads on one row of 256 bytes are 32 operations a byte, far below the tensor cores' rate). A warp owns a chunk of the
+// list and one key/value head; its query heads (8 at a time) are the n = 8 side of m16n8k16 products:
+//
+//   S^T [16 keys x 8 heads] = K Q^T        A = 16 key rows, straight from global memory to the lanes that need them
+//   O^T [dim x 8 heads]    += V^T P^T      A = V^T, B = P^T: S^T's lanes hold 8 x 8 blocks, movmatrix turns them
+//
+// The order of a sum is free, so the places of dim (for K) and of dim rows (for V^T) in the fragments are chosen such that each
+// lane's part of a row is whole 16-byte vectors and 4 (8) neighbouring lanes read 64 (128) neighbouring bytes: no shared memory,
+// no transposes but one byte permute per pair of V's keys. The next 16 keys are requested as soon as the products have read the
+// present ones, so each warp keeps about 8 KB in flight. Weights are split in two 16-bit parts, p = hi + lo, with a product
+// for each: the tensor cores are idle anyway, and the result is then as exact as with fp32 weights.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_decode.h"
+#include "rowvec.cuh"
+
+namespace dsp {
+namespace {
+
+constexpr int kThreads = 128;
+
+template <class T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&x);
+  } else {
+    const __half2 x = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&x);
+  }
+}
+
+// 16 keys of the list: K rows lane / 4 and lane / 4 + 8, of each the 16-byte vectors lane % 4 + 4 i; V rows (keys) 2 t, 2 t + 1,
+// 2 t + 8, 2 t + 9 for t = lane % 4, of each the vectors lane / 4 + 8 i.
+template <class T, int D>
+struct Tile {
+  uint4 k[2][D / 32];
+  uint4 v[4][D / 64];
+
+  // ids: entry e of the 16 in lanes e and e + 16; -1: behind the end, -2: no such key
+  __device__ __forceinline__ void load_k(const AttnArgs &a, int hk, int ids) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int id = __shfl_sync(0xffffffffu, ids, (lane >> 2) + 8 * j);
+      const T *src = (const T *)a.k.p + (int64_t)id * a.k.row + (int64_t)hk * a.k.head + t * 8;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+        k[j][i] = id >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * i)) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void load_v(const AttnArgs &a, int hk, int ids) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int id = __shfl_sync(0xffffffffu, ids, 2 * t + (j & 1) + 8 * (j >> 1));
+      const T *src = (const T *)a.v.p + (int64_t)id * a.v.row + (int64_t)hk * a.v.head + (lane >> 2) * 8;
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+        v[j][i] = id >= 0 ? __ldg(reinterpret_cast<const uint4 *>(src + 64 * i)) : make_uint4(0, 0, 0, 0);
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
+
+template <class T, int D>
+__global__ void __launch_bounds__(kThreads) attn_decode_kernel(const ListRows d, const AttnArgs a, int head_tiles) {
+  const int lane = threadIdx.x & 31, t = lane & 3, n8 = lane >> 2;
+  const int kv_heads = a.heads / a.group, per_chunk = kv_heads * head_tiles;
+  const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+  const int64_t chunk = item / per_chunk;
+  if (chunk >= d.n_chunks) return;
+  const int hk = (int)(item - chunk * per_chunk) / head_tiles, tile = (int)(item % head_tiles);
+  const int h0 = hk * a.group + tile * 8, live = min(8, a.group - tile * 8);  // query heads h0 .. h0 + live - 1
+  const float inv_cap2 = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f, scale2 = a.scale * kLog2e;
+  // of S^T this lane holds keys n8 and n8 + 8 of heads 2 t and 2 t + 1
+  float slope2[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) slope2[j] = a.slopes && 2 * t + j < live ? __ldg(a.slopes + h0 + 2 * t + j) * kLog2e : 0.f;
+  int64_t r0, r1, p, p1;
+  d.chunk(chunk, r0, r1, p, p1);
+  const bool head_cut = p > d.ptr(r0);
+  for (int64_t row = r0; row <= r1; ++row) {
+    if (row == r1 && (p >= p1 || row >= d.n())) break;
+    const int64_t end = d.ptr(row + 1), pe = row < r1 ? end : p1;
+    auto ids_at = [&](int64_t b) {
+      const int64_t at = b + (lane & 15);
+      if (at >= pe) return -1;
+      const int64_t c = d.col(at);
+      return d.in_range(c) ? (int)c : -2;
+    };
+    int ids = ids_at(p), next = ids_at(p + 16);
+    Tile<T, D> x;
+    x.load_k(a, hk, ids);
+    x.load_v(a, hk, ids);
+    // Q^T as B fragments: k steps of 16 in the order of K's vectors (step 2 i + j: words 2 j, 2 j + 1 of vector i)
+    uint32_t q[D / 16][2];
+    {
+      const T *src = (const T *)a.q.p + row * a.q.row + (int64_t)(h0 + n8) * a.q.head + t * 8;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) {
+        const uint4 w = n8 < live ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * i)) : make_uint4(0, 0, 0, 0);
+        q[2 * i][0] = w.x, q[2 * i][1] = w.y, q[2 * i + 1][0] = w.z, q[2 * i + 1][1] = w.w;
+      }
+    }
+    float acc[D / 16][4];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};  // of heads 2 t, 2 t + 1; l: this lane's keys only
+#pragma unroll 1
+    for (int64_t b = p; b < pe; b += 16) {
+      float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t w[4] = {word(x.k[0][i], 2 * j), word(x.k[1][i], 2 * j), word(x.k[0][i], 2 * j + 1), word(x.k[1][i], 2 * j + 1)};
+          mma16816<T>(s, w, q[2 * i + j][0], q[2 * i + j][1]);
+        }
+      const int now = ids;
+      ids = next;
+      x.load_k(a, hk, ids);  // the next 16, while these are weighed
+      next = ids_at(b + 32);
+      // scores, base 2, of keys n8 (s[0], s[1]) and n8 + 8 (s[2], s[3])
+      float top[2] = {m[0], m[1]};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = n8 + 8 * (j >> 1), id = __shfl_sync(0xffffffffu, now, key);
+        float th, u = s[j];
+        if (a.cap > 0.f) u = capped(u * a.scale, a.cap, inv_cap2, th) * kLog2e;
+        else u *= scale2;
+        u = fmaf(-slope2[j & 1], (float)(end - 1 - b - key), u);
+        if (id == -1) u = -INFINITY;
+        if (id == -2) u = NAN;
+        s[j] = u;
+        top[j & 1] = fmaxf(top[j & 1], u);
+      }
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) {
+        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
+        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+      }
+      float base[2], keep[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        base[j] = top[j] == -INFINITY ? 0.f : top[j];
+        keep[j] = exp2_approx(m[j] - base[j]);
+        m[j] = top[j];
+        l[j] *= keep[j];
+      }
+      if (__any_sync(0xffffffffu, keep[0] != 1.f || keep[1] != 1.f)) {
+        // acc's columns are heads 2 t, 2 t + 1 too (rows: places of dim)
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] *= keep[j & 1];
+      }
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {  // keys n8 + 8 j
+        const float p0 = exp2_approx(s[2 * j] - base[0]), p1w = exp2_approx(s[2 * j + 1] - base[1]);
+        l[0] += p0;
+        l[1] += p1w;
+        const uint32_t w = pack2<T>(p0, p1w);
+        float f[2];
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+          f[0] = __uint_as_float(w << 16), f[1] = __uint_as_float(w & 0xffff0000u);
+        } else {
+          const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+          f[0] = g.x, f[1] = g.y;
+        }
+        hi[j] = transpose8x8(w);
+        lo[j] = transpose8x8(pack2<T>(p0 - f[0], p1w - f[1]));
+      }
+      // V^T: rows (places of dim) n8 and n8 + 8 of m tile 4 i + c are elements 2 c and 2 c + 1 of vector n8 + 8 i; k: the keys
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t k0 = word(x.v[0][i], c), k1 = word(x.v[1][i], c), k2 = word(x.v[2][i], c), k3 = word(x.v[3][i], c);
+          const uint32_t w[4] = {__byte_perm(k0, k1, 0x5410), __byte_perm(k0, k1, 0x7632), __byte_perm(k2, k3, 0x5410),
+                                 __byte_perm(k2, k3, 0x7632)};
+          mma16816<T>(acc[4 * i + c], w, hi[0], hi[1]);
+          mma16816<T>(acc[4 * i + c], w, lo[0], lo[1]);
+        }
+      x.load_v(a, hk, ids);
+    }
+    // the sum over all keys, then the rows' results
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+    }
+    const bool cut_head = row == r0 && head_cut, cut = cut_head || row == r1;
+    const int64_t slot = (cut_head ? 2 * chunk : 2 * chunk + 1) * a.heads;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int h = h0 + 2 * t + j;
+      if (2 * t + j >= live) continue;
+      const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+#pragma unroll
+      for (int i = 0; i < D / 64; ++i) {
+        // elements 2 c (acc[.][j]) and 2 c + 1 (acc[.][2 + j]) of vector n8 + 8 i
+        float f[8];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f[2 * c] = acc[4 * i + c][j], f[2 * c + 1] = acc[4 * i + c][2 + j];
+        const int col = (n8 + 8 * i) * 8;
+        if (cut) {
+          st_f32<8>(a.slots + (slot + h) * D + col, f);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) f[c] *= inv;
+          RowVec<T, 8>::st((T *)a.out.p + row * a.out.row + (int64_t)h * a.out.head + col, f);
+        }
+      }
+      if (n8 == 0) {
+        if (cut) a.slot_ml[2 * (slot + h)] = m[j], a.slot_ml[2 * (slot + h) + 1] = l[j];
+        else if (a.lse) a.lse[row * a.heads + h] = l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * kLn2;
+      }
+    }
+    p = pe;
+  }
+}
+
+// Rows cut across chunks: a block per row and head. The partials' weights 2^(m - max) first, each by a thread, then the
+// weighted sums in chunk order, a thread per column.
+template <class T>
+__global__ void __launch_bounds__(kThreads) attn_decode_join_kernel(const ListRows d, const AttnArgs a) {
+  __shared__ float weight[kThreads], red[4];
+  const int64_t r = blockIdx.x;
+  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t c0 = row_start(r, d.ptr(r)) / d.L, c1 = min(row_start(r, d.ptr(r + 1)) / d.L, (int64_t)d.n_chunks - 1);
+  if (c0 >= c1) return;  // not cut
+  auto slot = [&](int64_t c) { return (c == c0 ? 2 * c + 1 : 2 * c) * a.heads + h; };
+  float m = -INFINITY;
+  for (int64_t c = c0 + tid; c <= c1; c += kThreads) m = fmaxf(m, a.slot_ml[2 * slot(c)]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (lane == 0) red[warp] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, acc[2] = {0.f, 0.f};
+  for (int64_t b = c0; b <= c1; b += kThreads) {
+    const int n = (int)min((int64_t)kThreads, c1 - b + 1);
+    float w = 0.f;
+    if (tid < n) {
+      const int64_t s = slot(b + tid);
+      w = exp2_approx(a.slot_ml[2 * s] - base);
+      l += w * a.slot_ml[2 * s + 1];
+    }
+    __syncthreads();
+    weight[tid] = w;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int col = tid + k * kThreads;
+      if (col >= a.dim) continue;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) acc[k] = fmaf(weight[i], a.slots[slot(b + i) * a.dim + col], acc[k]);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  __syncthreads();
+  if (lane == 0) red[warp] = l;
+  __syncthreads();
+  l = (red[0] + red[1]) + (red[2] + red[3]);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T *dst = (T *)a.out.p + r * a.out.row + (int64_t)h * a.out.head;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (tid + k * kThreads < a.dim) dst[tid + k * kThreads] = T(acc[k] * inv);
+  if (a.lse && tid == 0) a.lse[r * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+}
+
+template <class T>
+int run(const ListRows &d, const AttnArgs &a, cudaStream_t s) {
+  const int kv_heads = a.heads / a.group, head_tiles = (a.group + 7) / 8;
+  const unsigned blocks = (unsigned)(((int64_t)d.n_chunks * kv_heads * head_tiles + kThreads / 32 - 1) / (kThreads / 32));
+  if (a.dim == 64) attn_decode_kernel<T, 64><<<blocks, kThreads, 0, s>>>(d, a, head_tiles);
+  else attn_decode_kernel<T, 128><<<blocks, kThreads, 0, s>>>(d, a, head_tiles);
+  return decode_join(d, a, std::is_same<T, __nv_bfloat16>::value ? DSP_BF16 : DSP_F16, s);
+}
+
+}  // namespace
+
+bool decode_on_tensor_cores(int dtype, int dim) { return dtype != DSP_F32 && (dim == 64 || dim == 128); }
+
+int32_t decode_units(int64_t rows, int64_t nnz, int heads, int kv_heads, bool tensor) {
+  // tensor cores: a warp per key/value head and 8 query heads; some 24 warps for every SM, 32 to 512 units each
+  const int64_t width = tensor ? (int64_t)kv_heads * ((heads / kv_heads + 7) / 8) : heads;
+  const int64_t l = (row_start(rows, nnz) * width + 148 * 24 - 1) / (148 * 24);
+  return (int32_t)std::min<int64_t>(512, std::max<int64_t>(32, (l + 15) / 16 * 16));
+}
+
+int decode_join(const ListRows &d, const AttnArgs &a, int dtype, cudaStream_t s) {
+  if (d.n_chunks > 1) {
+    const dim3 grid((unsigned)d.rows, (unsigned)a.heads);
+    if (dtype == DSP_F32) attn_decode_join_kernel<float><<<grid, kThreads, 0, s>>>(d, a);
+    else if (dtype == DSP_BF16) attn_decode_join_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(d, a);
+    else attn_decode_join_kernel<__half><<<grid, kThreads, 0, s>>>(d, a);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_attn_decode: %s", cudaGetErrorString(e));
+}
+
+int decode_tensor(const ListRows &d, const AttnArgs &a, int dtype, cudaStream_t s) {
+  return dtype == DSP_BF16 ? run<__nv_bfloat16>(d, a, s) : run<__half>(d, a, s);
+}
+
+}  // namespace dsp
