@@ -23,22 +23,21 @@ __all__ = [
 ]
 
 
+_LAZY = {
+    "SpmmPlan": "spmm", "SparsePattern": "pattern",
+    **dict.fromkeys(("spmm_act", "spmm_act_forward", "spmm_act_backward"), "act"),
+    **dict.fromkeys(("sparse_attention", "sparse_attention_forward", "sparse_attention_backward",
+                     "sparse_attention_decode"), "attention"),
+    **dict.fromkeys(("Rank", "build_local_group", "TorchComm", "distributed_plan", "connect_peers", "make_rank",
+                     "global_plan", "fetch_view"), "dist"),
+}
+
+
 def __getattr__(name):
     # torch-dependent modules load on first use
-    if name in ("SpmmPlan",):
-        from .spmm import SpmmPlan
-        return SpmmPlan
-    if name in ("SparsePattern",):
-        from .pattern import SparsePattern
-        return SparsePattern
-    if name in ("spmm_act", "spmm_act_forward", "spmm_act_backward"):
-        from . import act
-        return getattr(act, name)
-    if name in ("sparse_attention", "sparse_attention_forward", "sparse_attention_backward", "sparse_attention_decode"):
-        from . import attention
-        return getattr(attention, name)
-    if name in ("Rank", "build_local_group", "TorchComm", "distributed_plan", "connect_peers", "make_rank",
-                "global_plan", "fetch_view"):
-        from . import dist
-        return getattr(dist, name)
-    raise AttributeError(name)
+    if name not in _LAZY:
+        raise AttributeError(name)
+    import importlib
+    value = getattr(importlib.import_module("." + _LAZY[name], __name__), name)
+    globals()[name] = value
+    return value

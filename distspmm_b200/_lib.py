@@ -96,7 +96,7 @@ class dsp_attn_grad_desc(ctypes.Structure):
 
 class dsp_attn_decode_desc(ctypes.Structure):
     _fields_ = [("fwd", dsp_attn_desc), ("rows", c_i64), ("nnz", c_i64), ("keys", c_i64), ("indptr", c_vp),
-                ("indices", c_vp)]
+                ("indices", c_vp), ("device", c_int)]
 
 
 class dsp_args(ctypes.Structure):

@@ -12,21 +12,23 @@ import ctypes
 import torch
 
 from ._lib import call, dsp_act_desc, dsp_act_grad_desc, lib
-from .pattern import DTYPES, SparsePattern, ld, need, on_device, ptr, rows_of, workspace
+from .pattern import DTYPES, SparsePattern, ld, need, on_device, ptr, rows_of, stream_of, wants_grad, workspace
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
 
 def _act(act):
-    need(act in ACTS, f"act must be one of {sorted(k for k in ACTS if k)}, is {act!r}")
+    if act not in ACTS:
+        need(False, f"act must be one of {sorted(k for k in ACTS if k)}, is {act!r}")
     return ACTS[act]
 
 
 def _check(p: SparsePattern, B, values):
     need(isinstance(p, SparsePattern), "the first argument must be a SparsePattern")
     on_device("B", B, p.device)
-    need(B.dtype in DTYPES, f"B must be fp32, bf16 or fp16, is {B.dtype}")
-    need(B.dim() == 2 and B.shape[0] == p.cols, f"B must have shape ({p.cols}, N), has {tuple(B.shape)}")
+    if B.dtype not in DTYPES or B.dim() != 2 or B.shape[0] != p.cols:
+        need(B.dtype in DTYPES, f"B must be fp32, bf16 or fp16, is {B.dtype}")
+        need(False, f"B must have shape ({p.cols}, N), has {tuple(B.shape)}")
     values = p.values if values is None else values
     on_device("values", values, p.device, torch.float32, (p.nnz,))
     return rows_of(B), values.contiguous()
@@ -52,8 +54,7 @@ def spmm_act_forward(p: SparsePattern, B: torch.Tensor, values=None, bias=None, 
                      ld(residual) if residual is not None else 0, ptr(out), N, ptr(pre), N)
     nbytes = lib().dsp_spmm_act_workspace(p._h, N)
     ws = workspace(nbytes, B.device)
-    call("dsp_spmm_act", p._h, ctypes.byref(d), ptr(ws), ws.numel(),
-         torch.cuda.current_stream(B.device).cuda_stream)
+    call("dsp_spmm_act", p._h, ctypes.byref(d), ptr(ws), nbytes, stream_of(p.device))
     return out, pre
 
 
@@ -74,13 +75,12 @@ def spmm_act_backward(p: SparsePattern, dout: torch.Tensor, B: torch.Tensor, pre
     dev = B.device
     dB = torch.empty((p.cols, N), dtype=B.dtype, device=dev) if need_B else None
     dvalues = torch.empty(p.nnz, dtype=torch.float32, device=dev) if need_values else None
-    # no row writes the sum over no rows
-    dbias = (torch.empty if p.rows else torch.zeros)(N, dtype=torch.float32, device=dev) if need_bias else None
+    dbias = torch.empty(N, dtype=torch.float32, device=dev) if need_bias else None
     d = dsp_act_grad_desc(DTYPES[B.dtype], code, N, ptr(values), ptr(B), ld(B), ptr(pre) if code else None,
                           ld(pre) if code else 0, ptr(dout), ld(dout), ptr(dB), N, ptr(dvalues), ptr(dbias))
     nbytes = lib().dsp_spmm_act_grad_workspace(p._h, ctypes.byref(d))
     ws = workspace(nbytes, dev)
-    call("dsp_spmm_act_grad", p._h, ctypes.byref(d), ptr(ws), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+    call("dsp_spmm_act_grad", p._h, ctypes.byref(d), ptr(ws), nbytes, stream_of(p.device))
     return dB, dvalues, dbias
 
 
@@ -110,6 +110,8 @@ def spmm_act(p: SparsePattern, B: torch.Tensor, values=None, bias=None, residual
 
     values: [nnz] fp32 in CSR order (None: A's own); bias: [N] fp32; residual: [rows, N] in B's
     type; act: None, "relu", "silu" or "gelu" (erf form). Runs on the current stream."""
+    if not wants_grad(B, values, bias, residual):
+        return spmm_act_forward(p, B, values, bias, residual, act)[0]
     if values is None:
-        values = p.values if isinstance(p, SparsePattern) else None
+        values = p.values
     return _SpmmAct.apply(p, act, B, values, bias, residual)

@@ -12,49 +12,50 @@ import math
 import torch
 
 from ._lib import call, dsp_attn_decode_desc, dsp_attn_desc, dsp_attn_grad_desc, lib
-from .pattern import DTYPES, SparsePattern, need, on_device, ptr, workspace
+from .pattern import DTYPES, SparsePattern, need, on_device, ptr, stream_of, wants_grad, workspace
 
 
 def _heads(t: torch.Tensor) -> torch.Tensor:
     """t itself where the kernels can read it in place (dim contiguous, address and strides multiples of 16 bytes, no axis
     expanded), else a contiguous copy."""
     e = t.element_size()
-    ok = t.stride(2) == 1 and t.data_ptr() % 16 == 0 and all(
-        n <= 1 or (s > 0 and (s * e) % 16 == 0) for n, s in zip(t.shape[:2], t.stride()[:2]))
+    (n, h, w), (rs, hs, ws) = t.shape, t.stride()
+    ok = (ws == 1 or w == 1) and t.data_ptr() % 16 == 0 and (n <= 1 or (rs > 0 and rs * e % 16 == 0)) and (
+        h <= 1 or (hs > 0 and hs * e % 16 == 0))
     return t if ok else t.contiguous()
 
 
-def _strides(t: torch.Tensor):
-    """(row, head) strides; those of axes of length one are free and are set to what the alignment rule accepts."""
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2], t.stride(1) if t.shape[1] > 1 else t.shape[2])
+def _at(t: torch.Tensor):
+    """(address, row stride, head stride); strides of axes of length one are free and are set to what the alignment rule
+    accepts."""
+    (n, h, w), (rs, hs, _) = t.shape, t.stride()
+    return t.data_ptr(), rs if n > 1 else h * w, hs if h > 1 else w
 
 
 def _desc(q, k, v, out, lse, scale, softcap, slopes, row_offset):
-    d = dsp_attn_desc(DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], scale, softcap, ptr(slopes), row_offset)
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        setattr(d, name, t.data_ptr())
-        row, head = _strides(t)
-        setattr(d, name + "_row", row)
-        setattr(d, name + "_head", head)
-    d.lse = ptr(lse)
-    return d
+    return dsp_attn_desc(DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], scale, softcap, ptr(slopes), row_offset, *_at(q),
+                         *_at(k), *_at(v), *_at(out), ptr(lse))
 
 
 def _check(device, rows, keys, q, k, v, scale, softcap, slopes):
     on_device("q", q, device)
-    need(q.dtype in DTYPES, f"q must be fp32, bf16 or fp16, is {q.dtype}")
-    need(q.dim() == 3 and q.shape[0] == rows, f"q must have shape ({rows}, heads, dim), has {tuple(q.shape)}")
-    on_device("k", k, device, q.dtype)
-    need(k.dim() == 3 and (keys is None or k.shape[0] == keys) and k.shape[2] == q.shape[2],
-         f"k must have shape ({'keys' if keys is None else keys}, kv_heads, {q.shape[2]}), has {tuple(k.shape)}")
-    on_device("v", v, device, q.dtype, k.shape)
-    need(k.shape[1] > 0 and q.shape[1] > 0 and q.shape[1] % k.shape[1] == 0,
-         f"{q.shape[1]} query heads over {k.shape[1]} key/value heads")
-    scale = 1.0 / math.sqrt(max(q.shape[2], 1)) if scale is None else float(scale)
+    t = q.dtype
+    if t not in DTYPES or q.dim() != 3 or q.shape[0] != rows:
+        need(t in DTYPES, f"q must be fp32, bf16 or fp16, is {t}")
+        need(False, f"q must have shape ({rows}, heads, dim), has {tuple(q.shape)}")
+    on_device("k", k, device, t)
+    heads, dim = q.shape[1:]
+    if k.dim() != 3 or (keys is not None and k.shape[0] != keys) or k.shape[2] != dim:
+        need(False, f"k must have shape ({'keys' if keys is None else keys}, kv_heads, {dim}), has {tuple(k.shape)}")
+    on_device("v", v, device, t, k.shape)
+    if k.shape[1] == 0 or heads == 0 or heads % k.shape[1]:
+        need(False, f"{heads} query heads over {k.shape[1]} key/value heads")
+    scale = 1.0 / math.sqrt(max(dim, 1)) if scale is None else float(scale)
     softcap = float(softcap or 0.0)
-    need(math.isfinite(scale) and math.isfinite(softcap) and softcap >= 0, f"scale {scale}, softcap {softcap}")
+    if not (math.isfinite(scale) and math.isfinite(softcap) and softcap >= 0):
+        need(False, f"scale {scale}, softcap {softcap}")
     if slopes is not None:
-        on_device("slopes", slopes, device, torch.float32, (q.shape[1],))
+        on_device("slopes", slopes, device, torch.float32, (heads,))
         need(not slopes.requires_grad, "slopes are constants: they get no gradient")
         slopes = slopes.contiguous()
     return _heads(q), _heads(k), _heads(v), scale, softcap, slopes
@@ -73,8 +74,9 @@ def sparse_attention_forward(p: SparsePattern, q, k, v, scale=None, softcap=0.0,
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
     d = _desc(q, k, v, out, lse, scale, softcap, slopes, row_offset)
-    ws = workspace(lib().dsp_attn_workspace(p._h, ctypes.byref(d)), q.device)
-    call("dsp_attn", p._h, ctypes.byref(d), ptr(ws), ws.numel(), torch.cuda.current_stream(q.device).cuda_stream)
+    nbytes = lib().dsp_attn_workspace(p._h, ctypes.byref(d))
+    ws = workspace(nbytes, q.device)
+    call("dsp_attn", p._h, ctypes.byref(d), ptr(ws), nbytes, stream_of(p.device))
     return out, lse
 
 
@@ -88,15 +90,12 @@ def sparse_attention_backward(p: SparsePattern, dout, q, k, v, out, lse, scale=N
     on_device("out", out, p.device, q.dtype, q.shape)
     on_device("lse", lse, p.device, torch.float32, q.shape[:2])
     dout, out, lse = _heads(dout), _heads(out), lse.contiguous()
-    g = dsp_attn_grad_desc(_desc(q, k, v, out, lse, scale, softcap, slopes, row_offset))
     res = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-    for name, t in zip(("dout", "dq", "dk", "dv"), [dout] + res):
-        setattr(g, name, t.data_ptr())
-        row, head = _strides(t)
-        setattr(g, name + "_row", row)
-        setattr(g, name + "_head", head)
-    ws = workspace(lib().dsp_attn_grad_workspace(p._h, ctypes.byref(g.fwd)), q.device)
-    call("dsp_attn_grad", p._h, ctypes.byref(g), ptr(ws), ws.numel(), torch.cuda.current_stream(q.device).cuda_stream)
+    g = dsp_attn_grad_desc(_desc(q, k, v, out, lse, scale, softcap, slopes, row_offset), *_at(dout), *_at(res[0]), *_at(res[1]),
+                           *_at(res[2]))
+    nbytes = lib().dsp_attn_grad_workspace(p._h, ctypes.byref(g.fwd))
+    ws = workspace(nbytes, q.device)
+    call("dsp_attn_grad", p._h, ctypes.byref(g), ptr(ws), nbytes, stream_of(p.device))
     return tuple(res)
 
 
@@ -127,6 +126,9 @@ def sparse_attention(p: SparsePattern, q, k, v, scale=None, softcap=0.0, slopes=
     bias of -slope |i + row_offset - j|, a constant; heads a multiple of kv_heads. Rows without entries give 0 (lse:
     -infinity). fp32, bf16 or fp16; dim a multiple of 8 up to 256. return_lse: (out, lse) (lse has no gradient)."""
     need(slopes is None or not slopes.requires_grad, "slopes are constants: they get no gradient")
+    if not wants_grad(q, k, v):
+        out, lse = sparse_attention_forward(p, q, k, v, scale, softcap, slopes, row_offset)
+        return (out, lse) if return_lse else out
     out, lse = _SparseAttention.apply(p, q, k, v, scale, softcap, slopes, row_offset)
     return (out, lse) if return_lse else out
 
@@ -139,19 +141,19 @@ def sparse_attention_decode(q, k_cache, v_cache, indptr, indices, scale=None, so
 
     The last listed token is the newest: entry t of n is at distance n - 1 - t for ``slopes``. An entry outside the cache
     makes its row NaN. No gradient."""
-    need(isinstance(q, torch.Tensor) and q.is_cuda, "q must be a CUDA tensor")
-    dev = q.device.index
+    need(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3, "q must be a CUDA tensor [rows, heads, dim]")
+    dev, rows = q.get_device(), q.shape[0]
     on_device("indptr", indptr, dev, torch.int64)
     on_device("indices", indices, dev, torch.int64)
-    need(indptr.dim() == 1 and indices.dim() == 1 and q.dim() == 3 and indptr.shape[0] == q.shape[0] + 1,
-         f"indptr must have {q.shape[0] + 1} entries, has {tuple(indptr.shape)}")
-    q, k, v, scale, softcap, slopes = _check(dev, q.shape[0], None, q, k_cache, v_cache, scale, softcap, slopes)
+    if indptr.dim() != 1 or indices.dim() != 1 or indptr.shape[0] != rows + 1:
+        need(False, f"indptr must have {rows + 1} entries, has {tuple(indptr.shape)}")
+    q, k, v, scale, softcap, slopes = _check(dev, rows, None, q, k_cache, v_cache, scale, softcap, slopes)
     indptr, indices = indptr.contiguous(), indices.contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    g = dsp_attn_decode_desc(_desc(q, k, v, out, lse, scale, softcap, slopes, 0), q.shape[0], indices.numel(), k.shape[0],
-                             ptr(indptr), ptr(indices))
-    ws = workspace(lib().dsp_attn_decode_workspace(ctypes.byref(g)), q.device)
-    with torch.cuda.device(q.device):
-        call("dsp_attn_decode", ctypes.byref(g), ptr(ws), ws.numel(), torch.cuda.current_stream(q.device).cuda_stream)
+    g = dsp_attn_decode_desc(_desc(q, k, v, out, lse, scale, softcap, slopes, 0), rows, indices.numel(), k.shape[0],
+                             indptr.data_ptr(), indices.data_ptr(), dev)
+    nbytes = lib().dsp_attn_decode_workspace(ctypes.byref(g))
+    ws = workspace(nbytes, q.device)
+    call("dsp_attn_decode", ctypes.byref(g), ptr(ws), nbytes, stream_of(dev))
     return (out, lse) if return_lse else out

@@ -436,6 +436,8 @@ extern "C" int dsp_attn_decode(const dsp_attn_decode_desc *g, void *workspace, i
   DSP_TRY_ARG(g->indptr && (g->indices || g->nnz == 0), "%s: null index list", who);
   rc = check_workspace(who, workspace, workspace_bytes, dsp_attn_decode_workspace(g));
   if (rc) return rc;
+  DeviceGuard dg(g->device);
+  if (dg.err != cudaSuccess) return fail(DSP_ERR_CUDA, "%s: %s", who, cudaGetErrorString(dg.err));
   if (g->fwd.dtype == DSP_F32) return decode<float>(g, (char *)workspace, (cudaStream_t)stream);
   if (g->fwd.dtype == DSP_BF16) return decode<__nv_bfloat16>(g, (char *)workspace, (cudaStream_t)stream);
   return decode<__half>(g, (char *)workspace, (cudaStream_t)stream);

@@ -80,13 +80,14 @@ constexpr int64_t kTileFill = 192;
 // False (and out untouched) where tiles would hold fewer than kTileFill entries on average.
 bool build_tiles(int32_t n, int32_t n_cols, const HostDir &d, bool always, HostTiles *out);
 
-// Restores the caller's current device on scope exit.
+// Makes `device` current where it is not, and restores the caller's on scope exit.
 struct DeviceGuard {
   int before = -1;
   cudaError_t err;
   explicit DeviceGuard(int device) {
-    err = cudaGetDevice(&before);
-    if (err == cudaSuccess && before != device) err = cudaSetDevice(device);
+    int now = -1;
+    err = cudaGetDevice(&now);
+    if (err == cudaSuccess && now != device && (err = cudaSetDevice(device)) == cudaSuccess) before = now;
   }
   ~DeviceGuard() {
     if (before >= 0) cudaSetDevice(before);

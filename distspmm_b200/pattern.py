@@ -75,27 +75,42 @@ def need(cond: bool, msg: str) -> None:
 
 def on_device(name: str, t: torch.Tensor, device: int, dtype=None, shape=None) -> None:
     """The checks that every dense operand goes through."""
+    if (type(t) is torch.Tensor and t.is_cuda and t.get_device() == device and (dtype is None or t.dtype == dtype)
+            and (shape is None or t.shape == shape)):
+        return
     need(isinstance(t, torch.Tensor), f"{name} must be a tensor")
-    need(t.is_cuda and t.device.index == device, f"{name} must be on cuda:{device}, is on {t.device}")
+    need(t.is_cuda and t.get_device() == device, f"{name} must be on cuda:{device}, is on {t.device}")
     need(dtype is None or t.dtype == dtype, f"{name} must be {dtype}, is {t.dtype}")
     need(shape is None or tuple(t.shape) == tuple(shape), f"{name} must have shape {shape}, has {tuple(t.shape)}")
 
 
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """t itself where its rows are contiguous and do not overlap, else a contiguous copy."""
+    if t.is_contiguous():
+        return t
     return t if (t.stride(1) == 1 or t.shape[1] <= 1) and (t.stride(0) >= t.shape[1] or t.shape[0] <= 1) else t.contiguous()
 
 
 def ld(t: torch.Tensor) -> int:
     """Leading dimension of rows_of(t)."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else max(t.shape[1], 1)
+    n, w = t.shape
+    return max(t.stride(0), w) if n > 1 else max(w, 1)
 
 
 def ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
 
-def workspace(nbytes: int, device: torch.device) -> torch.Tensor:
+def workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
     """Workspace of one call, from torch's allocator on the current stream (so that calls on other
     streams and captured graphs never share it)."""
-    return torch.empty(max(nbytes, 256), dtype=torch.uint8, device=device)
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def stream_of(device: int) -> int:
+    """The current stream of the device (cudaStream_t as int)."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def wants_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)

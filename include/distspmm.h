@@ -438,12 +438,13 @@ int dsp_attn_grad(const dsp_pattern *p, const dsp_attn_grad_desc *d, void *works
  * sequence; indices[indptr[r] .. indptr[r+1]) are the rows of k and v (of `keys` rows) that hold its tokens, oldest first: a
  * page table with pages of one row. Entry t of n is at distance n - 1 - t (for slopes); fwd.row_offset is not used. The
  * lists are not validated on the host; an entry outside [0, keys) makes its row of out and lse NaN and nothing is read there.
- * An entry listed twice counts twice. Runs on the current device. rows <= 2^24, nnz < 2^31 - 1, keys < 2^31. */
+ * An entry listed twice counts twice. Runs on `device`, whatever the current one is. rows <= 2^24, nnz < 2^31 - 1, keys < 2^31. */
 typedef struct dsp_attn_decode_desc {
   dsp_attn_desc fwd; /* q, out: rows x heads x dim; k, v: keys x kv_heads x dim */
   int64_t rows, nnz, keys;
   const int64_t *indptr;
   const int64_t *indices;
+  int device;
 } dsp_attn_decode_desc;
 int64_t dsp_attn_decode_workspace(const dsp_attn_decode_desc *d);
 int dsp_attn_decode(const dsp_attn_decode_desc *d, void *workspace, int64_t workspace_bytes, void *stream);

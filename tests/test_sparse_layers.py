@@ -65,7 +65,7 @@ def decode_desc(**kw):
     from distspmm_b200._lib import dsp_attn_decode_desc, dsp_attn_desc
     f = dict(dtype=1, heads=4, kv_heads=2, dim=64, scale=0.125, softcap=0.0, slopes=None, row_offset=0, q=1 << 12, q_row=256, q_head=64,
              k=1 << 13, k_row=128, k_head=64, v=1 << 14, v_row=128, v_head=64, out=1 << 15, out_row=256, out_head=64, lse=None)
-    g = dict(rows=1, nnz=5, keys=5, indptr=1 << 16, indices=1 << 17)
+    g = dict(rows=1, nnz=5, keys=5, indptr=1 << 16, indices=1 << 17, device=0)
     for k, v in kw.items():
         (f if k in f else g)[k] = v
     return dsp_attn_decode_desc(dsp_attn_desc(*f.values()), *g.values())
