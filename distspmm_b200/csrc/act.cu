@@ -6,8 +6,8 @@
 // The work is a gather of one row of B (or dz) per entry; the arithmetic is two operations per element read, so the kernels
 // are bound by how fast rows come out of L2 (or HBM, once B is larger than the 126 MB L2). What the design does about it:
 // 16-bit rows stay 16-bit until they are in registers, the epilogue adds no pass over the result, and work is cut into
-// chunks of equal entries + row ends, so that hub rows and runs of empty rows are spread evenly. A group of LPR lanes owns a
-// chunk, each lane VPL vectors of VE columns; no lane talks to another in the product kernel.
+// chunks of equal entries + row ends, so that hub rows and runs of empty rows are spread evenly. A warp owns a chunk; a row
+// is read in 16-byte vectors by as many lanes as it has, several rows side by side where it has fewer than 32.
 #include <algorithm>
 #include <type_traits>
 
@@ -23,7 +23,7 @@ struct ActArgs {
   int act, N;
   const float *values;
   const void *B;
-  int64_t ldb;
+  uint32_t ldb_bytes;
   const float *bias;
   const void *residual;
   int64_t ldr;
@@ -73,139 +73,212 @@ __device__ __forceinline__ void finish(const ActArgs &a, int64_t row, int col, f
   V::st_stream((T *)a.out + row * a.ldo + col, z);
 }
 
-// One chunk per group of LPR lanes, walked in steps of U entries: the U rows of B are requested together, whatever rows of A
-// they belong to, then added to the running row; a finished row goes through the epilogue, a cut one to its slot. The
-// residual of the running row is requested when the row begins, so that a row's end does not wait for it.
+// Lanes of a warp: LPR of them span a row (VE elements each, VPL vectors), so G = 32 / LPR entries are gathered side by side, and
+// each lane has the sums of its columns over its group's entries. scatter_sums adds the groups' sums and leaves FE = VE / G
+// elements, number part() * FE on, with each lane: the epilogue's work is spread over all lanes.
+template <int VE, int LPR>
+struct Spread {
+  static constexpr int G = 32 / LPR, FE = VE / G;
+  static_assert(G <= VE, "an element for every group");
+  static __device__ __forceinline__ int part() { return (threadIdx.x & 31) / LPR; }
+  static __device__ __forceinline__ void scatter_sums(const float (&x)[VE], float (&out)[FE]) {
+    float s[VE];
+#pragma unroll
+    for (int i = 0; i < VE; ++i) s[i] = x[i];
+    int h = VE;
+#pragma unroll
+    for (int o = 16; o >= LPR; o >>= 1) {
+      h >>= 1;
+      const bool up = threadIdx.x & o;
+#pragma unroll
+      for (int i = 0; i < VE / 2; ++i)
+        if (i < h) {
+          const float keep = up ? s[i + h] : s[i], give = up ? s[i] : s[i + h];
+          s[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < FE; ++i) out[i] = s[i];
+  }
+  // the inverse: every lane gets all VE elements
+  static __device__ __forceinline__ void gather(const float (&in)[FE], float (&x)[VE]) {
+#pragma unroll
+    for (int i = 0; i < FE; ++i) x[i] = in[i];
+    int h = FE;
+#pragma unroll
+    for (int o = LPR; o < 32; o <<= 1) {
+      const bool up = threadIdx.x & o;
+#pragma unroll
+      for (int i = 0; i < VE / 2; ++i)
+        if (i < h) {
+          const float mine = x[i], other = __shfl_xor_sync(0xffffffffu, mine, o);
+          x[i] = up ? other : mine;
+          x[i + h] = up ? mine : other;
+        }
+      h <<= 1;
+    }
+  }
+};
+
+// A warp's chunk in shared memory: its entries (column, value) and row pointers. One coalesced read per list brings them in, so
+// that a step waits for rows of B only, not for ids first (with ids read step by step the kernel spent 42 % of its time on
+// that chain: 352 us instead of the figure below).
+struct ChunkLists {
+  int2 entry[kMaxUnits];
+  int32_t ptr[kMaxUnits / kRowUnits + 4];
+};
+struct Chunk {
+  int32_t r0, r1, p0, p1;
+};
+// value(p): the value of entry p.
+template <class F>
+__device__ __forceinline__ Chunk load_chunk(const DirView &d, int64_t chunk, ChunkLists &s, F &&value) {
+  const int lane = threadIdx.x & 31;
+  const Chunk c = {__ldg(d.row0 + chunk), __ldg(d.row0 + chunk + 1), __ldg(d.nz0 + chunk), __ldg(d.nz0 + chunk + 1)};
+  __syncwarp();  // the last chunk's lists are read
+  for (int i = lane; i <= c.r1 - c.r0 + 1; i += 32)
+    if (c.r0 + i <= d.n) s.ptr[i] = __ldg(d.ptr + c.r0 + i);
+#pragma unroll 4
+  for (int i = lane; i < c.p1 - c.p0; i += 32) s.entry[i] = make_int2(__ldg(d.cols + c.p0 + i), __float_as_int(value(c.p0 + i)));
+  __syncwarp();
+  return c;
+}
+
+// One chunk per warp, row by row in steps of G U entries: a row's last step is partly masked. A finished row goes through the
+// epilogue, a cut one to its slot. The residual of the running row is requested when the row begins, so that its end does not
+// wait; rows without entries need no more than act(bias), worked out once.
 template <class T, int VE, int LPR, int VPL, int U, int MINB, bool PERM>
 __global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirView d, const ActArgs a) {
   using V = RowVec<T, VE>;
-  const int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LPR;
+  using S = Spread<VE, LPR>;
+  constexpr int G = S::G, FE = S::FE;
+  using F = RowVec<T, FE>;
+  __shared__ ChunkLists lists[kThreads / 32];
+  const int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
   if (chunk >= d.n_chunks) return;
-  const int col0 = blockIdx.y * (LPR * VE * VPL) + (threadIdx.x % LPR) * VE;
-  const int32_t r0 = __ldg(d.row0 + chunk), r1 = __ldg(d.row0 + chunk + 1);
-  const int32_t p0 = __ldg(d.nz0 + chunk), p1 = __ldg(d.nz0 + chunk + 1);
-  const bool head_cut = p0 > __ldg(d.ptr + r0);
-  float acc[VPL][VE], bias[VPL][VE];
-  typename V::Raw res[VPL];
-  int32_t row = r0;
-  auto begin_row = [&]() {
-#pragma unroll
-    for (int w = 0; w < VPL; ++w) {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) acc[w][i] = 0.f;
-      const int col = col0 + w * LPR * VE;
-      if (a.residual && row < r1 && col < a.N) res[w] = V::ld((const T *)a.residual + (int64_t)row * a.ldr + col);
-    }
-  };
+  ChunkLists &list = lists[threadIdx.x >> 5];
+  const Chunk k = load_chunk(d, chunk, list, [&](int32_t p) { return __ldg(a.values + (PERM ? __ldg(d.perm + p) : p)); });
+  const int g = S::part();
+  const int col0 = blockIdx.y * (LPR * VE * VPL) + (threadIdx.x % LPR) * VE;  // gathered columns
+  const int end0 = col0 + g * FE;                                            // columns finished here
+  const bool head_cut = k.p0 > list.ptr[0];
+  float acc[VPL][VE], bias[VPL][FE], idle[VPL][FE];
+  typename F::Raw res[VPL];
+  const char *src[VPL];  // lanes behind the last column read column 0 and store nothing
 #pragma unroll
   for (int w = 0; w < VPL; ++w) {
-    res[w] = V::zero();
+    src[w] = (const char *)((const T *)a.B + (col0 + w * LPR * VE < a.N ? col0 + w * LPR * VE : 0));
+    res[w] = F::zero();
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const int col = col0 + w * LPR * VE + i;
+    for (int i = 0; i < FE; ++i) {
+      const int col = end0 + w * LPR * VE + i;
       bias[w][i] = a.bias && col < a.N ? __ldg(a.bias + col) : 0.f;
+      idle[w][i] = act_of(bias[w][i], a.act);
     }
   }
-  begin_row();
+  int32_t row = k.r0;
+  auto request = [&](int32_t r) {  // the residual of a row that ends here
+#pragma unroll
+    for (int w = 0; w < VPL; ++w) {
+      const int col = end0 + w * LPR * VE;
+      if (a.residual && r < k.r1 && col < a.N) res[w] = F::ld((const T *)a.residual + (int64_t)r * a.ldr + col);
+    }
+  };
   auto store_slot = [&](int64_t slot) {
 #pragma unroll
     for (int w = 0; w < VPL; ++w) {
-      const int col = col0 + w * LPR * VE;
-      if (col < a.N) st_f32<VE>(a.slots + slot * a.N + col, acc[w]);
+      const int col = end0 + w * LPR * VE;
+      float z[FE];
+      S::scatter_sums(acc[w], z);
+      if (col < a.N) st_f32<FE>(a.slots + slot * a.N + col, z);
     }
   };
-  auto end_rows = [&](int32_t to) {  // rows row .. to - 1 end in this chunk
+  auto fetch = [&](int32_t c, int w) { return V::ldg((const T *)(src[w] + (uint64_t)(uint32_t)c * a.ldb_bytes)); };
+  const int2 *entry = list.entry - k.p0;
+  request(row);
+  int32_t p = k.p0;
 #pragma unroll 1
-    while (row < to) {
-      if (row == r0 && head_cut) {
-        store_slot(2 * chunk);
-        ++row;
-        begin_row();
-        continue;
-      }
-      typename V::Raw now[VPL];
-      float z[VPL][VE];
+  for (; row <= k.r1; ++row) {
+    const int32_t pe = row < k.r1 ? list.ptr[row - k.r0 + 1] : k.p1;
+    const bool cut_head = row == k.r0 && head_cut;
+    if (row == k.r1 && p >= pe) break;
+    if (p >= pe && !cut_head) {  // no entries
+      typename F::Raw now[VPL];
+#pragma unroll
+      for (int w = 0; w < VPL; ++w) now[w] = res[w];
+      request(row + 1);
 #pragma unroll
       for (int w = 0; w < VPL; ++w) {
-        now[w] = res[w];
+        const int col = end0 + w * LPR * VE;
+        if (col >= a.N) continue;
+        if (a.pre) st_f32<FE>(a.pre + (int64_t)row * a.ldp + col, bias[w]);
+        float y[FE], r[FE];
+        F::widen(now[w], r);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) z[w][i] = acc[w][i];
+        for (int i = 0; i < FE; ++i) y[i] = a.residual ? idle[w][i] + r[i] : idle[w][i];
+        F::st_stream((T *)a.out + (int64_t)row * a.ldo + col, y);
       }
-      const int64_t at = row++;
-      begin_row();
-#pragma unroll
-      for (int w = 0; w < VPL; ++w) {
-        const int col = col0 + w * LPR * VE;
-        if (col < a.N) finish<T, VE>(a, at, col, z[w], bias[w], now[w]);
-      }
+      continue;
     }
-  };
-  const T *B = (const T *)a.B + col0;
-  // entries come in aligned groups of 4 (the id lists are padded); those outside [p0, p1) are masked
+#pragma unroll
+    for (int w = 0; w < VPL; ++w)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[w][i] = 0.f;
 #pragma unroll 1
-  for (int32_t p = p0 & ~3; p < p1; p += U) {
-    int32_t c[U];
-    float v[U];
+    for (; p + G * U <= pe; p += G * U) {
+      typename V::Raw b[U][VPL];
+      float v[U];
 #pragma unroll
-    for (int q = 0; q < U / 4; ++q) {
-      const int4 c4 = __ldg(reinterpret_cast<const int4 *>(d.cols + p) + q);
-      c[4 * q] = c4.x, c[4 * q + 1] = c4.y, c[4 * q + 2] = c4.z, c[4 * q + 3] = c4.w;
-    }
-    const bool whole = p >= p0 && p + U <= p1;
-    const int32_t last = __ldg(d.row_of + (p + U <= p1 ? p + U : p1) - 1);
-    if (PERM) {
+      for (int u = 0; u < U; ++u) {
+        const int2 e = entry[p + u * G + g];
+        v[u] = __int_as_float(e.y);
 #pragma unroll
-      for (int q = 0; q < U / 4; ++q) {
-        const int4 x = __ldg(reinterpret_cast<const int4 *>(d.perm + p) + q);
-        const int32_t at = p + 4 * q;
-        v[4 * q] = at >= p0 && at < p1 ? __ldg(a.values + x.x) : 0.f;
-        v[4 * q + 1] = at + 1 >= p0 && at + 1 < p1 ? __ldg(a.values + x.y) : 0.f;
-        v[4 * q + 2] = at + 2 >= p0 && at + 2 < p1 ? __ldg(a.values + x.z) : 0.f;
-        v[4 * q + 3] = at + 3 >= p0 && at + 3 < p1 ? __ldg(a.values + x.w) : 0.f;
+        for (int w = 0; w < VPL; ++w) b[u][w] = fetch(e.x, w);
       }
-    } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = p + u >= p0 && p + u < p1 ? __ldg(a.values + p + u) : 0.f;
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int w = 0; w < VPL; ++w) fma_row<T, VE>(acc[w], v[u], b[u][w]);
     }
-    typename V::Raw b[U][VPL];
+    if (p < pe) {  // the last step: entries behind the row's end are read as its last one, and not added
+      typename V::Raw b[U][VPL];
+      float v[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = whole || (p + u >= p0 && p + u < p1);
-      const T *src = B + (int64_t)c[u] * a.ldb;
+      for (int u = 0; u < U; ++u) {
+        const int2 e = entry[min(p + u * G + g, pe - 1)];
+        v[u] = __int_as_float(e.y);
+        if (u == 0 || p + u * G < pe) {
 #pragma unroll
-      for (int w = 0; w < VPL; ++w) b[u][w] = in && col0 + w * LPR * VE < a.N ? V::ldg(src + w * LPR * VE) : V::zero();
-    }
-    auto add = [&](int u) {
-#pragma unroll
-      for (int w = 0; w < VPL; ++w) {
-        float f[VE];
-        V::widen(b[u][w], f);
-#pragma unroll
-        for (int i = 0; i < VE; ++i) acc[w][i] = fmaf(v[u], f[i], acc[w][i]);
-      }
-    };
-    if (whole && last == row) {  // rows are in order: the whole step belongs to the running row
-#pragma unroll
-      for (int u = 0; u < U; ++u) add(u);
-    } else {
-      int32_t r[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) r[u] = p + u < p0 ? -1 : p + u < p1 ? __ldg(d.row_of + p + u) : INT32_MAX;
-#pragma unroll 1
-      while (true) {
-        int32_t next = last;  // the first listed row after the running one
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          if (r[u] == row) add(u);
-          if (r[u] > row) next = min(next, r[u]);
+          for (int w = 0; w < VPL; ++w) b[u][w] = fetch(e.x, w);
         }
-        if (row >= last) break;
-        end_rows(next);
       }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (p + u * G + g < pe) {
+#pragma unroll
+          for (int w = 0; w < VPL; ++w) fma_row<T, VE>(acc[w], v[u], b[u][w]);
+        }
+      p = pe;
+    }
+    if (cut_head || row == k.r1) {
+      store_slot(cut_head ? 2 * chunk : 2 * chunk + 1);
+      request(row + 1);
+      continue;
+    }
+    typename F::Raw now[VPL];
+    float z[VPL][FE];
+#pragma unroll
+    for (int w = 0; w < VPL; ++w) {
+      now[w] = res[w];
+      S::scatter_sums(acc[w], z[w]);
+    }
+    request(row + 1);
+#pragma unroll
+    for (int w = 0; w < VPL; ++w) {
+      const int col = end0 + w * LPR * VE;
+      if (col < a.N) finish<T, FE>(a, row, col, z[w], bias[w], now[w]);
     }
   }
-  end_rows(r1);
-  if (p1 > max(p0, __ldg(d.ptr + r1))) store_slot(r1 == r0 && head_cut ? 2 * chunk : 2 * chunk + 1);
 }
 
 // Rows cut across chunks: their partials go through the epilogue, added in chunk order: by one warp where there are few, in
@@ -263,7 +336,7 @@ __global__ void __launch_bounds__(kThreads) act_join_kernel(const DirView d, con
 struct GradArgs {
   int act, N;
   const void *B;
-  int64_t ldb;
+  uint32_t ldb_bytes;
   const float *pre;
   int64_t ldp;
   const void *dout;
@@ -298,94 +371,119 @@ __device__ __forceinline__ float group_sums(float (&s)[U], int lane, uint32_t ma
 }
 
 // One pass over A's rows: dz (kept in registers in fp32, so that dvalues and dbias see it unrounded; written in T for the
-// product with A transposed, whose sums over many rows are rounded to T anyway), dvalues, and the block's share of dbias.
-template <class T, int VE, int LPR, int VPL>
-__global__ void __launch_bounds__(kThreads) act_grad_rows_kernel(const DirView d, const GradArgs a) {
+// product with A transposed, whose sums over many rows are rounded to T anyway), dvalues, and the block's share of dbias. The
+// walk is the product kernel's; dout and z of the next row are requested when a row begins.
+template <class T, int VE, int LPR, int VPL, int U, int MINB>
+__global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const DirView d, const GradArgs a) {
   using V = RowVec<T, VE>;
-  constexpr int U = 8;
+  using S = Spread<VE, LPR>;
+  constexpr int G = S::G, FE = S::FE;
+  using F = RowVec<T, FE>;
   static_assert(LPR >= U, "a group holds a step's sums");
-  __shared__ float sums[kThreads * VE * VPL];
-  const int lane = threadIdx.x % LPR;
-  const uint32_t mask = LPR == 32 ? 0xffffffffu : ((1u << (LPR & 31)) - 1u) << ((threadIdx.x & 31) / LPR * LPR);
-  const int col0 = blockIdx.y * (LPR * VE * VPL) + lane * VE;
-  const T *B = (const T *)a.B + col0;
-  float bsum[VPL][VE];
+  constexpr int cols = LPR * VE * VPL;
+  __shared__ union {
+    ChunkLists lists[kThreads / 32];
+    float sums[kThreads / 32][cols];
+  } sm;
+  ChunkLists &list = sm.lists[threadIdx.x >> 5];
+  const int lane = threadIdx.x % LPR, g = S::part();
+  const int col0 = blockIdx.y * cols + lane * VE;
+  const int end0 = col0 + g * FE;  // columns whose dz this lane works out
+  const char *src[VPL];  // lanes behind the last column read column 0 and drop it
+#pragma unroll
+  for (int w = 0; w < VPL; ++w) src[w] = (const char *)((const T *)a.B + (col0 + w * LPR * VE < a.N ? col0 + w * LPR * VE : 0));
+  float *dv = a.dvalues ? a.dvalues + (int64_t)blockIdx.y * a.nnz : nullptr;
+  float bsum[VPL][FE], z[VPL][FE];
+  typename F::Raw dout[VPL];
 #pragma unroll
   for (int w = 0; w < VPL; ++w)
 #pragma unroll
-    for (int i = 0; i < VE; ++i) bsum[w][i] = 0.f;
-  const int64_t groups = (int64_t)gridDim.x * (kThreads / LPR);
-  for (int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) / LPR; chunk < d.n_chunks; chunk += groups) {
-    const int32_t r0 = __ldg(d.row0 + chunk), r1 = __ldg(d.row0 + chunk + 1);
-    const int32_t p0 = __ldg(d.nz0 + chunk), p1 = __ldg(d.nz0 + chunk + 1);
-    int32_t p = p0;
-    for (int32_t row = r0; row <= r1; ++row) {
-      const int32_t pe = row < r1 ? __ldg(d.ptr + row + 1) : p1;
-      if (row == r1 && p >= pe) break;
-      float dz[VPL][VE];
+    for (int i = 0; i < FE; ++i) bsum[w][i] = z[w][i] = 0.f;
+  const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
+#pragma unroll 1
+  for (int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5; chunk < d.n_chunks; chunk += warps) {
+    const Chunk k = load_chunk(d, chunk, list, [](int32_t) { return 0.f; });
+    const int2 *entry = list.entry - k.p0;
+    auto request = [&](int32_t row) {  // dout and z of a row
 #pragma unroll
       for (int w = 0; w < VPL; ++w) {
-        const int col = col0 + w * LPR * VE;
-        const bool in = col < a.N;
-        V::widen(in ? V::ldg((const T *)a.dout + (int64_t)row * a.lddo + col) : V::zero(), dz[w]);
-        if (a.act != DSP_ACT_NONE && in) {
-          float z[VE];
-          ld_f32<VE>(a.pre + (int64_t)row * a.ldp + col, z);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) dz[w][i] *= act_slope(z[i], a.act);
-        }
-        if (row < r1) {  // the row ends here: it is counted and written once
-#pragma unroll
-          for (int i = 0; i < VE; ++i) bsum[w][i] += dz[w][i];
-          if (a.dz && in) V::st((T *)a.dz + (int64_t)row * a.N + col, dz[w]);
+        const int col = end0 + w * LPR * VE;
+        dout[w] = F::zero();
+        if (row <= k.r1 && row < d.n && col < a.N) {
+          dout[w] = F::ldg((const T *)a.dout + (int64_t)row * a.lddo + col);
+          if (a.act != DSP_ACT_NONE) ld_f32<FE>(a.pre + (int64_t)row * a.ldp + col, z[w]);
         }
       }
-      if (!a.dvalues) {
-        p = pe;
-        continue;
+    };
+    request(k.r0);
+    int32_t p = k.p0;
+#pragma unroll 1
+    for (int32_t row = k.r0; row <= k.r1; ++row) {
+      const int32_t pe = row < k.r1 ? list.ptr[row - k.r0 + 1] : k.p1;
+      if (row == k.r1 && p >= pe) break;
+      float dz[VPL][VE];
+      {
+        float own[VPL][FE];
+#pragma unroll
+        for (int w = 0; w < VPL; ++w) {
+          F::widen(dout[w], own[w]);
+          if (a.act != DSP_ACT_NONE) {
+#pragma unroll
+            for (int i = 0; i < FE; ++i) own[w][i] *= act_slope(z[w][i], a.act);
+          }
+        }
+        request(row + 1);
+#pragma unroll
+        for (int w = 0; w < VPL; ++w) {
+          const int col = end0 + w * LPR * VE;
+          if (row < k.r1) {  // the row ends here: counted and written once
+#pragma unroll
+            for (int i = 0; i < FE; ++i) bsum[w][i] += own[w][i];
+            if (a.dz && col < a.N) F::st((T *)a.dz + (int64_t)row * a.N + col, own[w]);
+          }
+          if (p < pe) S::gather(own[w], dz[w]);
+        }
       }
-      float *dv = a.dvalues + (int64_t)blockIdx.y * a.nnz;
-      for (; p < pe; p += U) {
-        const int n = min(U, pe - p);
+      if (!dv) p = pe;
+#pragma unroll 1
+      for (; p < pe; p += G * U) {
         typename V::Raw b[U][VPL];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const T *src = B + (u < n ? (int64_t)__ldg(d.cols + p + u) * a.ldb : 0);
-#pragma unroll
-          for (int w = 0; w < VPL; ++w)
-            b[u][w] = u < n && col0 + w * LPR * VE < a.N ? V::ldg(src + w * LPR * VE) : V::zero();
-        }
         float s[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          s[u] = 0.f;
+          const int2 e = entry[min(p + u * G + g, pe - 1)];
 #pragma unroll
-          for (int w = 0; w < VPL; ++w) {
-            float f[VE];
-            V::widen(b[u][w], f);
-#pragma unroll
-            for (int i = 0; i < VE; ++i) s[u] = fmaf(dz[w][i], f[i], s[u]);
-          }
+          for (int w = 0; w < VPL; ++w) b[u][w] = V::ldg((const T *)(src[w] + (uint64_t)(uint32_t)e.x * a.ldb_bytes));
         }
-        const float x = group_sums<U, LPR>(s, lane, mask);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float x[2] = {0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < VPL; ++w)
+            if (col0 + w * LPR * VE < a.N) dot_row<T, VE>(x, dz[w], b[u][w]);
+          s[u] = x[0] + x[1];
+        }
+        const float x = group_sums<U, LPR>(s, lane, 0xffffffffu);
         constexpr int per = LPR / U;
-        if (lane % per == 0 && lane / per < n) dv[p + lane / per] = x;
+        const int32_t at = p + (lane / per) * G + g;
+        if (lane % per == 0 && at < pe) dv[at] = x;
       }
       p = pe;
     }
   }
   if (!a.dbias) return;
+  __syncthreads();
 #pragma unroll
   for (int w = 0; w < VPL; ++w)
 #pragma unroll
-    for (int i = 0; i < VE; ++i) sums[(threadIdx.x / LPR) * (LPR * VE * VPL) + w * LPR * VE + lane * VE + i] = bsum[w][i];
+    for (int i = 0; i < FE; ++i) sm.sums[threadIdx.x >> 5][w * LPR * VE + lane * VE + g * FE + i] = bsum[w][i];
   __syncthreads();
-  constexpr int cols = LPR * VE * VPL;
   for (int c = threadIdx.x; c < cols; c += kThreads) {
     const int col = blockIdx.y * cols + c;
     if (col >= a.N) continue;
     float s = 0.f;
-    for (int g = 0; g < kThreads / LPR; ++g) s += sums[g * cols + c];
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) s += sm.sums[w][c];
     a.dbias[(int64_t)blockIdx.x * a.N + col] = s;
   }
 }
@@ -425,71 +523,87 @@ struct Shape {
 
 bool aligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
-// ve: the widest vector that every operand's address and leading dimension allow (8, 4 or 1). A whole warp spans a row where
-// the row fills it; narrower rows give each chunk a part of the warp.
+// ve: the widest vector that every operand's address and leading dimension allow (8, 4 or 1). Lanes that span a row are the
+// next power of two, at least 32 / VE; wider rows take two vectors a lane, then more column blocks.
 Shape shape_of(int N, int ve, int size) {
-  if (ve == 8 && size == 2 && N >= 256) return {8, 32, N > 256 ? 2 : 1};
-  if (ve >= 4) {
-    if (N > 64) return {4, 32, N > 128 ? 2 : 1};
-    return {4, N > 32 ? 16 : 8, 1};
-  }
-  return {1, 32, N > 32 ? 4 : 1};
+  if (ve == 1) return {1, 32, N > 32 ? 4 : 1};
+  int lpr = 32 / ve;
+  while (lpr < 32 && lpr * ve < N) lpr *= 2;
+  return {ve, lpr, lpr == 32 && N > 32 * ve ? 2 : 1};
 }
 
-template <class T, int VE, int LPR, int VPL, bool PERM>
-void run_product(const DirView &d, const ActArgs &a, cudaStream_t s) {
 #ifndef ACT_U
 #define ACT_U 4
 #define ACT_B 4
+#define GR_U 4
+#define GR_B 4
 #endif
-  constexpr int U = VE * VPL >= 8 ? 4 : ACT_U;
-  const dim3 grid((unsigned)(((int64_t)d.n_chunks * LPR + kThreads - 1) / kThreads),
+template <class T, int VE, int LPR, int VPL, bool PERM>
+void run_product(const DirView &d, const ActArgs &a, cudaStream_t s) {
+  constexpr int U = VE * VPL >= 16 ? 4 : VE == 4 && VPL == 2 ? 4 : ACT_U, minb = VE * VPL >= 16 ? 2 : ACT_B;
+  const dim3 grid((unsigned)((d.n_chunks + kThreads / 32 - 1) / (kThreads / 32)),
                   (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL)));
-  constexpr int minb = VE * VPL >= 16 ? 2 : VE * VPL == 8 ? ACT_B - 1 : ACT_B;
   act_product_kernel<T, VE, LPR, VPL, U, minb, PERM><<<grid, kThreads, 0, s>>>(d, a);
-}
-
-template <class T, bool PERM>
-void pick_product(const Shape &h, const DirView &d, const ActArgs &a, cudaStream_t s) {
-  if constexpr (sizeof(T) == 2) {
-    if (h.VE == 8) return h.VPL == 2 ? run_product<T, 8, 32, 2, PERM>(d, a, s) : run_product<T, 8, 32, 1, PERM>(d, a, s);
-  }
-  if (h.VE == 4) {
-    if (h.LPR == 32) return h.VPL == 2 ? run_product<T, 4, 32, 2, PERM>(d, a, s) : run_product<T, 4, 32, 1, PERM>(d, a, s);
-    return h.LPR == 16 ? run_product<T, 4, 16, 1, PERM>(d, a, s) : run_product<T, 4, 8, 1, PERM>(d, a, s);
-  }
-  return h.VPL == 4 ? run_product<T, 1, 32, 4, PERM>(d, a, s) : run_product<T, 1, 32, 1, PERM>(d, a, s);
-}
-
-template <class T>
-int product(const DirView &d, const ActArgs &a, bool transposed, int ve, cudaStream_t s) {
-  const Shape h = shape_of(a.N, ve, (int)sizeof(T));
-  if (d.n_chunks > 0) {
-    if (transposed) pick_product<T, true>(h, d, a, s);
-    else pick_product<T, false>(h, d, a, s);
-  }
-  if (d.n_split > 0)
-    act_join_kernel<T><<<dim3((unsigned)join_blocks(d), (unsigned)((a.N + 127) / 128)), kThreads, 0, s>>>(d, a);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_spmm_act: %s", cudaGetErrorString(e));
 }
 
 template <class T, int VE, int LPR, int VPL>
 void run_rows(const DirView &d, const GradArgs &a, int blocks, cudaStream_t s) {
-  act_grad_rows_kernel<T, VE, LPR, VPL>
+  constexpr int U = GR_U < LPR ? GR_U : 4, minb = VE * VPL >= 16 ? 2 : GR_B;
+  act_grad_rows_kernel<T, VE, LPR, VPL, U, minb>
       <<<dim3((unsigned)blocks, (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL))), kThreads, 0, s>>>(d, a);
 }
 
-template <class T>
-void pick_rows(const Shape &h, const DirView &d, const GradArgs &a, int blocks, cudaStream_t s) {
+// f.template operator()<VE, LPR, VPL>() of a shape.
+template <class T, class F>
+void with_shape(const Shape &h, F &&f) {
   if constexpr (sizeof(T) == 2) {
-    if (h.VE == 8) return h.VPL == 2 ? run_rows<T, 8, 32, 2>(d, a, blocks, s) : run_rows<T, 8, 32, 1>(d, a, blocks, s);
+    if (h.VE == 8) {
+      if (h.LPR == 4) return f.template operator()<8, 4, 1>();
+      if (h.LPR == 8) return f.template operator()<8, 8, 1>();
+      if (h.LPR == 16) return f.template operator()<8, 16, 1>();
+      return h.VPL == 2 ? f.template operator()<8, 32, 2>() : f.template operator()<8, 32, 1>();
+    }
   }
   if (h.VE == 4) {
-    if (h.LPR == 32) return h.VPL == 2 ? run_rows<T, 4, 32, 2>(d, a, blocks, s) : run_rows<T, 4, 32, 1>(d, a, blocks, s);
-    return h.LPR == 16 ? run_rows<T, 4, 16, 1>(d, a, blocks, s) : run_rows<T, 4, 8, 1>(d, a, blocks, s);
+    if (h.LPR == 8) return f.template operator()<4, 8, 1>();
+    if (h.LPR == 16) return f.template operator()<4, 16, 1>();
+    return h.VPL == 2 ? f.template operator()<4, 32, 2>() : f.template operator()<4, 32, 1>();
   }
-  return h.VPL == 4 ? run_rows<T, 1, 32, 4>(d, a, blocks, s) : run_rows<T, 1, 32, 1>(d, a, blocks, s);
+  return h.VPL == 4 ? f.template operator()<1, 32, 4>() : f.template operator()<1, 32, 1>();
+}
+
+template <class T>
+struct Product {
+  const DirView &d;
+  const ActArgs &a;
+  bool transposed;
+  cudaStream_t s;
+  template <int VE, int LPR, int VPL>
+  void operator()() const {
+    if (transposed) run_product<T, VE, LPR, VPL, true>(d, a, s);
+    else run_product<T, VE, LPR, VPL, false>(d, a, s);
+  }
+};
+
+template <class T>
+struct GradRows {
+  const DirView &d;
+  const GradArgs &a;
+  int blocks;
+  cudaStream_t s;
+  template <int VE, int LPR, int VPL>
+  void operator()() const {
+    run_rows<T, VE, LPR, VPL>(d, a, blocks, s);
+  }
+};
+
+template <class T>
+int product(const DirView &d, const ActArgs &a, bool transposed, int ve, cudaStream_t s) {
+  if (d.n_chunks > 0) with_shape<T>(shape_of(a.N, ve, (int)sizeof(T)), Product<T>{d, a, transposed, s});
+  if (d.n_split > 0)
+    act_join_kernel<T><<<dim3((unsigned)join_blocks(d), (unsigned)((a.N + 127) / 128)), kThreads, 0, s>>>(d, a);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_spmm_act: %s", cudaGetErrorString(e));
 }
 
 int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -518,6 +632,12 @@ int check_type(const char *who, int dtype, int act, int N) {
 
 int esize(int dtype) { return dtype == DSP_F32 ? 4 : 2; }
 
+// Row strides of gathered operands are 32-bit byte counts in the kernels.
+int check_stride(const char *who, const char *name, int64_t ld) {
+  if (ld >= (1ll << 30)) return fail(DSP_ERR_UNSUPPORTED, "%s: %s = %lld: less than 2^30 is wanted", who, name, (long long)ld);
+  return DSP_OK;
+}
+
 int check_workspace(const char *who, const void *ws, int64_t have, int64_t need) {
   if (need == 0) return DSP_OK;
   DSP_TRY_ARG(ws && have >= need, "%s: workspace of %lld bytes, %lld needed", who, (long long)(ws ? have : 0),
@@ -542,7 +662,7 @@ GradPlan grad_plan(const dsp_pattern *p, const dsp_act_grad_desc *d) {
   g.shape = shape_of(d->N, al.ve, esize(d->dtype));
   g.col_blocks = (d->N + g.shape.cols() - 1) / g.shape.cols();
   g.blocks = (int)std::max<int64_t>(
-      1, std::min<int64_t>(8ll * p->sms, ((int64_t)p->a.n_chunks * g.shape.LPR + kThreads - 1) / kThreads));
+      1, std::min<int64_t>(8ll * p->sms, (p->a.n_chunks + kThreads / 32 - 1) / (kThreads / 32)));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -563,12 +683,13 @@ int grad(const dsp_pattern *p, const dsp_act_grad_desc *d, char *ws, cudaStream_
   const bool needs_dz = d->dB && d->act != DSP_ACT_NONE;
   if (needs_dz || d->dvalues || d->dbias) {
     GradArgs a = {};
-    a.act = d->act, a.N = d->N, a.B = d->B, a.ldb = d->ldb, a.pre = d->pre, a.ldp = d->ldp, a.dout = d->dout;
+    a.act = d->act, a.N = d->N, a.B = d->B, a.ldb_bytes = (uint32_t)(d->ldb * sizeof(T)), a.pre = d->pre, a.ldp = d->ldp, a.dout = d->dout;
     a.lddo = d->lddo, a.nnz = p->nnz;
     a.dz = needs_dz ? ws + g.dz : nullptr;
     a.dvalues = !d->dvalues || p->nnz == 0 ? nullptr : g.col_blocks > 1 ? (float *)(ws + g.dvalues) : d->dvalues;
     a.dbias = d->dbias ? (float *)(ws + g.dbias) : nullptr;
-    pick_rows<T>(g.shape, view(p->a), a, g.blocks, s);
+    const DirView rows = view(p->a);
+    with_shape<T>(g.shape, GradRows<T>{rows, a, g.blocks, s});
     if (d->dbias)
       column_sums_kernel<<<(d->N + 31) / 32, kThreads, 0, s>>>((float *)(ws + g.dbias), g.blocks, d->N, d->dbias);
     if (a.dvalues && g.col_blocks > 1)
@@ -579,10 +700,11 @@ int grad(const dsp_pattern *p, const dsp_act_grad_desc *d, char *ws, cudaStream_
     ActArgs a = {};
     a.act = DSP_ACT_NONE, a.N = d->N, a.values = d->values, a.out = d->dB, a.ldo = d->lddb;
     a.B = needs_dz ? ws + g.dz : d->dout;
-    a.ldb = needs_dz ? d->N : d->lddo;
+    const int64_t ldb = needs_dz ? d->N : d->lddo;
+    a.ldb_bytes = (uint32_t)(ldb * sizeof(T));
     a.slots = (float *)(ws + g.slots);
     Align al((int)sizeof(T), d->N);
-    al.row(a.B, a.ldb);
+    al.row(a.B, ldb);
     al.row(a.out, a.ldo);
     return product<T>(view(p->t), a, true, al.ve, s);
   }
@@ -611,6 +733,7 @@ extern "C" int dsp_spmm_act(const dsp_pattern *p, const dsp_act_desc *d, void *w
   DSP_TRY_ARG(!d->residual || d->ldr >= d->N, "%s: ldr = %lld", who, (long long)d->ldr);
   DSP_TRY_ARG(!d->pre || d->ldp >= d->N, "%s: ldp = %lld", who, (long long)d->ldp);
   DSP_TRY_ARG(d->residual != d->out || d->ldr == d->ldo, "%s: a residual in place needs ldr = ldo", who);
+  if ((rc = check_stride(who, "ldb", d->ldb))) return rc;
   rc = check_workspace(who, workspace, workspace_bytes, dsp_spmm_act_workspace(p, d->N));
   if (rc) return rc;
   DeviceGuard g(p->device);
@@ -620,8 +743,8 @@ extern "C" int dsp_spmm_act(const dsp_pattern *p, const dsp_act_desc *d, void *w
   al.row(d->residual, d->ldr);
   al.row(d->out, d->ldo);
   al.row_f32(d->pre, d->ldp);
-  ActArgs a = {d->act, d->N,      d->values, d->B,   d->ldb, d->bias, d->residual,
-               d->ldr, d->out,    d->ldo,    d->pre, d->ldp, (float *)workspace};
+  ActArgs a = {d->act, d->N,   d->values, d->B,   (uint32_t)(d->ldb * esize(d->dtype)), d->bias, d->residual,
+               d->ldr, d->out, d->ldo,    d->pre, d->ldp, (float *)workspace};
   cudaStream_t s = (cudaStream_t)stream;
   if (d->dtype == DSP_F32) return product<float>(view(p->a), a, false, al.ve, s);
   if (d->dtype == DSP_BF16) return product<__nv_bfloat16>(view(p->a), a, false, al.ve, s);
@@ -658,6 +781,7 @@ extern "C" int dsp_spmm_act_grad(const dsp_pattern *p, const dsp_act_grad_desc *
     }
     return DSP_OK;
   }
+  if ((rc = check_stride(who, "ldb", d->ldb)) || (rc = check_stride(who, "lddo", d->lddo))) return rc;
   rc = check_workspace(who, workspace, workspace_bytes, dsp_spmm_act_grad_workspace(p, d));
   if (rc) return rc;
   char *ws = (char *)workspace;

@@ -37,24 +37,14 @@ struct HeadRow {
     for (int w = 0; w < VPL; ++w) V::widen(r[w], f[w]);
   }
   static __device__ __forceinline__ float dot(const float (&x)[VPL][VE], const Raw (&r)[VPL]) {
-    float s = 0.f;
+    float s[2] = {0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < VPL; ++w) {
-      float f[VE];
-      V::widen(r[w], f);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) s = fmaf(x[w][i], f[i], s);
-    }
-    return s;
+    for (int w = 0; w < VPL; ++w) dot_row<T, VE>(s, x[w], r[w]);
+    return s[0] + s[1];
   }
   static __device__ __forceinline__ void add(float (&acc)[VPL][VE], float x, const Raw (&r)[VPL]) {
 #pragma unroll
-    for (int w = 0; w < VPL; ++w) {
-      float f[VE];
-      V::widen(r[w], f);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) acc[w][i] = fmaf(x, f[i], acc[w][i]);
-    }
+    for (int w = 0; w < VPL; ++w) fma_row<T, VE>(acc[w], x, r[w]);
   }
   static __device__ __forceinline__ void store(const HeadsOut &x, int64_t row, int head, int lane, int dim, const float (&f)[VPL][VE]) {
     T *dst = (T *)x.p + row * x.row + head * x.head + lane * VE;

@@ -12,7 +12,7 @@ namespace dsp {
 static int32_t chunk_units(int64_t units) {
   int64_t l = (units + 148 * 32 - 1) / (148 * 32);
   l = (l + 31) / 32 * 32;
-  return (int32_t)std::min<int64_t>(512, std::max<int64_t>(64, l));
+  return (int32_t)std::min<int64_t>(kMaxUnits, std::max<int64_t>(64, l));
 }
 
 void pattern_chunks(int32_t n, HostDir *d) {
@@ -132,7 +132,7 @@ namespace {
 template <class V>
 int put(dsp_pattern *p, const std::vector<V> &h, V **out) {
   *out = nullptr;
-  const size_t bytes = std::max<size_t>(h.size(), 1) * sizeof(V) + 64;  // id lists are read in aligned steps of up to 8
+  const size_t bytes = std::max<size_t>(h.size(), 1) * sizeof(V);
   void *d = nullptr;
   cudaError_t e = cudaMalloc(&d, bytes);
   if (e != cudaSuccess) {

@@ -20,6 +20,7 @@ namespace dsp {
 // kLongSlots partials first (n_long of them).
 constexpr int kRowUnits = 8;
 constexpr int kLongSlots = 16;
+constexpr int kMaxUnits = 512;  // of a chunk
 DSP_HD int64_t row_start(int64_t r, int64_t p) { return r * kRowUnits + p; }
 
 struct PatternDir {

@@ -78,6 +78,40 @@ struct RowVec {
   }
 };
 
+// Two fused multiply-adds in one instruction, each rounded as fmaf.
+__device__ __forceinline__ void fma2(float &c0, float &c1, float a0, float a1, float b0, float b1) {
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%0, %1};\n fma.rn.f32x2 c, a, b, c;\n "
+      "mov.b64 {%0, %1}, c;\n}"
+      : "+f"(c0), "+f"(c1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+// acc += x * row
+template <class T, int VE>
+__device__ __forceinline__ void fma_row(float (&acc)[VE], float x, typename RowVec<T, VE>::Raw r) {
+  float f[VE];
+  RowVec<T, VE>::widen(r, f);
+  if constexpr (VE % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VE; i += 2) fma2(acc[i], acc[i + 1], f[i], f[i + 1], x, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[i] = fmaf(x, f[i], acc[i]);
+  }
+}
+// s += x . row, in two interleaved sums where VE is even
+template <class T, int VE>
+__device__ __forceinline__ void dot_row(float (&s)[2], const float (&x)[VE], typename RowVec<T, VE>::Raw r) {
+  float f[VE];
+  RowVec<T, VE>::widen(r, f);
+  if constexpr (VE % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < VE; i += 2) fma2(s[0], s[1], f[i], f[i + 1], x[i], x[i + 1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) s[0] = fmaf(x[i], f[i], s[0]);
+  }
+}
+
 // fp32 rows beside rows of T (pre-activations, partial sums): VE floats as float4s, or one by one.
 template <int VE>
 __device__ __forceinline__ void ld_f32(const float *p, float (&f)[VE]) {

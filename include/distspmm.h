@@ -339,7 +339,7 @@ int dsp_pattern_check_error(dsp_pattern *p);
 
 /* out = act(A*B + bias) + residual, row by row:
  *   values    [nnz] fp32, device, in A's CSR order
- *   B         cols x N, dtype, leading dimension ldb (elements)
+ *   B         cols x N, dtype, leading dimension ldb (elements; ldb and lddo < 2^30)
  *   bias      [N] fp32, or NULL
  *   residual  rows x N, dtype, ldr, or NULL; may be `out` itself (the same address and ldr = ldo)
  *   out       rows x N, dtype, ldo; no overlap with B. Rows of A without entries give act(bias) + residual.
