@@ -17,7 +17,11 @@
 namespace dsp {
 namespace {
 
-constexpr int kThreads = 256;
+#ifndef ACT_T
+#define ACT_T 256
+#define ACT_G 4
+#endif
+constexpr int kThreads = 256, kWalk = ACT_T;  // kWalk: threads of the kernels that walk chunks
 
 struct ActArgs {
   int act, N;
@@ -34,22 +38,77 @@ struct ActArgs {
   float *slots;  // [2 n_chunks][N] partial rows
 };
 
-__device__ __forceinline__ float act_of(float z, int act) {
-  if (act == DSP_ACT_RELU) return z > 0.f ? z : (z == z ? 0.f : z);  // NaN stays NaN
-  if (act == DSP_ACT_SILU) return z / (1.f + expf(-z));
-  if (act == DSP_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
-  return z;
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-__device__ __forceinline__ float act_slope(float z, int act) {
-  if (act == DSP_ACT_RELU) return z > 0.f ? 1.f : 0.f;
-  if (act == DSP_ACT_SILU) {
-    const float e = 1.f / (1.f + expf(-z));
-    return e * (1.f + z * (1.f - e));
+// Phi(z) (the normal distribution) and exp(-z^2 / 2) of two values. With x = |z| / sqrt 2 and t = 1 / (1 + 0.45 x):
+// erfc(x) = t exp(-x^2) Q(t), Q the polynomial of degree 9 through erfcx(x) / t at Chebyshev nodes of (0, 1]; it is within 4e-8
+// of it, and evaluated in fp32 within 4e-7, relative to erfc itself. (erfcf costs five times the instructions: 50 of 272 us
+// of an R-MAT 18 product with gelu.)
+__device__ __forceinline__ void normal2(float z0, float z1, float &c0, float &c1, float &e0, float &e1) {
+  constexpr float Q[10] = {0.253885329f, 0.253883481f, 0.228263408f, 0.175332934f, 0.119559288f, -0.021311678f, 0.140786096f, -0.299159557f, 0.190028757f, -0.041268073f};
+  const float t0 = __fdividef(1.f, fmaf(fabsf(z0), 0.45f * 0.70710678f, 1.f)), t1 = __fdividef(1.f, fmaf(fabsf(z1), 0.45f * 0.70710678f, 1.f));
+  e0 = exp2_fast(z0 * z0 * -0.72134752f), e1 = exp2_fast(z1 * z1 * -0.72134752f);
+  float q0 = Q[9], q1 = Q[9];
+#pragma unroll
+  for (int i = 8; i >= 0; --i) {
+    float r0 = Q[i], r1 = Q[i];
+    fma2(r0, r1, q0, q1, t0, t1);
+    q0 = r0, q1 = r1;
   }
-  if (act == DSP_ACT_GELU)
-    return 0.5f * erfcf(-0.70710678118654752f * z) + z * 0.39894228040143268f * expf(-0.5f * z * z);
-  return 1.f;
+  c0 = 0.5f * t0 * q0 * e0, c1 = 0.5f * t1 * q1 * e1;
+  c0 = z0 > 0.f ? 1.f - c0 : c0, c1 = z1 > 0.f ? 1.f - c1 : c1;
+}
+
+// act of each element.
+template <int N>
+__device__ __forceinline__ void act_all(float (&z)[N], int act) {
+  if (act == DSP_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = z[i] < 0.f ? 0.f : z[i];  // NaN stays NaN
+  } else if (act == DSP_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) z[i] = __fdividef(z[i], 1.f + exp2_fast(z[i] * -1.44269504f));
+  } else if (act == DSP_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      constexpr int last = N - 1;
+      const int j = i < last ? i + 1 : i;
+      float c0, c1, e0, e1;
+      normal2(z[i], z[j], c0, c1, e0, e1);
+      const float y0 = z[i] * c0, y1 = z[j] * c1;
+      z[i] = y0;
+      if (j != i) z[j] = y1;
+    }
+  }
+}
+
+// x *= act'(z) of each element.
+template <int N>
+__device__ __forceinline__ void act_slopes(float (&x)[N], const float (&z)[N], int act) {
+  if (act == DSP_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = z[i] > 0.f ? x[i] : x[i] * 0.f;
+  } else if (act == DSP_ACT_SILU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float e = __fdividef(1.f, 1.f + exp2_fast(z[i] * -1.44269504f));
+      x[i] *= e * fmaf(z[i], 1.f - e, 1.f);
+    }
+  } else if (act == DSP_ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      constexpr int last = N - 1;
+      const int j = i < last ? i + 1 : i;
+      float c0, c1, e0, e1;
+      normal2(z[i], z[j], c0, c1, e0, e1);
+      x[i] *= fmaf(z[i] * 0.39894228f, e0, c0);
+      if (j != i) x[j] *= fmaf(z[j] * 0.39894228f, e1, c1);
+    }
+  }
 }
 
 // The epilogue of VE columns of one row: sum -> z -> pre, out. r: the residual's vector (zero where there is none).
@@ -60,10 +119,7 @@ __device__ __forceinline__ void finish(const ActArgs &a, int64_t row, int col, f
 #pragma unroll
   for (int i = 0; i < VE; ++i) z[i] += bias[i];
   if (a.pre) st_f32<VE>(a.pre + row * a.ldp + col, z);
-  if (a.act != DSP_ACT_NONE) {
-#pragma unroll
-    for (int i = 0; i < VE; ++i) z[i] = act_of(z[i], a.act);
-  }
+  act_all(z, a.act);
   if (a.residual) {
     float r[VE];
     V::widen(res, r);
@@ -148,13 +204,13 @@ __device__ __forceinline__ Chunk load_chunk(const DirView &d, int64_t chunk, Chu
 // epilogue, a cut one to its slot. The residual of the running row is requested when the row begins, so that its end does not
 // wait; rows without entries need no more than act(bias), worked out once.
 template <class T, int VE, int LPR, int VPL, int U, int MINB, bool PERM>
-__global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirView d, const ActArgs a) {
+__global__ void __launch_bounds__(kWalk, MINB) act_product_kernel(const DirView d, const ActArgs a) {
   using V = RowVec<T, VE>;
   using S = Spread<VE, LPR>;
   constexpr int G = S::G, FE = S::FE;
   using F = RowVec<T, FE>;
-  __shared__ ChunkLists lists[kThreads / 32];
-  const int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+  __shared__ ChunkLists lists[kWalk / 32];
+  const int64_t chunk = ((int64_t)blockIdx.x * kWalk + threadIdx.x) >> 5;
   if (chunk >= d.n_chunks) return;
   ChunkLists &list = lists[threadIdx.x >> 5];
   const Chunk k = load_chunk(d, chunk, list, [&](int32_t p) { return __ldg(a.values + (PERM ? __ldg(d.perm + p) : p)); });
@@ -172,9 +228,9 @@ __global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirVi
 #pragma unroll
     for (int i = 0; i < FE; ++i) {
       const int col = end0 + w * LPR * VE + i;
-      bias[w][i] = a.bias && col < a.N ? __ldg(a.bias + col) : 0.f;
-      idle[w][i] = act_of(bias[w][i], a.act);
+      bias[w][i] = idle[w][i] = a.bias && col < a.N ? __ldg(a.bias + col) : 0.f;
     }
+    act_all(idle[w], a.act);
   }
   int32_t row = k.r0;
   auto request = [&](int32_t r) {  // the residual of a row that ends here
@@ -374,7 +430,7 @@ __device__ __forceinline__ float group_sums(float (&s)[U], int lane, uint32_t ma
 // product with A transposed, whose sums over many rows are rounded to T anyway), dvalues, and the block's share of dbias. The
 // walk is the product kernel's; dout and z of the next row are requested when a row begins.
 template <class T, int VE, int LPR, int VPL, int U, int MINB>
-__global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const DirView d, const GradArgs a) {
+__global__ void __launch_bounds__(kWalk, MINB) act_grad_rows_kernel(const DirView d, const GradArgs a) {
   using V = RowVec<T, VE>;
   using S = Spread<VE, LPR>;
   constexpr int G = S::G, FE = S::FE;
@@ -382,8 +438,8 @@ __global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const Dir
   static_assert(LPR >= U, "a group holds a step's sums");
   constexpr int cols = LPR * VE * VPL;
   __shared__ union {
-    ChunkLists lists[kThreads / 32];
-    float sums[kThreads / 32][cols];
+    ChunkLists lists[kWalk / 32];
+    float sums[kWalk / 32][cols];
   } sm;
   ChunkLists &list = sm.lists[threadIdx.x >> 5];
   const int lane = threadIdx.x % LPR, g = S::part();
@@ -399,9 +455,9 @@ __global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const Dir
   for (int w = 0; w < VPL; ++w)
 #pragma unroll
     for (int i = 0; i < FE; ++i) bsum[w][i] = z[w][i] = 0.f;
-  const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
+  const int64_t warps = (int64_t)gridDim.x * (kWalk / 32);
 #pragma unroll 1
-  for (int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5; chunk < d.n_chunks; chunk += warps) {
+  for (int64_t chunk = ((int64_t)blockIdx.x * kWalk + threadIdx.x) >> 5; chunk < d.n_chunks; chunk += warps) {
     const Chunk k = load_chunk(d, chunk, list, [](int32_t) { return 0.f; });
     const int2 *entry = list.entry - k.p0;
     auto request = [&](int32_t row) {  // dout and z of a row
@@ -427,10 +483,7 @@ __global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const Dir
 #pragma unroll
         for (int w = 0; w < VPL; ++w) {
           F::widen(dout[w], own[w]);
-          if (a.act != DSP_ACT_NONE) {
-#pragma unroll
-            for (int i = 0; i < FE; ++i) own[w][i] *= act_slope(z[w][i], a.act);
-          }
+          act_slopes(own[w], z[w], a.act);
         }
         request(row + 1);
 #pragma unroll
@@ -478,29 +531,31 @@ __global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const Dir
 #pragma unroll
     for (int i = 0; i < FE; ++i) sm.sums[threadIdx.x >> 5][w * LPR * VE + lane * VE + g * FE + i] = bsum[w][i];
   __syncthreads();
-  for (int c = threadIdx.x; c < cols; c += kThreads) {
+  for (int c = threadIdx.x; c < cols; c += kWalk) {
     const int col = blockIdx.y * cols + c;
     if (col >= a.N) continue;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) s += sm.sums[w][c];
+    for (int w = 0; w < kWalk / 32; ++w) s += sm.sums[w][c];
     a.dbias[(int64_t)blockIdx.x * a.N + col] = s;
   }
 }
 
-// out[c] = sum over the n rows of part, in an order that depends on n alone: 32 columns per block, 8 interleaved sums.
-__global__ void __launch_bounds__(kThreads) column_sums_kernel(const float *part, int n, int N, float *out) {
-  __shared__ float s[8][33];
+// out[c] = sum over the n rows of part, in an order that depends on n alone: 32 columns per block, 32 interleaved sums.
+__global__ void __launch_bounds__(1024) column_sums_kernel(const float *part, int n, int N, float *out) {
+  __shared__ float s[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, col = blockIdx.x * 32 + lane;
   float x = 0.f;
-  if (col < N)
-    for (int r = warp; r < n; r += 8) x += part[(int64_t)r * N + col];
+  if (col < N) {
+#pragma unroll 8
+    for (int r = warp; r < n; r += 32) x += part[(int64_t)r * N + col];
+  }
   s[warp][lane] = x;
   __syncthreads();
   if (warp == 0 && col < N) {
     x = 0.f;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) x += s[w][lane];
+    for (int w = 0; w < 32; ++w) x += s[w][lane];
     out[col] = x;
   }
 }
@@ -541,16 +596,16 @@ Shape shape_of(int N, int ve, int size) {
 template <class T, int VE, int LPR, int VPL, bool PERM>
 void run_product(const DirView &d, const ActArgs &a, cudaStream_t s) {
   constexpr int U = VE * VPL >= 16 ? 4 : VE == 4 && VPL == 2 ? 4 : ACT_U, minb = VE * VPL >= 16 ? 2 : ACT_B;
-  const dim3 grid((unsigned)((d.n_chunks + kThreads / 32 - 1) / (kThreads / 32)),
+  const dim3 grid((unsigned)((d.n_chunks + kWalk / 32 - 1) / (kWalk / 32)),
                   (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL)));
-  act_product_kernel<T, VE, LPR, VPL, U, minb, PERM><<<grid, kThreads, 0, s>>>(d, a);
+  act_product_kernel<T, VE, LPR, VPL, U, minb * 256 / kWalk, PERM><<<grid, kWalk, 0, s>>>(d, a);
 }
 
 template <class T, int VE, int LPR, int VPL>
 void run_rows(const DirView &d, const GradArgs &a, int blocks, cudaStream_t s) {
   constexpr int U = GR_U < LPR ? GR_U : 4, minb = VE * VPL >= 16 ? 2 : GR_B;
-  act_grad_rows_kernel<T, VE, LPR, VPL, U, minb>
-      <<<dim3((unsigned)blocks, (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL))), kThreads, 0, s>>>(d, a);
+  act_grad_rows_kernel<T, VE, LPR, VPL, U, minb * 256 / kWalk>
+      <<<dim3((unsigned)blocks, (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL))), kWalk, 0, s>>>(d, a);
 }
 
 // f.template operator()<VE, LPR, VPL>() of a shape.
@@ -662,7 +717,7 @@ GradPlan grad_plan(const dsp_pattern *p, const dsp_act_grad_desc *d) {
   g.shape = shape_of(d->N, al.ve, esize(d->dtype));
   g.col_blocks = (d->N + g.shape.cols() - 1) / g.shape.cols();
   g.blocks = (int)std::max<int64_t>(
-      1, std::min<int64_t>(8ll * p->sms, (p->a.n_chunks + kThreads / 32 - 1) / (kThreads / 32)));
+      1, std::min<int64_t>((int64_t)ACT_G * 256 / kWalk * p->sms, (p->a.n_chunks + kWalk / 32 - 1) / (kWalk / 32)));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -691,7 +746,7 @@ int grad(const dsp_pattern *p, const dsp_act_grad_desc *d, char *ws, cudaStream_
     const DirView rows = view(p->a);
     with_shape<T>(g.shape, GradRows<T>{rows, a, g.blocks, s});
     if (d->dbias)
-      column_sums_kernel<<<(d->N + 31) / 32, kThreads, 0, s>>>((float *)(ws + g.dbias), g.blocks, d->N, d->dbias);
+      column_sums_kernel<<<(d->N + 31) / 32, 1024, 0, s>>>((float *)(ws + g.dbias), g.blocks, d->N, d->dbias);
     if (a.dvalues && g.col_blocks > 1)
       add_blocks_kernel<<<(unsigned)((p->nnz + kThreads - 1) / kThreads), kThreads, 0, s>>>(a.dvalues, g.col_blocks, p->nnz,
                                                                                            d->dvalues);
