@@ -13,7 +13,8 @@
 // back into the same columns as the A operand of the second product, so neither passes through shared memory; the stream's
 // tiles serve both products from one swizzled image (K-major in the first, N-major in the second). The sums over keys stay in
 // tensor memory; the forward pass rescales its own only when a row's maximum grew by more than 2^8 (kSlack), which leaves
-// the result the same (weights and their sum share the stale maximum).
+// the result the same (weights and their sum share the stale maximum). It takes the tiles from the last to the first: under a
+// causal mask with a distance bias scores fall along that way, and the maximum stands after one tile.
 //
 // Rounding: weights enter the second product in the operands' 16-bit type (half a step each; the sum l is of unrounded
 // weights). fp16 has few exponents: weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is
@@ -60,7 +61,7 @@ template <int D, Mode M>
 struct Cfg {
   static constexpr int kStatic = M == kFwd ? 1 : 2;            // stationary operands
   static constexpr int kScores = M == kFwd ? 1 : 2;            // score tiles of 64 columns
-  static constexpr int NB = M == kFwd && D == 128 ? 2 : M != kFwd && D == 128 ? 2 : 1;  // score buffers
+  static constexpr int NB = M == kFwd || D == 128 ? 2 : 1;  // score buffers
   static constexpr int ST = 2;                                 // stages of each streamed operand
   static constexpr int kAcc = kScores * NB * 64;               // first accumulator column
   static constexpr int kUsed = kAcc + (M == kDkv ? 2 : 1) * D;
@@ -107,10 +108,12 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, wait(bar, parity, dead, err, code));
 }
 
-// The last of n phases. When a thread has seen the last scores, the phase n - 3 is over, n - 2 perhaps not: a wait for n - 1
-// alone would take the parity of n - 3 for it.
-__device__ __forceinline__ bool wait_last(uint32_t bar, int n, volatile int *dead, int *err, int code) {
-  return (n < 2 || warp_wait(bar, n & 1, dead, err, code)) && warp_wait(bar, (n - 1) & 1, dead, err, code);
+// The second products of iterations 0, 1, ... complete on kAccBars barriers in turn. A thread waits for some of them only, and a
+// wait tells two phases of a barrier apart by their parity alone: with one barrier, a late thread would take phase n for phase
+// n - 2. On these, the phase before the awaited one is four iterations old and the one after it four ahead.
+constexpr int kAccBars = 4;
+__device__ __forceinline__ bool wait_acc(uint32_t bars, int it, volatile int *dead, int *err, int code) {
+  return warp_wait(bars + 8 * (it % kAccBars), (it / kAccBars) & 1, dead, err, code);
 }
 
 template <class T>
@@ -123,6 +126,77 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&x);
   }
 }
+
+// s -> cap tanh(k s), k = scale / cap, of N columns of this thread's row. Where no score of the warp's rows is above 0.75 of the cap,
+// as is usual, tanh x = x P(x^2) (degree 11, through Chebyshev nodes, within 1.6e-7) leaves the special function units to the
+// softmax; else through the exponential (capped).
+template <int N>
+__device__ __forceinline__ void cap_row(float (&s)[N], float k, float cap, float scale, float inv_cap2) {
+  float top = 0.f;
+#pragma unroll
+  for (int c = 0; c < N; c += 2) {
+    float x0, x1, y0, y1;
+    mul2(x0, x1, s[c], s[c + 1], k, k);
+    mul2(y0, y1, x0, x1, x0, x1);
+    top = max3(top, y0, y1);
+  }
+  if (__all_sync(0xffffffffu, top <= 0.5625f)) {
+    constexpr float P[6] = {0.999999972f, -0.333329667f, 0.133255153f, -0.0533498202f, 0.0195937858f, -0.00472395227f};
+#pragma unroll
+    for (int c = 0; c < N; c += 2) {
+      float x0, x1, y0, y1, q0 = P[5], q1 = P[5];
+      mul2(x0, x1, s[c], s[c + 1], k, k);
+      mul2(y0, y1, x0, x1, x0, x1);
+#pragma unroll
+      for (int i = 4; i >= 0; --i) {
+        float r0 = P[i], r1 = P[i];
+        fma2(r0, r1, q0, q1, y0, y1);
+        q0 = r0, q1 = r1;
+      }
+      mul2(x0, x1, x0, x1, cap, cap);
+      mul2(s[c], s[c + 1], x0, x1, q0, q1);
+    }
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      float th;
+      s[c] = capped(s[c] * scale, cap, inv_cap2, th);
+    }
+  }
+}
+
+// Tiles of the list as a thread of the weights sees them, in the order first, first + step, ...: place and mask two iterations
+// ahead, the row's presence bits one ahead, so that no load is waited for.
+struct TileWalk {
+  const TileView &t;
+  int r, at, left, step, wrap;  // wrap: tiles until the list starts again
+  int mask, col, mask2 = 0, col2 = 0;
+  uint64_t bits;
+  int seen = 0;
+  __device__ __forceinline__ uint64_t words(int m) const {
+    return m < 0 ? ~0ull : __ldg(t.words + (int64_t)m * kTileRows + r);
+  }
+  __device__ __forceinline__ TileWalk(const TileView &t_, int first, int step_, int n, int total, int r_)
+      : t(t_), r(r_), at(first), left(total), step(step_), wrap(n) {
+    mask = col = 0, bits = 0;
+    if (left > 0) {
+      mask = __ldg(t.mask + at), col = __ldg(t.col + at);
+      next2();
+      bits = words(mask);
+    }
+  }
+  __device__ __forceinline__ void next2() {  // place and mask of the tile after the present one
+    if (--left <= 0) return;
+    at += step;
+    if (++seen == wrap) seen = 0, at -= step * wrap;
+    mask2 = __ldg(t.mask + at), col2 = __ldg(t.col + at);
+  }
+  __device__ __forceinline__ void advance() {
+    mask = mask2, col = col2;
+    bits = words(mask);
+    next2();
+  }
+};
 
 // Rows of a warp whose result is not finite (bits of `bad`), again by gather.
 template <class T, int D, Mode M>
@@ -187,10 +261,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
   constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr int NB = C::NB, ST = C::ST;
   extern __shared__ uint8_t raw_smem[];
-  __shared__ uint64_t bars[1 + 4 * ST + 2 * NB + 2];
+  __shared__ uint64_t bars[1 + 4 * ST + 2 * NB + kAccBars + 1];
   __shared__ uint32_t tmem_result;
   __shared__ int dead_flag;
-  __shared__ float2 row_stats[2][64];  // dk, dv: lse (base 2) and delta of the streamed rows
+  __shared__ __align__(16) float row_lse[2][64], row_delta[2][64];  // dk, dv: -lse (base 2) and -delta of the streamed rows
   volatile int *dead = &dead_flag;
 
   const int warp = threadIdx.x >> 5;
@@ -211,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
   const uint32_t b0 = smem_addr(bars);
   const uint32_t bar_static = b0, bar_x0_full = b0 + 8, bar_x0_free = bar_x0_full + 8 * ST, bar_x1_full = bar_x0_free + 8 * ST,
                  bar_x1_free = bar_x1_full + 8 * ST, bar_scores = bar_x1_free + 8 * ST, bar_weights = bar_scores + 8 * NB,
-                 bar_acc = bar_weights + 8 * NB, bar_stats = bar_acc + 8;
+                 bar_acc = bar_weights + 8 * NB, bar_stats = bar_acc + 8 * kAccBars;
 
   if (iters > 0 && warp == 5) tmem_alloc(smem_addr(&tmem_result), C::kCols);
   if (threadIdx.x == 0) {
@@ -227,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
       mbar_init(bar_scores + 8 * i, 1);
       mbar_init(bar_weights + 8 * i, kWeightThreads);
     }
-    mbar_init(bar_acc, 1);
+    for (int i = 0; i < kAccBars; ++i) mbar_init(bar_acc + 8 * i, 1);
     mbar_init(bar_stats, kWeightThreads);
     mbar_fence_init();
   }
@@ -245,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         if (C::kStatic == 2) tma_load3(sm_a1 + c * 16384, &map_a1, c * 64, head_a, (int)row0, bar_static);
       }
       for (int it = 0; it < iters; ++it) {
-        const int s = it % ST, col = __ldg(x.t.col + t0 + it % nt) * kTileCols;
+        const int s = it % ST, col = __ldg(x.t.col + (M == kFwd ? t1 - 1 - it : t0 + it % nt)) * kTileCols;
         const uint32_t parity = ((it / ST) & 1) ^ 1;
         const int hx = M == kDkv ? head * x.a.group + it / nt : head / x.a.group;
         if (!wait(bar_x0_free + 8 * s, parity, dead, x.err, 1)) break;
@@ -305,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         }
         if (M != kFwd) mma_commit(bar_x0_free + 8 * s);
         if (M != kDq) mma_commit(bar_x1_free + 8 * s);
-        mma_commit(bar_acc);
+        mma_commit(bar_acc + 8 * (it % kAccBars));
         return true;
       };
       bool ok = wait(bar_static, 0, dead, x.err, 7);
@@ -327,21 +401,19 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
     const float cap = x.a.cap, inv_cap2 = cap > 0.f ? 2.f * kLog2e / cap : 0.f;
     const float scale2 = x.a.scale * kLog2e;
     bool ok = true;
-    // the score of streamed row c of the tile, base 2; d0 + c * step: the signed distance
-    auto score = [&](float dot, float slope2, float dist, float &th) {
-      float u;
-      if (cap > 0.f) u = capped(dot * x.a.scale, cap, inv_cap2, th) * kLog2e;
-      else u = dot * scale2;
-      return fmaf(-slope2, fabsf(dist), u);
-    };
+    const float cap_k = cap > 0.f ? x.a.scale / cap : 0.f;
+    // scores of base 2 are f s - slope2 |distance|, s: as the product left them, or capped
+    const float f = cap > 0.f ? kLog2e : scale2;
+    TileWalk walk(x.t, M == kFwd ? t1 - 1 : t0, M == kFwd ? -1 : 1, nt, iters, r);
     if constexpr (M == kFwd) {
       constexpr float kUp = kBf16 ? 0.f : 6.f;
       const float slope2 = x.a.slopes ? __ldg(x.a.slopes + head) * kLog2e : 0.f;
       float m = -INFINITY, l = 0.f;  // weights are exp2(u - m); m lies kUp below a maximum of the row
       for (int it = 0; it < iters; ++it) {
-        const int b = it % NB, t = t0 + it, mi = __ldg(x.t.mask + t);
-        const uint64_t bits = mi < 0 ? ~0ull : __ldg(x.t.words + (int64_t)mi * kTileRows + r);
-        const float d0 = (float)(row + x.a.row_offset - (int64_t)__ldg(x.t.col + t) * kTileCols);
+        const int b = it % NB;
+        const int now_mask = walk.mask, now_col = walk.col;
+        const uint64_t now_bits = walk.bits;
+        walk.advance();
         if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x.err, 8))) break;
         tc_fence_after();
         float u[64];
@@ -353,18 +425,23 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
 #pragma unroll
           for (int c = 0; c < 32; ++c) u[c] = __uint_as_float(lo[c]), u[c + 32] = __uint_as_float(hi[c]);
         }
-        if (cap > 0.f || slope2 != 0.f) {
+        if (cap > 0.f) cap_row(u, cap_k, cap, x.a.scale, inv_cap2);
+        float fu = f;  // what is left to multiply with; a factor of 0 would make NaN of a masked -infinity below
+        if (slope2 != 0.f || f <= 0.f) {
+          // -slope2 |d0 - c| = -+ |slope2 c - slope2 d0|
+          const float k0 = -slope2 * (float)(row + x.a.row_offset - (int64_t)now_col * kTileCols), sign = slope2 < 0.f ? 1.f : -1.f;
 #pragma unroll
-          for (int c = 0; c < 64; ++c) {
-            float th;
-            u[c] = score(u[c], slope2, d0 - (float)c, th);
+          for (int c = 0; c < 64; c += 2) {
+            float x0 = k0, x1 = k0;
+            fma2(x0, x1, (float)c, (float)(c + 1), slope2, slope2);
+            x0 = sign * fabsf(x0), x1 = sign * fabsf(x1);
+            fma2(x0, x1, u[c], u[c + 1], f, f);
+            u[c] = x0, u[c + 1] = x1;
           }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 64; ++c) u[c] *= scale2;
+          fu = 1.f;
         }
-        if (mi >= 0) {
-          const uint32_t lo = (uint32_t)bits, hi = (uint32_t)(bits >> 32);
+        if (now_mask >= 0) {
+          const uint32_t lo = (uint32_t)now_bits, hi = (uint32_t)(now_bits >> 32);
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
             u[c] = lo & (1u << c) ? u[c] : -INFINITY;
@@ -373,15 +450,20 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         }
         float top[4] = {u[0], u[1], u[2], u[3]};
 #pragma unroll
-        for (int c = 4; c < 64; ++c) top[c & 3] = fmaxf(top[c & 3], u[c]);
-        const float mt = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) - kUp;
+        for (int c = 4; c < 60; c += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top[k] = max3(top[k], u[c + k], u[c + 4 + k]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], u[60 + k]);
+        const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        const float mt = best == -INFINITY ? best : fmaf(best, fu, -kUp);
         const bool grow = mt > m + kSlack || (m == -INFINITY && mt > m);
         if (__any_sync(0xffffffffu, grow)) {
-          const float m2 = grow ? mt : m, f = grow ? exp2_approx(m - m2) : 1.f;
+          const float m2 = grow ? mt : m, less = grow ? exp2_approx(m - m2) : 1.f;
           m = m2;
-          l *= f;
+          l *= less;
           if (it > 0) {  // the sum so far, once the previous product has been added to it
-            if (!(ok = warp_wait(bar_acc, (it - 1) & 1, dead, x.err, 9))) break;
+            if (!(ok = wait_acc(bar_acc, it - 1, dead, x.err, 9))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -389,18 +471,21 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
               tmem_ld32(tm_acc0 + lanes + c, w);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * f);
+              for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(__uint_as_float(w[i]) * less);
               tmem_st32(tm_acc0 + lanes + c, w);
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        const float base = m == -INFINITY ? 0.f : -m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         uint32_t w[32];
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          const float p0 = exp2_approx(u[2 * c] - base), p1 = exp2_approx(u[2 * c + 1] - base);
-          sum[c & 3] += p0 + p1;
+          float p0 = base, p1 = base;
+          fma2(p0, p1, u[2 * c], u[2 * c + 1], fu, fu);
+          p0 = exp2_approx(p0), p1 = exp2_approx(p1);
+          const int k = 2 * (c & 1);
+          add2(sum[k], sum[k + 1], sum[k], sum[k + 1], p0, p1);
           w[c] = pack2<T>(p0, p1);
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
@@ -409,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         tc_fence_before();
         mbar_arrive(bar_weights + 8 * b);
       }
-      if (ok && iters > 0) ok = wait_last(bar_acc, iters, dead, x.err, 10);
+      if (ok && iters > 0) ok = wait_acc(bar_acc, iters - 1, dead, x.err, 10);
       tc_fence_after();
       const bool live = row < n_rows;
       if (ok && x.splits > 1) {
@@ -446,6 +531,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         const int e = (int)(__ldg(x.dout_max) >> 23);  // biased exponent; 255: not finite
         if (e > 0 && e < 255) up = __uint_as_float((uint32_t)min(max(127 + 4 - (e - 127), 1), 254) << 23);
       }
+      const float down = x.a.scale / up;
+      if (M == kDkv && !kBf16) up *= 0x1p-12f;  // the weights of dk, dv are 2^12 up themselves
       constexpr float kUp = kBf16 ? 0.f : 12.f;
       const bool live = row < n_rows;
       float lse2 = INFINITY, delta = 0.f;
@@ -454,81 +541,132 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without entries: weights of 0
         delta = x.a.delta[row * x.a.heads + head];
       }
+      // dk, dv: lse and delta of streamed row r of the tile (threads below 64), requested one iteration ahead
+      float next_lse = 0.f, next_delta = 0.f;
+      auto request_stats = [&](int col, int h) {
+        const int64_t q = (int64_t)col * kTileCols + r;
+        next_lse = -INFINITY, next_delta = 0.f;
+        if (r < 64 && q < x.a.n_queries) {
+          next_lse = x.a.lse[q * x.a.heads + h];
+          next_delta = x.a.delta[q * x.a.heads + h];
+        }
+      };
+      if (M == kDkv && iters > 0) request_stats(walk.col, head * x.a.group);
       for (int it = 0; it < iters; ++it) {
-        const int b = it % NB, t = t0 + it % nt, mi = __ldg(x.t.mask + t);
-        const uint64_t bits = mi < 0 ? ~0ull : __ldg(x.t.words + (int64_t)mi * kTileRows + r);
-        const int64_t col = (int64_t)__ldg(x.t.col + t) * kTileCols;
+        const int b = it % NB;
+        const int now_mask = walk.mask, now_col = walk.col;
+        const uint64_t now_bits = walk.bits;
+        walk.advance();
         const int h = M == kDkv ? head * x.a.group + it / nt : head;
-        const float slope2 = x.a.slopes ? __ldg(x.a.slopes + h) * kLog2e : 0.f;
-        // query position - key position; along the columns it falls (dq: columns are keys) or rises (dk, dv: queries)
-        const float d0 = M == kDq ? (float)(row + x.a.row_offset - col) : (float)(col + x.a.row_offset - row);
         if (M == kDkv) {
-          if (r < 64) {
-            const int64_t q = col + r;
-            float2 st = make_float2(INFINITY, 0.f);
-            if (q < x.a.n_queries) {
-              st.x = x.a.lse[q * x.a.heads + h] * kLog2e;
-              if (st.x == -INFINITY) st.x = INFINITY;
-              st.x -= kUp;
-              st.y = x.a.delta[q * x.a.heads + h];
-            }
-            row_stats[it & 1][r] = st;
+          if (r < 64) {  // a row without entries (lse = -infinity): weights of 0
+            row_lse[it & 1][r] = next_lse == -INFINITY ? -INFINITY : fmaf(next_lse, -kLog2e, kUp);
+            row_delta[it & 1][r] = -next_delta;
           }
           mbar_arrive(bar_stats);
-          if (!(ok = warp_wait(bar_stats, it & 1, dead, x.err, 13))) break;
         }
+        if (M == kDkv && it + 1 < iters) request_stats(walk.col, head * x.a.group + (it + 1) / nt);
+        const float slope2 = x.a.slopes ? __ldg(x.a.slopes + h) * kLog2e : 0.f;
+        // -slope2 |distance| = sign |slope2 c + k0|, c the column
+        const int64_t col = (int64_t)now_col * kTileCols;
+        const float k0 = slope2 * (M == kDq ? -(float)(row + x.a.row_offset - col) : (float)(col + x.a.row_offset - row));
+        const float sign = slope2 < 0.f ? 1.f : -1.f;
+        if (M == kDkv && !(ok = warp_wait(bar_stats, it & 1, dead, x.err, 13))) break;
         if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x.err, 11))) break;
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-          uint32_t s[32], e[32];
-          tmem_ld32(tm_s + lanes + b * 64 + half * 32, s);
-          tmem_ld32(tm_r + lanes + b * 64 + half * 32, e);
-          tmem_wait_ld();
-          const uint32_t bit = half ? (uint32_t)(bits >> 32) : (uint32_t)bits;
-          uint32_t w[16], v[16];
+          float s[32], e[32], p[32];
+          {
+            uint32_t s_raw[32], e_raw[32];
+            tmem_ld32(tm_s + lanes + b * 64 + half * 32, s_raw);
+            tmem_ld32(tm_r + lanes + b * 64 + half * 32, e_raw);
+            tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            float p[2], g[2];
+            for (int c = 0; c < 32; ++c) s[c] = __uint_as_float(s_raw[c]), e[c] = __uint_as_float(e_raw[c]);
+          }
+          if (cap > 0.f) cap_row(s, cap_k, cap, x.a.scale, inv_cap2);
+          const float *stat_lse = row_lse[it & 1] + half * 32, *stat_delta = row_delta[it & 1] + half * 32;
+          // weights
+          if (slope2 != 0.f) {
+            const float kh = fmaf(slope2, (float)(half * 32), k0);
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int cc = half * 32 + c + k;
-              float th = 0.f, lse_c = lse2, delta_c = delta;
+            for (int c = 0; c < 32; c += 2) {
+              p[c] = p[c + 1] = kh;
+              fma2(p[c], p[c + 1], (float)c, (float)(c + 1), slope2, slope2);
+              p[c] = sign * fabsf(p[c]), p[c + 1] = sign * fabsf(p[c + 1]);
+              fma2(p[c], p[c + 1], s[c], s[c + 1], f, f);
               if (M == kDkv) {
-                const float2 st = row_stats[it & 1][cc];
-                lse_c = st.x, delta_c = st.y;
+                const float2 l = *reinterpret_cast<const float2 *>(stat_lse + c);
+                add2(p[c], p[c + 1], p[c], p[c + 1], l.x, l.y);
+              } else {
+                add2(p[c], p[c + 1], p[c], p[c + 1], -lse2, -lse2);
               }
-              float u = score(__uint_as_float(s[c + k]), slope2, M == kDq ? d0 - (float)cc : d0 + (float)cc, th);
-              p[k] = exp2_approx(u - lse_c);
-              g[k] = p[k] * (__uint_as_float(e[c + k]) - delta_c) * up;
-              if (cap > 0.f) g[k] *= 1.f - th * th;
-              if (M == kDkv && !kBf16) g[k] *= 0x1p-12f;
-              if (!(bit & (1u << (c + k)))) p[k] = g[k] = 0.f;
+              p[c] = exp2_approx(p[c]), p[c + 1] = exp2_approx(p[c + 1]);
             }
-            if (M == kDkv) w[c / 2] = pack2<T>(p[0], p[1]);
-            v[c / 2] = pack2<T>(g[0], g[1]);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              p[c] = p[c + 1] = -lse2;
+              if (M == kDkv) {
+                const float2 l = *reinterpret_cast<const float2 *>(stat_lse + c);
+                p[c] = l.x, p[c + 1] = l.y;
+              }
+              fma2(p[c], p[c + 1], s[c], s[c + 1], f, f);
+              p[c] = exp2_approx(p[c]), p[c + 1] = exp2_approx(p[c + 1]);
+            }
+          }
+          if (now_mask >= 0) {
+            const uint32_t bit = half ? (uint32_t)(now_bits >> 32) : (uint32_t)now_bits;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) p[c] = bit & (1u << c) ? p[c] : 0.f;
           }
           if (M == kDkv) {
+            uint32_t w[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) w[c / 2] = pack2<T>(p[c], p[c + 1]);
             tmem_st16(tm_s + lanes + b * 64 + half * 16, w);
-            tmem_st16(tm_r + lanes + b * 64 + half * 16, v);
-          } else {
-            tmem_st16(tm_s + lanes + b * 64 + half * 16, v);
           }
+          // score gradients: p (dp - delta) (1 - tanh^2), up to the scale
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float d0 = -delta, d1 = -delta;
+            if (M == kDkv) {
+              const float2 l = *reinterpret_cast<const float2 *>(stat_delta + c);
+              d0 = l.x, d1 = l.y;
+            }
+            add2(e[c], e[c + 1], e[c], e[c + 1], d0, d1);
+            if (!kBf16) mul2(e[c], e[c + 1], e[c], e[c + 1], up, up);
+            mul2(e[c], e[c + 1], e[c], e[c + 1], p[c], p[c + 1]);
+          }
+          if (cap > 0.f) {
+            const float inv = -1.f / (cap * cap);
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              float y0, y1, z0 = 1.f, z1 = 1.f;
+              mul2(y0, y1, s[c], s[c + 1], s[c], s[c + 1]);
+              fma2(z0, z1, y0, y1, inv, inv);
+              mul2(e[c], e[c + 1], e[c], e[c + 1], z0, z1);
+            }
+          }
+          uint32_t v[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) v[c / 2] = pack2<T>(e[c], e[c + 1]);
+          tmem_st16((M == kDkv ? tm_r : tm_s) + lanes + b * 64 + half * 16, v);
         }
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(bar_weights + 8 * b);
       }
-      if (ok && iters > 0) ok = wait_last(bar_acc, iters, dead, x.err, 12);
+      if (ok && iters > 0) ok = wait_acc(bar_acc, iters - 1, dead, x.err, 12);
       tc_fence_after();
-      const float f = x.a.scale / up;
       if (ok && iters > 0) {
         bool fine;
         if constexpr (M == kDq) {
-          fine = put_acc<T, D>(tm_acc0 + lanes, f, x.a.dq, row, head, live);
+          fine = put_acc<T, D>(tm_acc0 + lanes, down, x.a.dq, row, head, live);
         } else {
           fine = put_acc<T, D>(tm_acc0 + lanes, kBf16 ? 1.f : 0x1p-12f, x.a.dv, row, head, live);
-          fine = put_acc<T, D>(tm_acc1 + lanes, f, x.a.dk, row, head, live) && fine;
+          fine = put_acc<T, D>(tm_acc1 + lanes, down, x.a.dk, row, head, live) && fine;
         }
         const uint32_t bad = __ballot_sync(0xffffffffu, live && !fine);
         if (bad) redo<T, D, M>(x, row0 + 32 * warp, head, bad);

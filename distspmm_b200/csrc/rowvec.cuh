@@ -85,6 +85,22 @@ __device__ __forceinline__ void fma2(float &c0, float &c1, float a0, float a1, f
       : "+f"(c0), "+f"(c1)
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
+// c = a + b, c = a b of pairs.
+__device__ __forceinline__ void add2(float &c0, float &c1, float a0, float a1, float b0, float b1) {
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 c, a, b;\n mov.b64 {%0, %1}, c;\n}"
+      : "=f"(c0), "=f"(c1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void mul2(float &c0, float &c1, float a0, float a1, float b0, float b1) {
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 c, a, b;\n mov.b64 {%0, %1}, c;\n}"
+      : "=f"(c0), "=f"(c1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
 // acc += x * row
 template <class T, int VE>
 __device__ __forceinline__ void fma_row(float (&acc)[VE], float x, typename RowVec<T, VE>::Raw r) {

@@ -54,6 +54,7 @@ def check(a, heads, kv, dim, t, cap=0.0, bias=False, offset=0, grad=True, seed=0
         for name, x, y in zip(("dq", "dk", "dv"), got, grads):
             assert x.dtype == t
             near(x, y, tol[name], name)
+    p.check_error()  # no bounded wait gave up
     return p
 
 
