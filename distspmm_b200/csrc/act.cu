@@ -55,9 +55,7 @@ __device__ __forceinline__ void normal2(float z0, float z1, float &c0, float &c1
   float q0 = Q[9], q1 = Q[9];
 #pragma unroll
   for (int i = 8; i >= 0; --i) {
-    float r0 = Q[i], r1 = Q[i];
-    fma2(r0, r1, q0, q1, t0, t1);
-    q0 = r0, q1 = r1;
+    fma2(q0, q1, q0, q1, t0, t1, Q[i], Q[i]);
   }
   c0 = 0.5f * t0 * q0 * e0, c1 = 0.5f * t1 * q1 * e1;
   c0 = z0 > 0.f ? 1.f - c0 : c0, c1 = z1 > 0.f ? 1.f - c1 : c1;

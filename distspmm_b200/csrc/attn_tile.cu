@@ -127,34 +127,39 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
-// s -> cap tanh(k s), k = scale / cap, of N columns of this thread's row. Where no score of the warp's rows is above 0.75 of the cap,
-// as is usual, tanh x = x P(x^2) (degree 11, through Chebyshev nodes, within 1.6e-7) leaves the special function units to the
-// softmax; else through the exponential (capped).
+// s -> cap tanh(k s), k = scale / cap, of N columns of this thread's row. Where no score of the warp's rows is above half the cap, as
+// is usual, tanh x = x P(x^2) (degree 9, through Chebyshev nodes, within 1.2e-7) leaves the special function units to the
+// softmax, with k and the cap in the coefficients: 6 operations an element; else through the exponential (capped).
+struct CapPoly {
+  float limit, c[5];  // of s^2; s (c0 + c1 s^2 + ...)
+  __device__ __forceinline__ CapPoly(float scale, float cap) {
+    const float k = cap > 0.f ? scale / cap : 0.f, k2 = k * k;
+    limit = k2 > 0.f ? 0.25f / k2 : INFINITY;
+    float f = k * cap;
+    c[0] = 0.999999987f * f;
+    c[1] = -0.333330719f * (f *= k2);
+    c[2] = 0.13324829f * (f *= k2);
+    c[3] = -0.0529892412f * (f *= k2);
+    c[4] = 0.017141319f * (f *= k2);
+  }
+};
 template <int N>
-__device__ __forceinline__ void cap_row(float (&s)[N], float k, float cap, float scale, float inv_cap2) {
-  float top = 0.f;
+__device__ __forceinline__ void cap_row(float (&s)[N], const CapPoly &p, float cap, float scale, float inv_cap2) {
+  float y[N], top = 0.f;
 #pragma unroll
   for (int c = 0; c < N; c += 2) {
-    float x0, x1, y0, y1;
-    mul2(x0, x1, s[c], s[c + 1], k, k);
-    mul2(y0, y1, x0, x1, x0, x1);
-    top = max3(top, y0, y1);
+    mul2(y[c], y[c + 1], s[c], s[c + 1], s[c], s[c + 1]);
+    top = max3(top, y[c], y[c + 1]);
   }
-  if (__all_sync(0xffffffffu, top <= 0.5625f)) {
-    constexpr float P[6] = {0.999999972f, -0.333329667f, 0.133255153f, -0.0533498202f, 0.0195937858f, -0.00472395227f};
+  if (__all_sync(0xffffffffu, top <= p.limit)) {
 #pragma unroll
     for (int c = 0; c < N; c += 2) {
-      float x0, x1, y0, y1, q0 = P[5], q1 = P[5];
-      mul2(x0, x1, s[c], s[c + 1], k, k);
-      mul2(y0, y1, x0, x1, x0, x1);
-#pragma unroll
-      for (int i = 4; i >= 0; --i) {
-        float r0 = P[i], r1 = P[i];
-        fma2(r0, r1, q0, q1, y0, y1);
-        q0 = r0, q1 = r1;
-      }
-      mul2(x0, x1, x0, x1, cap, cap);
-      mul2(s[c], s[c + 1], x0, x1, q0, q1);
+      float q0, q1;
+      fma2(q0, q1, p.c[4], p.c[4], y[c], y[c + 1], p.c[3], p.c[3]);
+      fma2(q0, q1, q0, q1, y[c], y[c + 1], p.c[2], p.c[2]);
+      fma2(q0, q1, q0, q1, y[c], y[c + 1], p.c[1], p.c[1]);
+      fma2(q0, q1, q0, q1, y[c], y[c + 1], p.c[0], p.c[0]);
+      mul2(s[c], s[c + 1], s[c], s[c + 1], q0, q1);
     }
   } else {
 #pragma unroll
@@ -173,9 +178,8 @@ struct TileWalk {
   int mask, col, mask2 = 0, col2 = 0;
   uint64_t bits;
   int seen = 0;
-  __device__ __forceinline__ uint64_t words(int m) const {
-    return m < 0 ? ~0ull : __ldg(t.words + (int64_t)m * kTileRows + r);
-  }
+  // full tiles read their words too: a choice between loaded and constant bits would wait for the load
+  __device__ __forceinline__ uint64_t words(int m) const { return __ldg(t.words + (int64_t)m * kTileRows + r); }
   __device__ __forceinline__ TileWalk(const TileView &t_, int first, int step_, int n, int total, int r_)
       : t(t_), r(r_), at(first), left(total), step(step_), wrap(n) {
     mask = col = 0, bits = 0;
@@ -401,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
     const float cap = x.a.cap, inv_cap2 = cap > 0.f ? 2.f * kLog2e / cap : 0.f;
     const float scale2 = x.a.scale * kLog2e;
     bool ok = true;
-    const float cap_k = cap > 0.f ? x.a.scale / cap : 0.f;
+    const CapPoly cap_poly(x.a.scale, cap);
     // scores of base 2 are f s - slope2 |distance|, s: as the product left them, or capped
     const float f = cap > 0.f ? kLog2e : scale2;
     TileWalk walk(x.t, M == kFwd ? t1 - 1 : t0, M == kFwd ? -1 : 1, nt, iters, r);
@@ -413,34 +417,40 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         const int b = it % NB;
         const int now_mask = walk.mask, now_col = walk.col;
         const uint64_t now_bits = walk.bits;
-        walk.advance();
         if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x.err, 8))) break;
         tc_fence_after();
         float u[64];
         {
-          uint32_t lo[32], hi[32];
-          tmem_ld32(tm_s + lanes + b * 64, lo);
-          tmem_ld32(tm_s + lanes + b * 64 + 32, hi);
+          uint32_t raw[2][32];
+          tmem_ld32(tm_s + lanes + b * 64, raw[0]);
+          tmem_ld32(tm_s + lanes + b * 64 + 32, raw[1]);
+          walk.advance();  // while they come
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) u[c] = __uint_as_float(lo[c]), u[c + 32] = __uint_as_float(hi[c]);
+          for (int half = 0; half < 2; ++half) {
+            float part[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) part[c] = __uint_as_float(raw[half][c]);
+            if (cap > 0.f) cap_row(part, cap_poly, cap, x.a.scale, inv_cap2);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) u[half * 32 + c] = part[c];
+          }
         }
-        if (cap > 0.f) cap_row(u, cap_k, cap, x.a.scale, inv_cap2);
         float fu = f;  // what is left to multiply with; a factor of 0 would make NaN of a masked -infinity below
         if (slope2 != 0.f || f <= 0.f) {
           // -slope2 |d0 - c| = -+ |slope2 c - slope2 d0|
           const float k0 = -slope2 * (float)(row + x.a.row_offset - (int64_t)now_col * kTileCols), sign = slope2 < 0.f ? 1.f : -1.f;
 #pragma unroll
           for (int c = 0; c < 64; c += 2) {
-            float x0 = k0, x1 = k0;
-            fma2(x0, x1, (float)c, (float)(c + 1), slope2, slope2);
+            float x0, x1;
+            fma2(x0, x1, (float)c, (float)(c + 1), slope2, slope2, k0, k0);
             x0 = sign * fabsf(x0), x1 = sign * fabsf(x1);
             fma2(x0, x1, u[c], u[c + 1], f, f);
             u[c] = x0, u[c + 1] = x1;
           }
           fu = 1.f;
         }
-        if (now_mask >= 0) {
+        if (now_mask != 0) {
           const uint32_t lo = (uint32_t)now_bits, hi = (uint32_t)(now_bits >> 32);
 #pragma unroll
           for (int c = 0; c < 32; ++c) {
@@ -481,8 +491,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         uint32_t w[32];
 #pragma unroll
         for (int c = 0; c < 32; ++c) {
-          float p0 = base, p1 = base;
-          fma2(p0, p1, u[2 * c], u[2 * c + 1], fu, fu);
+          float p0, p1;
+          fma2(p0, p1, u[2 * c], u[2 * c + 1], fu, fu, base, base);
           p0 = exp2_approx(p0), p1 = exp2_approx(p1);
           const int k = 2 * (c & 1);
           add2(sum[k], sum[k + 1], sum[k], sum[k + 1], p0, p1);
@@ -585,15 +595,14 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
 #pragma unroll
             for (int c = 0; c < 32; ++c) s[c] = __uint_as_float(s_raw[c]), e[c] = __uint_as_float(e_raw[c]);
           }
-          if (cap > 0.f) cap_row(s, cap_k, cap, x.a.scale, inv_cap2);
+          if (cap > 0.f) cap_row(s, cap_poly, cap, x.a.scale, inv_cap2);
           const float *stat_lse = row_lse[it & 1] + half * 32, *stat_delta = row_delta[it & 1] + half * 32;
           // weights
           if (slope2 != 0.f) {
             const float kh = fmaf(slope2, (float)(half * 32), k0);
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-              p[c] = p[c + 1] = kh;
-              fma2(p[c], p[c + 1], (float)c, (float)(c + 1), slope2, slope2);
+              fma2(p[c], p[c + 1], (float)c, (float)(c + 1), slope2, slope2, kh, kh);
               p[c] = sign * fabsf(p[c]), p[c + 1] = sign * fabsf(p[c + 1]);
               fma2(p[c], p[c + 1], s[c], s[c + 1], f, f);
               if (M == kDkv) {
@@ -607,16 +616,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
           } else {
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-              p[c] = p[c + 1] = -lse2;
-              if (M == kDkv) {
-                const float2 l = *reinterpret_cast<const float2 *>(stat_lse + c);
-                p[c] = l.x, p[c + 1] = l.y;
-              }
-              fma2(p[c], p[c + 1], s[c], s[c + 1], f, f);
+              float2 l = make_float2(-lse2, -lse2);
+              if (M == kDkv) l = *reinterpret_cast<const float2 *>(stat_lse + c);
+              fma2(p[c], p[c + 1], s[c], s[c + 1], f, f, l.x, l.y);
               p[c] = exp2_approx(p[c]), p[c + 1] = exp2_approx(p[c + 1]);
             }
           }
-          if (now_mask >= 0) {
+          if (now_mask != 0) {
             const uint32_t bit = half ? (uint32_t)(now_bits >> 32) : (uint32_t)now_bits;
 #pragma unroll
             for (int c = 0; c < 32; ++c) p[c] = bit & (1u << c) ? p[c] : 0.f;
@@ -643,9 +649,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             const float inv = -1.f / (cap * cap);
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-              float y0, y1, z0 = 1.f, z1 = 1.f;
+              float y0, y1, z0, z1;
               mul2(y0, y1, s[c], s[c + 1], s[c], s[c + 1]);
-              fma2(z0, z1, y0, y1, inv, inv);
+              fma2(z0, z1, y0, y1, inv, inv, 1.f, 1.f);
               mul2(e[c], e[c + 1], e[c], e[c + 1], z0, z1);
             }
           }

@@ -107,19 +107,20 @@ bool build_tiles(int32_t n, int32_t n_cols, const HostDir &d, bool always, HostT
     }
   }, 8);
   if (no_memory.load()) throw std::bad_alloc();
-  int32_t masks = 0;
+  int32_t masks = 0;  // words of tile k < masks hold a kept mask
   for (int64_t k = 0; k < count; ++k) {
     const uint64_t *w = &words[(size_t)k * kTileRows];
     bool full = true;
     for (int r = 0; r < kTileRows; ++r) full &= w[r] == ~0ull;
-    o.mask[k] = full ? -1 : masks;
+    o.mask[k] = full ? 0 : masks + 1;
     if (!full) {
       if (masks != k) std::copy(w, w + kTileRows, &words[(size_t)masks * kTileRows]);
       ++masks;
     }
   }
   words.resize((size_t)masks * kTileRows);
-  o.words = std::move(words);
+  o.words.assign(kTileRows, ~0ull);  // number 0: the full tile
+  o.words.insert(o.words.end(), words.begin(), words.end());
   o.order.resize(nt);
   for (int32_t t = 0; t < nt; ++t) o.order[t] = t;
   std::stable_sort(o.order.begin(), o.order.end(),

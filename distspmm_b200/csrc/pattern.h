@@ -60,14 +60,14 @@ struct HostDir {
 void pattern_chunks(int32_t n, HostDir *d);
 
 // The tile form: tiles of kTileRows x kTileCols entries that hold at least one entry, by row tiles, columns rising. A tile
-// with gaps has a 64-bit word of presence bits for each of its rows; a full one (mask = -1) has none.
+// with gaps has a 64-bit word of presence bits for each of its rows; the full ones share mask 0, all ones.
 constexpr int kTileRows = 128, kTileCols = 64;
 struct PatternTiles {
   int32_t n = 0, max_tiles = 0;  // row tiles; tiles of the longest one
   int64_t count = 0;
   int32_t *ptr = nullptr;     // [n + 1]
   int32_t *col = nullptr;     // [count] column tile
-  int32_t *mask = nullptr;    // [count] words + 128 * mask, or -1
+  int32_t *mask = nullptr;    // [count] its words at 128 * mask; 0: full
   int32_t *order = nullptr;   // [n] row tiles, longest first
   uint64_t *words = nullptr;
 };

@@ -85,6 +85,13 @@ __device__ __forceinline__ void fma2(float &c0, float &c1, float a0, float a1, f
       : "+f"(c0), "+f"(c1)
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
 }
+// d = a b + c of pairs (a c that is used again, such as a constant, needs no copy).
+__device__ __forceinline__ void fma2(float &d0, float &d1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n .reg .b64 a, b, c, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n fma.rn.f32x2 d, a, b, c;\n "
+      "mov.b64 {%0, %1}, d;\n}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
 // c = a + b, c = a b of pairs.
 __device__ __forceinline__ void add2(float &c0, float &c1, float a0, float a1, float b0, float b1) {
   asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 c, a, b;\n mov.b64 {%0, %1}, c;\n}"
