@@ -32,9 +32,9 @@ CXX = os.environ.get("CXX", "g++")
 CXX_FLAGS = ["-O3", "-fPIC", "-std=c++17", "-ffp-contract=off", "-pthread", "-Wall",
              "-I" + os.path.join(ROOT, "include"), "-I" + os.path.join(os.path.dirname(NVCC), "..", "include")]
 
-CU_SOURCES = ["spmm.cu", "rank.cu", "fetch.cu", "setup.cu", "pattern.cu", "act.cu", "attn.cu", "attn_tile.cu", "attn_decode.cu"]
+CU_SOURCES = ["spmm.cu", "rank.cu", "fetch.cu", "setup.cu", "pattern.cu", "act.cu", "attn.cu", "attn_tile.cu", "attn_decode.cu", "attn_graph.cu"]
 CPP_SOURCES = ["host_csr.cpp", "host_gen.cpp", "host_plan.cpp", "run.cpp", "run_rank.cpp", "store.cpp"]
-HEADERS = ["common.h", "internal.h", "device.cuh", "pattern.h", "rowvec.cuh", "attn.h", "attn_row.cuh", "attn_tile.h", "attn_decode.h", "tcgen05.cuh", "mbar.cuh"]
+HEADERS = ["common.h", "internal.h", "device.cuh", "pattern.h", "rowvec.cuh", "attn.h", "attn_row.cuh", "attn_tile.h", "attn_decode.h", "attn_graph.h", "frag.cuh", "tcgen05.cuh", "mbar.cuh"]
 CLI_SOURCES = {"dist_spmm_node": "cli_dist_spmm_node.cpp"}
 
 

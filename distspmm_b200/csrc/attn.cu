@@ -15,6 +15,7 @@
 
 #include "attn_row.cuh"
 #include "attn_decode.h"
+#include "attn_graph.h"
 #include "attn_tile.h"
 
 namespace dsp {
@@ -195,10 +196,8 @@ int status(const char *who) {
 
 unsigned warps_grid(int64_t warps) { return (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32)); }
 
-enum Pass { kForward, kDq, kDkv };
-
 template <class Rows, class T, int VE, int LPR, int VPL>
-void launch_shape(Pass pass, const Rows &rows, const AttnArgs &a, int64_t n_chunks, cudaStream_t s) {
+void launch_shape(AttnPass pass, const Rows &rows, const AttnArgs &a, int64_t n_chunks, cudaStream_t s) {
   const int64_t warps = n_chunks * (pass == kDkv ? a.heads / a.group : a.heads);
   if (pass == kForward) {
     attn_rows_kernel<Rows, T, VE, LPR, VPL><<<warps_grid(warps), kThreads, 0, s>>>(rows, a);
@@ -209,7 +208,7 @@ void launch_shape(Pass pass, const Rows &rows, const AttnArgs &a, int64_t n_chun
 }
 
 template <class Rows, class T>
-void launch_pass(Pass pass, const Rows &rows, const AttnArgs &a, int64_t n_chunks, cudaStream_t s) {
+void launch_pass(AttnPass pass, const Rows &rows, const AttnArgs &a, int64_t n_chunks, cudaStream_t s) {
   if (n_chunks == 0) return;
   if constexpr (sizeof(T) == 2) {
     if (a.dim <= 32) launch_shape<Rows, T, 8, 4, 1>(pass, rows, a, n_chunks, s);
@@ -248,11 +247,12 @@ ForwardPlan forward_plan(int64_t n_chunks, bool cut, int heads, int dim) {
 }
 
 struct GradPlan {
-  int64_t slots, ml, total;
+  int64_t dout_max, slots, ml, total;
 };
 GradPlan grad_plan(const dsp_pattern *p, const dsp_attn_desc *d) {
   GradPlan g = {};
-  g.slots = up256(4 * p->rows * d->heads);  // delta
+  g.dout_max = up256(4 * p->rows * d->heads);  // delta lies before it
+  g.slots = g.dout_max + 256;
   const int64_t q = p->a.n_split ? 16ll * p->a.n_chunks * d->heads * d->dim : 0;
   const int64_t kv = p->t.n_split ? 16ll * p->t.n_chunks * d->kv_heads * d->dim : 0;
   g.ml = g.slots + up256(std::max(q, kv));  // dq's partials are joined before dk's and dv's are written
@@ -267,7 +267,8 @@ int forward(const dsp_pattern *p, const dsp_attn_desc *d, char *ws, cudaStream_t
   a.slots = (float *)ws;
   a.slot_ml = (float *)(ws + f.ml);
   const PlanRows rows = {view(p->a)};
-  launch_pass<PlanRows, T>(kForward, rows, a, p->a.n_chunks, s);
+  if (graph_on_tensor_cores(d->dtype, d->dim)) graph_pass(kForward, rows.d, a, d->dtype, s);
+  else launch_pass<PlanRows, T>(kForward, rows, a, p->a.n_chunks, s);
   if (p->a.n_split)
     attn_join_kernel<T><<<dim3((unsigned)((p->a.n_split + 7) / 8), (unsigned)d->heads), kThreads, 0, s>>>(rows.d, a);
   return status("dsp_attn");
@@ -291,10 +292,18 @@ int gradients(const dsp_pattern *p, const dsp_attn_grad_desc *g, char *ws, cudaS
   a.slots = (float *)(ws + f.slots);
   a.slot_ml = (float *)(ws + f.ml);
   const PlanRows ra = {view(p->a)}, rt = {view(p->t)};
-  launch_pass<PlanRows, T>(kDq, ra, a, ra.d.n_chunks, s);
+  const bool tensor = graph_on_tensor_cores(d->dtype, d->dim);
+  if (tensor && d->dtype == DSP_F16) {
+    a.dout_max = (uint32_t *)(ws + f.dout_max);
+    const int rc = graph_dout_max(a.dout, p->rows, d->heads, d->dim, (uint32_t *)(ws + f.dout_max), s);
+    if (rc) return rc;
+  }
+  if (tensor) graph_pass(kDq, ra.d, a, d->dtype, s);
+  else launch_pass<PlanRows, T>(kDq, ra, a, ra.d.n_chunks, s);
   if (ra.d.n_split)
     attn_sum_kernel<T, true><<<dim3((unsigned)((ra.d.n_split + 7) / 8), (unsigned)d->heads), kThreads, 0, s>>>(ra.d, d->heads, a);
-  launch_pass<PlanRows, T>(kDkv, rt, a, rt.d.n_chunks, s);
+  if (tensor) graph_pass(kDkv, rt.d, a, d->dtype, s);
+  else launch_pass<PlanRows, T>(kDkv, rt, a, rt.d.n_chunks, s);
   if (rt.d.n_split)
     attn_sum_kernel<T, false>
         <<<dim3((unsigned)((rt.d.n_split + 7) / 8), (unsigned)d->kv_heads), kThreads, 0, s>>>(rt.d, d->kv_heads, a);

@@ -24,6 +24,7 @@ struct AttnArgs {
   HeadsOut out, dq, dk, dv;
   float *lse;        // [rows][heads]
   float *delta;      // [rows][heads] dout . out
+  const uint32_t *dout_max;  // bits of the largest finite |dout| (fp16 gradients)
   float *slots;      // partials of cut rows: [2 n_chunks][heads][width]
   float *slot_ml;    // [2 n_chunks][heads][2] running maximum and sum (forward)
 };
@@ -41,6 +42,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ float capped(float s, float cap, float inv_cap2, float &th) {
   th = 1.f - __fdividef(2.f, exp2_approx(s * inv_cap2) + 1.f);  // 2 / inf = 0
   return cap * th;
+}
+
+// fp16 has few exponents: gradients of scores are carried with a power of two that brings the largest |dout| near 16.
+__device__ __forceinline__ float dout_scale(const uint32_t *dout_max) {
+  const int e = (int)(__ldg(dout_max) >> 23);  // biased exponent; 255: not finite
+  return e > 0 && e < 255 ? __uint_as_float((uint32_t)min(max(127 + 4 - (e - 127), 1), 254) << 23) : 1.f;
 }
 
 int check_attn(const char *who, const dsp_attn_desc *d, int64_t rows, int64_t keys);

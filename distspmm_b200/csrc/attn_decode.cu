@@ -7,50 +7,19 @@
 //   S^T [16 keys x 8 heads] = K Q^T        A = 16 key rows, straight from global memory to the lanes that need them
 //   O^T [dim x 8 heads]    += V^T P^T      A = V^T, B = P^T: S^T's lanes hold 8 x 8 blocks, movmatrix turns them
 //
-// The order of a sum is free, so the places of dim (for K) and of dim rows (for V^T) in the fragments are chosen such that each
-// lane's part of a row is whole 16-byte vectors and 4 (8) neighbouring lanes read 64 (128) neighbouring bytes: no shared memory,
-// no transposes but one byte permute per pair of V's keys. The next 16 keys are requested as soon as the products have read the
-// present ones, so each warp keeps about 8 KB in flight. Weights are split in two 16-bit parts, p = hi + lo, with a product
+// Rows go from global memory to fragments without a stop (frag.cuh). The next 16 keys are requested as soon as the products
+// have read the present ones, so each warp keeps about 8 KB in flight. Weights are split in two 16-bit parts, p = hi + lo, with a product
 // for each: the tensor cores are idle anyway, and the result is then as exact as with fp32 weights.
 #include <algorithm>
 #include <type_traits>
 
 #include "attn_decode.h"
-#include "rowvec.cuh"
+#include "frag.cuh"
 
 namespace dsp {
 namespace {
 
 constexpr int kThreads = 128;
-
-template <class T>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&x);
-  } else {
-    const __half2 x = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&x);
-  }
-}
 
 // A row is read once: past L1, and as DRAM delivers it (240 -> 231 us on 64 x ~4800 tokens, 8 heads of 128, against plain loads).
 __device__ __forceinline__ uint4 ld_row(const void *p) {
@@ -93,8 +62,6 @@ struct Tile {
   }
 };
 
-__device__ __forceinline__ uint32_t word(const uint4 &x, int i) { return i == 0 ? x.x : i == 1 ? x.y : i == 2 ? x.z : x.w; }
-
 template <class T, int D>
 __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows d, const AttnArgs a, int head_tiles) {
   const int lane = threadIdx.x & 31, t = lane & 3, n8 = lane >> 2;
@@ -127,14 +94,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
     x.load_v(a, hk, ids);
     // Q^T as B fragments: k steps of 16 in the order of K's vectors (step 2 i + j: words 2 j, 2 j + 1 of vector i)
     uint32_t q[D / 16][2];
-    {
-      const T *src = (const T *)a.q.p + row * a.q.row + (int64_t)(h0 + n8) * a.q.head + t * 8;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint4 w = n8 < live ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * i)) : make_uint4(0, 0, 0, 0);
-        q[2 * i][0] = w.x, q[2 * i][1] = w.y, q[2 * i + 1][0] = w.z, q[2 * i + 1][1] = w.w;
-      }
-    }
+    load_column<T, D>(q, (const T *)a.q.p + row * a.q.row + (int64_t)(h0 + n8) * a.q.head, n8 < live);
     float acc[D / 16][4];
 #pragma unroll
     for (int i = 0; i < D / 16; ++i)
@@ -144,13 +104,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
 #pragma unroll 1
     for (int64_t b = p; b < pe; b += 16) {
       float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const uint32_t w[4] = {word(x.k[0][i], 2 * j), word(x.k[1][i], 2 * j), word(x.k[0][i], 2 * j + 1), word(x.k[1][i], 2 * j + 1)};
-          mma16816<T>(s, w, q[2 * i + j][0], q[2 * i + j][1]);
-        }
+      rows_times<T, D>(s, x.k, q);
       const int now = ids;
       ids = next;
       x.load_k(a, hk, ids);  // the next 16, while these are weighed
@@ -189,34 +143,18 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
 #pragma unroll
           for (int j = 0; j < 4; ++j) acc[i][j] *= keep[j & 1];
       }
-      uint32_t hi[2], lo[2];
+      uint32_t parts[2][2];  // weights of keys n8 + 8 j as hi and lo parts, turned
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {  // keys n8 + 8 j
+      for (int j = 0; j < 2; ++j) {
         const float p0 = exp2_approx(s[2 * j] - base[0]), p1w = exp2_approx(s[2 * j + 1] - base[1]);
         l[0] += p0;
         l[1] += p1w;
-        const uint32_t w = pack2<T>(p0, p1w);
-        float f[2];
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-          f[0] = __uint_as_float(w << 16), f[1] = __uint_as_float(w & 0xffff0000u);
-        } else {
-          const float2 g = __half22float2(*reinterpret_cast<const __half2 *>(&w));
-          f[0] = g.x, f[1] = g.y;
-        }
-        hi[j] = transpose8x8(w);
-        lo[j] = transpose8x8(pack2<T>(p0 - f[0], p1w - f[1]));
+        uint32_t hi, lo;
+        split2<T>(p0, p1w, hi, lo);
+        parts[0][j] = transpose8x8(hi);
+        parts[1][j] = transpose8x8(lo);
       }
-      // V^T: rows (places of dim) n8 and n8 + 8 of m tile 4 i + c are elements 2 c and 2 c + 1 of vector n8 + 8 i; k: the keys
-#pragma unroll
-      for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t k0 = word(x.v[0][i], c), k1 = word(x.v[1][i], c), k2 = word(x.v[2][i], c), k3 = word(x.v[3][i], c);
-          const uint32_t w[4] = {__byte_perm(k0, k1, 0x5410), __byte_perm(k0, k1, 0x7632), __byte_perm(k2, k3, 0x5410),
-                                 __byte_perm(k2, k3, 0x7632)};
-          mma16816<T>(acc[4 * i + c], w, hi[0], hi[1]);
-          mma16816<T>(acc[4 * i + c], w, lo[0], lo[1]);
-        }
+      turned_times<T, D, 2>(acc, x.v, parts);
       x.load_v(a, hk, ids);
     }
     // the sum over all keys, then the rows' results

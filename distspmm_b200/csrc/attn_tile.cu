@@ -53,7 +53,6 @@ struct TileArgs {
   int n_heads;          // heads of the grid (query heads, or key/value heads for dk, dv)
   int splits;           // pieces of a row tile's list (forward)
   float *part, *part_ml;  // their partial results: [splits][rows][heads][dim], [splits][rows][heads][2]
-  const uint32_t *dout_max;  // bits of the largest finite |dout| (fp16 gradients)
   int *err;
 };
 
@@ -535,12 +534,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         if (x.a.lse) x.a.lse[row * x.a.heads + head] = -INFINITY;
       }
     } else {
-      // fp16: dS carries a power of two that brings the largest |dout| near 16
-      float up = 1.f;
-      if (!kBf16) {
-        const int e = (int)(__ldg(x.dout_max) >> 23);  // biased exponent; 255: not finite
-        if (e > 0 && e < 255) up = __uint_as_float((uint32_t)min(max(127 + 4 - (e - 127), 1), 254) << 23);
-      }
+      float up = kBf16 ? 1.f : dout_scale(x.a.dout_max);
       const float down = x.a.scale / up;
       if (M == kDkv && !kBf16) up *= 0x1p-12f;  // the weights of dk, dv are 2^12 up themselves
       constexpr float kUp = kBf16 ? 0.f : 12.f;
@@ -841,7 +835,7 @@ int gradients(const dsp_pattern *p, TileArgs x, uint32_t *dout_max, cudaStream_t
   if (std::is_same<T, __half>::value) e = cudaMemsetAsync(dout_max, 0, 4, s);
   if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_attn_grad: %s", cudaGetErrorString(e));
   attn_delta_kernel<T, D><<<(unsigned)((p->rows * x.a.heads + 7) / 8), 256, 0, s>>>(p->rows, x.a, dout_max);
-  x.dout_max = dout_max;
+  x.a.dout_max = dout_max;
   const int rc = launch<T, D, kDq>(p, x, s);
   return rc ? rc : launch<T, D, kDkv>(p, x, s);
 }

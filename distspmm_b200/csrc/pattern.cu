@@ -228,8 +228,8 @@ int create(int device, const dsp_csr *a, int flags, dsp_pattern *p) {
     pattern_chunks(K, &t);
   }
   HostTiles ta, tt;
-  if (flags & DSP_PATTERN_ATTENTION) {
-    p->tiled = build_tiles(M, K, h, false, &ta);
+  if ((flags & DSP_PATTERN_ATTENTION) && !(flags & DSP_PATTERN_ROWS)) {
+    p->tiled = build_tiles(M, K, h, flags & DSP_PATTERN_TILES, &ta);
     if (p->tiled && (flags & DSP_PATTERN_GRAD)) build_tiles(K, M, t, true, &tt);
   }
   DeviceGuard g(device);
@@ -252,7 +252,9 @@ using namespace dsp;
 extern "C" int dsp_pattern_create(int device, const dsp_csr *a, int flags, dsp_pattern **out) {
   DSP_TRY_ARG(a && out && a->indptr, "dsp_pattern_create: null argument");
   *out = nullptr;
-  DSP_TRY_ARG((flags & ~(DSP_PATTERN_GRAD | DSP_PATTERN_ATTENTION)) == 0, "dsp_pattern_create: flags %d", flags);
+  const int forms = DSP_PATTERN_TILES | DSP_PATTERN_ROWS;
+  DSP_TRY_ARG((flags & ~(DSP_PATTERN_GRAD | DSP_PATTERN_ATTENTION | forms)) == 0 && (flags & forms) != forms,
+              "dsp_pattern_create: flags %d", flags);
   DSP_TRY_ARG(a->num_rows >= 0 && a->num_cols >= 0 && a->nnz >= 0, "dsp_pattern_create: negative size");
   DSP_TRY_ARG(a->nnz == 0 || a->indices, "dsp_pattern_create: null indices");
   if (a->num_rows >= INT32_MAX || a->num_cols >= INT32_MAX || a->nnz >= INT32_MAX)

@@ -19,11 +19,14 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 class SparsePattern:
     """grad: keep the transposed lists that gradients need. attention: check that no row lists a
-    column twice and prepare the forms that attention reads."""
+    column twice and prepare the forms that attention reads. form: "tiles" or "rows" force how
+    attention reads the pattern (None: tiles where they are filled well enough)."""
 
     GRAD, ATTENTION = 1, 2
+    FORMS = {None: 0, "tiles": 4, "rows": 8}
 
-    def __init__(self, a: Csr, device: int = 0, grad: bool = False, attention: bool = False):
+    def __init__(self, a: Csr, device: int = 0, grad: bool = False, attention: bool = False, form: str | None = None):
+        need(form in self.FORMS, f"form must be one of {sorted(k for k in self.FORMS if k)}, is {form!r}")
         self.device = device
         self.rows = a.num_rows
         self.cols = a.num_cols
@@ -32,8 +35,8 @@ class SparsePattern:
         self.attention = bool(attention)
         c = a.to_c()
         h = c_vp()
-        call("dsp_pattern_create", device, ctypes.byref(c), self.GRAD * self.grad + self.ATTENTION * self.attention,
-             ctypes.byref(h))
+        call("dsp_pattern_create", device, ctypes.byref(c), self.GRAD * self.grad + self.ATTENTION * self.attention +
+             self.FORMS[form], ctypes.byref(h))
         self._h = h
         self._host_values = a.values
         self._values = None

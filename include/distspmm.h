@@ -309,6 +309,10 @@ int dsp_spmm_csr_f32_noalloc(const int64_t *indptr, const int64_t *indices, cons
 typedef struct dsp_pattern dsp_pattern;
 #define DSP_PATTERN_GRAD 1      /* transposed lists, for dsp_spmm_act_grad and dsp_attn_grad          */
 #define DSP_PATTERN_ATTENTION 2 /* for dsp_attn: refuses a row that lists a column twice (FORMAT)     */
+/* Attention reads a pattern by tiles of 128 x 64 entries on the tensor cores where they are filled well enough, else row by
+ * row. These force the choice (for comparisons, or to save the tiles' memory); both at once are refused. */
+#define DSP_PATTERN_TILES 4
+#define DSP_PATTERN_ROWS 8
 
 typedef struct dsp_pattern_info {
   int64_t rows, cols, nnz;

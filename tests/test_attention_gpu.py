@@ -33,8 +33,17 @@ def near(got, want, tol, what):
         f"{((got - want).abs() / tol)[bad].max():.2f} of the tolerance, first at {bad.nonzero()[0].tolist()}"
 
 
+FORMS = ["tiles", "rows"]
+
+
 def check(a, heads, kv, dim, t, cap=0.0, bias=False, offset=0, grad=True, seed=0, scale=None):
-    p = d.SparsePattern(a, grad=grad, attention=True)
+    """Both forms of the pattern, where the operands have two."""
+    for form in FORMS if t != F32 and dim in (64, 128) else FORMS[1:]:
+        check_form(form, a, heads, kv, dim, t, cap, bias, offset, grad, seed, scale)
+
+
+def check_form(form, a, heads, kv, dim, t, cap, bias, offset, grad, seed, scale):
+    p = d.SparsePattern(a, grad=grad, attention=True, form=form)
     q, k, v, dout = inputs(a.num_rows, a.num_cols, heads, kv, dim, t, seed)
     sl = slopes_of(heads) if bias else None
     opt = dict(scale=scale, softcap=cap, slopes=sl.cuda() if bias else None, row_offset=offset)
@@ -55,7 +64,6 @@ def check(a, heads, kv, dim, t, cap=0.0, bias=False, offset=0, grad=True, seed=0
             assert x.dtype == t
             near(x, y, tol[name], name)
     p.check_error()  # no bounded wait gave up
-    return p
 
 
 @pytest.mark.parametrize("t", [F32, BF16, F16])
@@ -110,13 +118,14 @@ def test_large_scores(gpu, t):
 
 
 @pytest.mark.parametrize("t", [F32, BF16, F16])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("kind", ["window", "rmat"])
-def test_unlisted_keys_never_count(gpu, kind, t):
+def test_unlisted_keys_never_count(gpu, kind, form, t):
     """NaN and infinities in k and v rows that a query row does not list, inside the same tiles as rows it does: its result and
     the other rows' gradients are those without them."""
     a = positional("window", 260, window=50, first=2) if kind == "window" else d.gen_rmat(8, seed=3)
     n = a.num_rows
-    p = d.SparsePattern(a, grad=True, attention=True)
+    p = d.SparsePattern(a, grad=True, attention=True, form=form)
     q, k, v, dout = inputs(n, n, 4, 2, 64, t, 3)
     mask = mask_of(a)
     bad = torch.tensor([37, 100, 101, 200])
@@ -159,11 +168,12 @@ def backward(p, dout, q, k, v):
     return d.sparse_attention_backward(p, dout, q, k, v, out, lse)
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("t", [F32, BF16])
-def test_bad_query_rows_stay_alone(gpu, t):
+def test_bad_query_rows_stay_alone(gpu, t, form):
     """A NaN query row spoils itself and the gradients of the keys it lists, nothing else."""
     a = positional("window", 260, window=50)
-    p = d.SparsePattern(a, grad=True, attention=True)
+    p = d.SparsePattern(a, grad=True, attention=True, form=form)
     q, k, v, dout = inputs(260, 260, 2, 2, 64, t, 4)
     qb, db = q.clone(), dout.clone()
     qb[130] = float("nan")
@@ -179,12 +189,15 @@ def test_bad_query_rows_stay_alone(gpu, t):
     near(dv[keys], want["dv"][keys], tol["dv"][keys], "dv")
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("size", [1.0, 2.0 ** -10, 2.0 ** 9])
-def test_fp16_gradients_of_any_size(gpu, size):
+def test_fp16_gradients_of_any_size(gpu, size, form):
     """Small and large gradients in fp16: what the type cannot hold in between is scaled, results keep the tolerance."""
     a = positional("window", 400, window=220)
-    p = d.SparsePattern(a, grad=True, attention=True)
-    q, k, v, dout = inputs(400, 400, 2, 1, 64, F16, 11)
+    n = a.num_rows
+    p = d.SparsePattern(a, grad=True, attention=True, form=form)
+    assert (p.info()["tiles"] > 0) == (form == "tiles")
+    q, k, v, dout = inputs(n, n, 2, 1, 64, F16, 11)
     dout = (dout.float() * size).to(F16)
     dq, dk, dv = (x.cpu() for x in backward(p, dout, q, k, v))
     want, tol = want64(mask_of(a), q, k, v, dout)
@@ -247,12 +260,13 @@ def test_autograd_and_differences(gpu):
 
 
 @pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("kind", ["window", "rmat"])
-def test_strides(gpu, kind, t):
+def test_strides(gpu, kind, form, t):
     """q, k, v as parts of one fused projection, head-major storage, odd offsets, expanded heads."""
     a = positional("window", 200, window=90) if kind == "window" else d.gen_rmat(8, seed=2)
     n = a.num_rows
-    p = d.SparsePattern(a, grad=True, attention=True)
+    p = d.SparsePattern(a, grad=True, attention=True, form=form)
     q, k, v, dout = (x.cuda() for x in inputs(n, n, 4, 4, 64, t, 6))
     want = d.sparse_attention_forward(p, q, k, v)
     wg = d.sparse_attention_backward(p, dout, q, k, v, *want)
@@ -288,11 +302,12 @@ def test_broadcast_keys_get_summed_gradients(gpu):
     torch.testing.assert_close(v1.grad, v2.grad, rtol=1e-4, atol=1e-4)
 
 
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("kind", ["window", "rmat"])
-def test_same_bits_graphs_and_streams(gpu, kind):
+def test_same_bits_graphs_and_streams(gpu, kind, form):
     a = positional("window", 600, window=200, first=4) if kind == "window" else d.gen_rmat(10, seed=2)
     n = a.num_rows
-    p = d.SparsePattern(a, grad=True, attention=True)
+    p = d.SparsePattern(a, grad=True, attention=True, form=form)
     sets = []
     for s in range(2):
         q, k, v, dout = (x.cuda() for x in inputs(n, n, 4, 2, 64, BF16, s))

@@ -32,6 +32,9 @@ def test_pattern_refuses_bad_matrices():
     c = csr_of([[0]], 1).to_c()
     h = c_vp()
     assert status("dsp_pattern_create", 0, ctypes.byref(c), 64, ctypes.byref(h)) == -1
+    assert status("dsp_pattern_create", 0, ctypes.byref(c), 2 + 4 + 8, ctypes.byref(h)) == -1
+    with pytest.raises(ValueError, match="form must be"):
+        d.SparsePattern(csr_of([[0]], 1), attention=True, form="columns")
     assert status("dsp_pattern_create", 0, None, 0, ctypes.byref(h)) == -1
     assert status("dsp_pattern_info_get", None, ctypes.byref(dsp_pattern_info())) == -1
     d.lib().dsp_pattern_destroy(None)
