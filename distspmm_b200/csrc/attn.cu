@@ -122,65 +122,113 @@ __global__ void __launch_bounds__(kThreads) attn_dkv_kernel(const PlanRows d, co
   }
 }
 
-// Partials of cut rows (forward): merged in chunk order. blockIdx.y: head. Lane l holds columns l, l + 32, ...
+// A cut row of the list and the warps that join it: a block for each long one (warp w takes slots w, w + 8, ...), a warp for each
+// other. join_blocks(d) blocks of 8 warps.
+struct CutRow {
+  int64_t row, c0, c1;
+  bool wide;
+  __device__ __forceinline__ bool find(const DirView &d) {
+    wide = (int)blockIdx.x < d.n_long;
+    const int at = wide ? (int)blockIdx.x : d.n_long + ((int)blockIdx.x - d.n_long) * 8 + (threadIdx.x >> 5);
+    if (at >= d.n_split) return false;
+    row = __ldg(d.split_row + at);
+    c0 = row_start(row, __ldg(d.ptr + row)) / d.L, c1 = row_start(row, __ldg(d.ptr + row + 1)) / d.L;
+    return true;
+  }
+  __device__ __forceinline__ int64_t slot(int64_t c) const { return c == c0 ? 2 * c + 1 : 2 * c; }
+};
+
+// Partials of cut rows (forward), merged in a fixed order. blockIdx.y: head. Lane l holds columns l, l + 32, ...
 template <class T>
 __global__ void __launch_bounds__(kThreads) attn_join_kernel(const DirView d, const AttnArgs a) {
-  const int lane = threadIdx.x & 31, h = blockIdx.y;
-  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (at >= d.n_split) return;
-  const int64_t r = __ldg(d.split_row + at);
-  const int64_t c0 = row_start(r, __ldg(d.ptr + r)) / d.L, c1 = row_start(r, __ldg(d.ptr + r + 1)) / d.L;
+  __shared__ float part[8][256], part_ml[8][2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
+  CutRow r;
+  if (!r.find(d)) return;  // whole warps of a block without barriers
   float m = -INFINITY, l = 0.f, acc[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.f;
-#pragma unroll 4
-  for (int64_t c = c0; c <= c1; ++c) {
-    const int64_t slot = (c == c0 ? 2 * c + 1 : 2 * c) * a.heads + h;
-    const float m2 = a.slot_ml[2 * slot], l2 = a.slot_ml[2 * slot + 1];
+  auto merge = [&](float m2, float l2, const float *src) {
     const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
     const float f1 = exp2_approx(m - base), f2 = exp2_approx(m2 - base);
     l = l * f1 + l2 * f2;
     m = top;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (lane + 32 * i < a.dim) acc[i] = acc[i] * f1 + a.slots[slot * a.dim + lane + 32 * i] * f2;
+      if (lane + 32 * i < a.dim) acc[i] = acc[i] * f1 + src[lane + 32 * i] * f2;
+  };
+#pragma unroll 4
+  for (int64_t c = r.c0 + (r.wide ? warp : 0); c <= r.c1; c += r.wide ? 8 : 1) {
+    const int64_t slot = r.slot(c) * a.heads + h;
+    merge(a.slot_ml[2 * slot], a.slot_ml[2 * slot + 1], a.slots + slot * a.dim);
+  }
+  if (r.wide) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < a.dim) part[warp][lane + 32 * i] = acc[i];
+    if (lane == 0) part_ml[warp][0] = m, part_ml[warp][1] = l;
+    __syncthreads();
+    if (warp > 0) return;
+    for (int w = 1; w < 8; ++w) merge(part_ml[w][0], part_ml[w][1], part[w]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *dst = (T *)a.out.p + r * a.out.row + h * a.out.head;
+  T *dst = (T *)a.out.p + r.row * a.out.row + h * a.out.head;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (lane + 32 * i < a.dim) dst[lane + 32 * i] = T(acc[i] * inv);
-  if (a.lse && lane == 0) a.lse[r * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (a.lse && lane == 0) a.lse[r.row * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// Partials of cut rows (gradients), 2 dim floats per slot and head, summed in chunk order. DQ: the sums x and y of a row and
+// Partials of cut rows (gradients), 2 dim floats per slot and head, summed in a fixed order. DQ: the sums x and y of a row and
 // its delta (attend_dq); else dk and dv of a key.
 template <class T, bool DQ>
 __global__ void __launch_bounds__(kThreads) attn_sum_kernel(const DirView d, int n_heads, const AttnArgs a) {
-  const int lane = threadIdx.x & 31, h = blockIdx.y;
-  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (at >= d.n_split) return;
-  const int64_t r = __ldg(d.split_row + at);
-  const int64_t c0 = row_start(r, __ldg(d.ptr + r)) / d.L, c1 = row_start(r, __ldg(d.ptr + r + 1)) / d.L;
-  float delta = 0.f;
-  if (DQ) {
+  __shared__ float part[8][512], part_delta[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
+  CutRow r;
+  if (!r.find(d)) return;
+  const int64_t first = r.c0 + (r.wide ? warp : 0);
+  const int step = r.wide ? 8 : 1;
+  float delta = 0.f, x[8], y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
 #pragma unroll 4
-    for (int64_t c = c0; c <= c1; ++c) delta += a.slot_ml[(c == c0 ? 2 * c + 1 : 2 * c) * n_heads + h];
-    if (lane == 0) a.delta[r * a.heads + h] = delta;
+  for (int64_t c = first; c <= r.c1; c += step) {
+    const int64_t slot = r.slot(c) * n_heads + h;
+    const float *src = a.slots + slot * 2 * a.dim + lane;
+    if (DQ) delta += a.slot_ml[slot];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < a.dim) x[i] += src[32 * i], y[i] += src[a.dim + 32 * i];
   }
-  for (int col = lane; col < a.dim; col += 32) {
-    float x = 0.f, y = 0.f;
-#pragma unroll 4
-    for (int64_t c = c0; c <= c1; ++c) {
-      const float *src = a.slots + ((c == c0 ? 2 * c + 1 : 2 * c) * n_heads + h) * 2 * a.dim + col;
-      x += src[0];
-      y += src[a.dim];
+  if (r.wide) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (lane + 32 * i < a.dim) part[warp][lane + 32 * i] = x[i], part[warp][256 + lane + 32 * i] = y[i];
+    if (lane == 0) part_delta[warp] = delta;
+    __syncthreads();
+    if (warp > 0) return;
+    for (int w = 1; w < 8; ++w) {
+      delta += part_delta[w];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (lane + 32 * i < a.dim) x[i] += part[w][lane + 32 * i], y[i] += part[w][256 + lane + 32 * i];
     }
+  }
+  if (DQ && lane == 0) {
+    const float lse = a.lse[r.row * a.heads + h];
+    if (a.stats) a.stats[r.row * a.heads + h] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, delta);
+    else a.delta[r.row * a.heads + h] = delta;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int col = lane + 32 * i;
+    if (col >= a.dim) continue;
     if (DQ) {
-      ((T *)a.dq.p)[r * a.dq.row + h * a.dq.head + col] = T((x - delta * y) * a.scale);
+      ((T *)a.dq.p)[r.row * a.dq.row + h * a.dq.head + col] = T((x[i] - delta * y[i]) * a.scale);
     } else {
-      ((T *)a.dk.p)[r * a.dk.row + h * a.dk.head + col] = T(x);
-      ((T *)a.dv.p)[r * a.dv.row + h * a.dv.head + col] = T(y);
+      ((T *)a.dk.p)[r.row * a.dk.row + h * a.dk.head + col] = T(x[i]);
+      ((T *)a.dv.p)[r.row * a.dv.row + h * a.dv.head + col] = T(y[i]);
     }
   }
 }
@@ -251,7 +299,7 @@ struct GradPlan {
 };
 GradPlan grad_plan(const dsp_pattern *p, const dsp_attn_desc *d) {
   GradPlan g = {};
-  g.dout_max = up256(4 * p->rows * d->heads);  // delta lies before it
+  g.dout_max = up256(8 * p->rows * d->heads);  // delta, or stats, lie before it
   g.slots = g.dout_max + 256;
   const int64_t q = p->a.n_split ? 16ll * p->a.n_chunks * d->heads * d->dim : 0;
   const int64_t kv = p->t.n_split ? 16ll * p->t.n_chunks * d->kv_heads * d->dim : 0;
@@ -270,7 +318,7 @@ int forward(const dsp_pattern *p, const dsp_attn_desc *d, char *ws, cudaStream_t
   if (graph_on_tensor_cores(d->dtype, d->dim)) graph_pass(kForward, rows.d, a, d->dtype, s);
   else launch_pass<PlanRows, T>(kForward, rows, a, p->a.n_chunks, s);
   if (p->a.n_split)
-    attn_join_kernel<T><<<dim3((unsigned)((p->a.n_split + 7) / 8), (unsigned)d->heads), kThreads, 0, s>>>(rows.d, a);
+    attn_join_kernel<T><<<dim3((unsigned)join_blocks(rows.d), (unsigned)d->heads), kThreads, 0, s>>>(rows.d, a);
   return status("dsp_attn");
 }
 
@@ -293,6 +341,7 @@ int gradients(const dsp_pattern *p, const dsp_attn_grad_desc *g, char *ws, cudaS
   a.slot_ml = (float *)(ws + f.ml);
   const PlanRows ra = {view(p->a)}, rt = {view(p->t)};
   const bool tensor = graph_on_tensor_cores(d->dtype, d->dim);
+  if (tensor) a.stats = (float2 *)ws;
   if (tensor && d->dtype == DSP_F16) {
     a.dout_max = (uint32_t *)(ws + f.dout_max);
     const int rc = graph_dout_max(a.dout, p->rows, d->heads, d->dim, (uint32_t *)(ws + f.dout_max), s);
@@ -301,12 +350,12 @@ int gradients(const dsp_pattern *p, const dsp_attn_grad_desc *g, char *ws, cudaS
   if (tensor) graph_pass(kDq, ra.d, a, d->dtype, s);
   else launch_pass<PlanRows, T>(kDq, ra, a, ra.d.n_chunks, s);
   if (ra.d.n_split)
-    attn_sum_kernel<T, true><<<dim3((unsigned)((ra.d.n_split + 7) / 8), (unsigned)d->heads), kThreads, 0, s>>>(ra.d, d->heads, a);
+    attn_sum_kernel<T, true><<<dim3((unsigned)join_blocks(ra.d), (unsigned)d->heads), kThreads, 0, s>>>(ra.d, d->heads, a);
   if (tensor) graph_pass(kDkv, rt.d, a, d->dtype, s);
   else launch_pass<PlanRows, T>(kDkv, rt, a, rt.d.n_chunks, s);
   if (rt.d.n_split)
     attn_sum_kernel<T, false>
-        <<<dim3((unsigned)((rt.d.n_split + 7) / 8), (unsigned)d->kv_heads), kThreads, 0, s>>>(rt.d, d->kv_heads, a);
+        <<<dim3((unsigned)join_blocks(rt.d), (unsigned)d->kv_heads), kThreads, 0, s>>>(rt.d, d->kv_heads, a);
   return status("dsp_attn_grad");
 }
 
@@ -330,6 +379,9 @@ int check_heads(const char *who, const char *name, const void *p, int64_t row, i
   DSP_TRY_ARG(p, "%s: %s is null", who, name);
   DSP_TRY_ARG(((uintptr_t)p & 15) == 0 && row * e % 16 == 0 && head * e % 16 == 0,
               "%s: %s and its strides (%lld, %lld) must be multiples of 16 bytes", who, name, (long long)row, (long long)head);
+  DSP_TRY_ARG(row >= 0 && head >= 0, "%s: %s with strides (%lld, %lld)", who, name, (long long)row, (long long)head);
+  if (row >= (1ll << 30))
+    return fail(DSP_ERR_UNSUPPORTED, "%s: %s with a row stride of %lld: less than 2^30 is wanted", who, name, (long long)row);
   return DSP_OK;
 }
 

@@ -2,10 +2,10 @@
 //
 // For patterns too thin for tiles (a graph's edges). The formulas are those of attn.cu; what bounds both is the gather of a row
 // of k and one of v (q and dout, by columns) for each entry and head out of L2. Here the arithmetic is given to mma.sync, though
-// an entry has but one query to be multiplied with (of m16n8k16 products, 16 rows are entries and 1 to 8 columns are query
-// heads): 16 entries of dim 64 take some 120 instructions where dot products by shuffles took 780 (R-MAT 15, 8 heads of 64).
+// an entry has but one query for each head to be multiplied with (of m16n8k16 products, 8 columns are entries and 1 to 8 rows
+// query heads): 16 entries of dim 64 take some 120 instructions where dot products by shuffles took 780 (R-MAT 15, 8 heads of 64).
 //
-//   pass      rows of 16 entries      columns                      then, turned
+//   pass      16 entries as columns   rows                         then, entries turned
 //   forward   k                       q of up to 8 heads           v   x weights
 //   dq        k, v                    q, dout of up to 4 heads,    k   x [p c dp | p c]   (x and y of attn_row.cuh)
 //                                     twice
@@ -24,6 +24,7 @@ namespace dsp {
 namespace {
 
 constexpr int kThreads = 128;
+constexpr float kSlack = 8.f;
 
 struct Lists {
   int32_t cols[kMaxUnits];
@@ -63,12 +64,11 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
   constexpr float kUp = kHalf && M == kDkv ? 4096.f : 1.f;
   const float inv_cap2 = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f, scale2 = a.scale * kLog2e;
 
-  // places this lane's columns 2 t, 2 t + 1 have among the heads
-  auto head_of = [&](int j) { return M == kForward ? 2 * t + j : M == kDq ? (2 * t + j) & 3 : 0; };
-  float slope2[2];
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-    slope2[j] = M != kDkv && a.slopes && head_of(j) < live ? __ldg(a.slopes + h0 + head_of(j)) * kLog2e : 0.f;
+  // a lane has the scores of column n8, a query head (dk, dv: the key, in columns 0 and 1), for the entries 2 t, 2 t + 1, 2 t + 8,
+  // 2 t + 9 of a step: as they enter the second product
+  const int head = M == kForward ? n8 : M == kDq ? n8 & 3 : 0;
+  const float slope2 = M != kDkv && a.slopes && head < live ? __ldg(a.slopes + h0 + head) * kLog2e : 0.f;
+  auto entry = [&](int j) { return 2 * t + (j & 1) + 8 * (j >> 1); };
 
   auto first_of = [&](Step s) {  // the first row from s.row on with entries in this chunk; row r1 + 1: none
     for (; s.row <= r1; ++s.row) {
@@ -118,31 +118,32 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
           const HeadsOut &o = M == kForward ? a.out : a.dq;
           if (lane < D / 8) *reinterpret_cast<uint4 *>((T *)o.p + (int64_t)row * o.row + (int64_t)h * o.head + 8 * lane) = zero;
           if (lane == 0 && M == kForward && a.lse) a.lse[(int64_t)row * a.heads + h] = -INFINITY;
-          if (lane == 0 && M == kDq) a.delta[(int64_t)row * a.heads + h] = 0.f;
+          if (lane == 0 && M == kDq) a.stats[(int64_t)row * a.heads + h] = make_float2(INFINITY, 0.f);
         }
       }
     }
   };
 
-  // gathers: rows n8, n8 + 8 of a step; turned rows
+  // gathers: rows n8, n8 + 8 of a step; turned rows. Entries behind the row's end are read as its last one; their weights are 0.
+  auto at_row = [](const Heads &m, int head, int vec) { return (const char *)((const T *)m.p + (int64_t)head * m.head + vec * 8); };
   auto load_rows = [&](uint4(&x)[2][VR], const Heads &m, const Step &s, int head) {
+    const char *base = at_row(m, head, t);
+    const uint32_t stride = (uint32_t)m.row * (uint32_t)sizeof(T);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int32_t at = s.b + n8 + 8 * j;
-      const bool on = at < s.pe;
-      const T *src = (const T *)m.p + (int64_t)cols[on ? at : s.b] * m.row + (int64_t)head * m.head + t * 8;
+      const char *src = base + (uint64_t)(uint32_t)cols[min(s.b + n8 + 8 * j, s.pe - 1)] * stride;
 #pragma unroll
-      for (int i = 0; i < VR; ++i) x[j][i] = on ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * i)) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < VR; ++i) x[j][i] = __ldg(reinterpret_cast<const uint4 *>(src + 64 * i));
     }
   };
   auto load_turned = [&](uint4(&x)[4][VT], const Heads &m, const Step &s, int head) {
+    const char *base = at_row(m, head, D >= 64 ? n8 : min(n8, D / 8 - 1));
+    const uint32_t stride = (uint32_t)m.row * (uint32_t)sizeof(T);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int32_t at = s.b + 2 * t + (j & 1) + 8 * (j >> 1);
-      const bool on = at < s.pe && (D >= 64 || n8 < D / 8);
-      const T *src = (const T *)m.p + (int64_t)cols[at < s.pe ? at : s.b] * m.row + (int64_t)head * m.head + n8 * 8;
+      const char *src = base + (uint64_t)(uint32_t)cols[min(s.b + entry(j), s.pe - 1)] * stride;
 #pragma unroll
-      for (int i = 0; i < VT; ++i) x[j][i] = on ? __ldg(reinterpret_cast<const uint4 *>(src + 64 * i)) : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < VT; ++i) x[j][i] = __ldg(reinterpret_cast<const uint4 *>(src + 128 * i));
     }
   };
   auto head_at = [&](const Step &s) { return M == kDkv ? hk * a.group + s.h : hk; };
@@ -162,40 +163,32 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
   load_rows(x0, M == kDkv ? a.q : a.k, now, head_at(now));
   if constexpr (M != kForward) load_rows(x1, M == kDkv ? a.dout : a.v, now, head_at(now));
   else load_turned(xt, a.v, now, hk);
-  float lse_e[2] = {0.f, 0.f}, delta_e[2] = {0.f, 0.f};  // dk, dv: of the queries n8, n8 + 8
+  float2 stat_e[4] = {};  // dk, dv: of this lane's queries (columns 0 and 1 need them)
   auto load_stats = [&](const Step &s) {
+    if (n8 >= 2) return;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int32_t at = s.b + n8 + 8 * j;
-      const int64_t i = (int64_t)cols[at < s.pe ? at : s.b] * a.heads + head_at(s);
-      lse_e[j] = __ldg(a.lse + i);
-      delta_e[j] = a.delta[i];
-    }
+    for (int j = 0; j < 4; ++j) stat_e[j] = a.stats[(int64_t)cols[min(s.b + entry(j), s.pe - 1)] * a.heads + head_at(s)];
   };
   if (M == kDkv) load_stats(now);
 
   int32_t row = -1;
-  uint32_t c0[D / 16][2], c1[M == kForward ? 1 : D / 16][2];  // columns: q; dout    (dk, dv: k; v)
+  uint32_t pair[D / 16][4];  // q over dout (dk, dv: k over v)
   float acc[NT][4], acc2[M == kDkv ? NT : 1][4];
-  float m[2], l[2], lse2[2];  // forward: maximum, sum; dq: l is delta
+  float m = -INFINITY, l = 0.f, lse2 = 0.f;  // forward: maximum, sum; dq: l is delta
 
 #pragma unroll 1
   while (true) {
     if (now.row != row) {
       row = now.row;
       if (M == kDkv) {
-        load_column<T, D>(c0, (const T *)a.k.p + (int64_t)row * a.k.row + (int64_t)hk * a.k.head, n8 < 2);
-        if constexpr (M != kForward) load_column<T, D>(c1, (const T *)a.v.p + (int64_t)row * a.v.row + (int64_t)hk * a.v.head, n8 < 2);
+        load_pair<T, D>(pair, (const T *)a.k.p + (int64_t)row * a.k.row + (int64_t)hk * a.k.head, n8 < 2,
+                        (const T *)a.v.p + (int64_t)row * a.v.row + (int64_t)hk * a.v.head, n8 < 2);
       } else {
-        const int h = M == kForward ? n8 : n8 & 3;
-        load_column<T, D>(c0, (const T *)a.q.p + (int64_t)row * a.q.row + (int64_t)(h0 + h) * a.q.head, h < live);
+        load_pair<T, D>(pair, (const T *)a.q.p + (int64_t)row * a.q.row + (int64_t)(h0 + head) * a.q.head, head < live,
+                        (const T *)a.dout.p + (int64_t)row * a.dout.row + (int64_t)(h0 + head) * a.dout.head, M == kDq && head < live);
         if constexpr (M == kDq) {
-          load_column<T, D>(c1, (const T *)a.dout.p + (int64_t)row * a.dout.row + (int64_t)(h0 + h) * a.dout.head, h < live);
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            lse2[j] = head_of(j) < live ? __ldg(a.lse + (int64_t)row * a.heads + h0 + head_of(j)) * kLog2e : 0.f;
-            if (lse2[j] == -INFINITY) lse2[j] = INFINITY;
-          }
+          lse2 = head < live ? __ldg(a.lse + (int64_t)row * a.heads + h0 + head) * kLog2e : 0.f;
+          if (lse2 == -INFINITY) lse2 = INFINITY;
         }
       }
 #pragma unroll
@@ -205,14 +198,16 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
           acc[i][j] = 0.f;
           if constexpr (M == kDkv) acc2[i][j] = 0.f;
         }
-      m[0] = m[1] = -INFINITY, l[0] = l[1] = 0.f;
+      m = -INFINITY, l = 0.f;
     }
     const Step next = next_of(now);
     const bool more = next.row <= r1;
-    float s[4] = {0.f, 0.f, 0.f, 0.f}, dp[4] = {0.f, 0.f, 0.f, 0.f};
-    rows_times<T, D>(s, x0, c0);
-    if constexpr (M != kForward) rows_times<T, D>(dp, x1, c1);
-    float lse_n[2] = {lse_e[0], lse_e[1]}, delta_n[2] = {delta_e[0], delta_e[1]};
+    float s[4], dp[4];
+    pair_times<T, D, false>(s, pair, x0);
+    if constexpr (M != kForward) pair_times<T, D, true>(dp, pair, x1);
+    float2 stat[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) stat[j] = stat_e[j];
     // the next step's rows; of this one the turned rows, which the first product has brought to L1
     if constexpr (M == kDq) load_turned(xt, a.k, now, hk);
     if constexpr (M == kDkv) load_turned(xt, a.dout, now, head_at(now));
@@ -221,87 +216,84 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
       if constexpr (M != kForward) load_rows(x1, M == kDkv ? a.dout : a.v, next, head_at(next));
       if (M == kDkv) load_stats(next);
     }
-    // scores, base 2, of entries n8 (s[0], s[1]) and n8 + 8
+    // scores, base 2
     float th[4];
-    bool on[2];
+    bool on[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int32_t at = now.b + n8 + 8 * (j >> 1);
-      on[j >> 1] = at < now.pe;
+      const int32_t at = now.b + entry(j);
+      on[j] = at < now.pe;
       float u = s[j];
       th[j] = 0.f;
       if (a.cap > 0.f) u = capped(u * a.scale, a.cap, inv_cap2, th[j]) * kLog2e;
       else u *= scale2;
       if (a.slopes) {
-        const int32_t c = cols[on[j >> 1] ? at : now.b];
+        const int32_t c = cols[min(at, now.pe - 1)];
         const int64_t dist = M == kDkv ? c + a.row_offset - row : row + a.row_offset - c;
-        const float sl = M == kDkv ? __ldg(a.slopes + head_at(now)) * kLog2e : slope2[j & 1];
+        const float sl = M == kDkv ? __ldg(a.slopes + head_at(now)) * kLog2e : slope2;
         u = fmaf(-sl, fabsf((float)dist), u);
       }
       s[j] = u;
     }
     uint32_t parts[2][2];
     if constexpr (M == kForward) {
-      float top[2] = {m[0], m[1]}, base[2];
+      // m: a maximum of the row that the column's lanes agree on; renewed when a score is above it by more than 2^kSlack
+      float top = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (!on[j >> 1]) s[j] = -INFINITY;
-        top[j & 1] = fmaxf(top[j & 1], s[j]);
+        if (!on[j]) s[j] = -INFINITY;
+        top = fmaxf(top, s[j]);
       }
+      if (__any_sync(0xffffffffu, top > m + kSlack)) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const float m2 = fmaxf(m, top), keep = m2 == -INFINITY ? 0.f : exp2_approx(m - m2);
+        m = m2;
+        l *= keep;
+        // the sums' columns are heads 2 t and 2 t + 1
+        const float k0 = __shfl_sync(0xffffffffu, keep, 8 * t), k1 = __shfl_sync(0xffffffffu, keep, 8 * t + 4);
 #pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        top[0] = fmaxf(top[0], __shfl_xor_sync(0xffffffffu, top[0], o));
-        top[1] = fmaxf(top[1], __shfl_xor_sync(0xffffffffu, top[1], o));
+        for (int i = 0; i < NT; ++i) acc[i][0] *= k0, acc[i][2] *= k0, acc[i][1] *= k1, acc[i][3] *= k1;
       }
+      const float base = m == -INFINITY ? 0.f : m;
+      float w[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        base[j] = top[j] == -INFINITY ? 0.f : top[j];
-        const float keep = exp2_approx(m[j] - base[j]);
-        m[j] = top[j];
-        l[j] *= keep;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) acc[i][j] *= keep, acc[i][2 + j] *= keep;
+      for (int j = 0; j < 4; ++j) {
+        w[j] = exp2_approx(s[j] - base);
+        l += w[j];
       }
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float pa = exp2_approx(s[2 * j] - base[0]), pb = exp2_approx(s[2 * j + 1] - base[1]);
-        l[0] += pa;
-        l[1] += pb;
-        uint32_t hi, lo;
-        split2<T>(pa, pb, hi, lo);
-        parts[0][j] = transpose8x8(hi);
-        parts[1][j] = transpose8x8(lo);
-      }
+      split2<T>(w[0], w[1], parts[0][0], parts[1][0]);
+      split2<T>(w[2], w[3], parts[0][1], parts[1][1]);
       turned_times<T, D, 2>(acc, xt, parts);
       if (more) load_turned(xt, a.v, next, hk);
     } else if constexpr (M == kDq) {
+      float v[4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float v[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int e = 2 * j + k;
-          const float w = on[j] ? exp2_approx(s[e] - lse2[k]) : 0.f, wc = w * (1.f - th[e] * th[e]);
-          if (on[j]) l[k] = fmaf(w, dp[e], l[k]);
-          v[k] = t < 2 ? (on[j] ? wc * dp[e] * up : 0.f) : wc;
-        }
-        uint32_t hi, lo;
-        split2<T>(v[0], v[1], hi, lo);
-        parts[0][j] = transpose8x8(hi);
-        parts[1][j] = transpose8x8(lo);
+      for (int j = 0; j < 4; ++j) {
+        const float w = on[j] ? exp2_approx(s[j] - lse2) : 0.f, wc = w * (1.f - th[j] * th[j]);
+        l = fmaf(w, dp[j], l);
+        v[j] = n8 < 4 ? wc * dp[j] * up : wc;
       }
+      split2<T>(v[0], v[1], parts[0][0], parts[1][0]);
+      split2<T>(v[2], v[3], parts[0][1], parts[1][1]);
       turned_times<T, D, 2>(acc, xt, parts);
     } else {
-      // column 0: the value rounded, column 1: what rounding took (lanes of t = 0 hold both)
+      // column 0: the value rounded, column 1: what rounding took
       uint32_t wp[1][2], wd[1][2];
+      float w[4], g[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        w[j] = on[j] ? exp2_approx(s[j] - stat[j].x) : 0.f;
+        g[j] = w[j] * (dp[j] - stat[j].y) * (1.f - th[j] * th[j]) * up;
+        w[j] *= kUp;
+      }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const float lse = lse_n[j] * kLog2e;
-        const float w = on[j] && lse_n[j] != -INFINITY ? exp2_approx(s[2 * j] - lse) : 0.f;
-        const float g = on[j] ? w * (dp[2 * j] - delta_n[j]) * (1.f - th[2 * j] * th[2 * j]) * up : 0.f;
-        const float wk = w * kUp, w_hi = unpack2<T>(pack2<T>(wk, 0.f)).x, g_hi = unpack2<T>(pack2<T>(g, 0.f)).x;
-        wp[0][j] = transpose8x8(pack2<T>(wk, wk - w_hi));
-        wd[0][j] = transpose8x8(pack2<T>(g, g - g_hi));
+        uint32_t hi, lo;
+        split2<T>(w[2 * j], w[2 * j + 1], hi, lo);
+        wp[0][j] = n8 == 0 ? hi : lo;
+        split2<T>(g[2 * j], g[2 * j + 1], hi, lo);
+        wd[0][j] = n8 == 0 ? hi : lo;
       }
       turned_times<T, D, 1>(acc, xt, wp);
       load_turned(xt, a.q, now, head_at(now));
@@ -315,19 +307,18 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
     const bool cut_head = row == r0 && head_cut, cut = cut_head || row == r1;
     const int64_t slot = cut_head ? 2 * chunk : 2 * chunk + 1;
     if constexpr (M != kDkv) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) {
-        l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
-        l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
-      }
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
     }
+    // of the heads 2 t, 2 t + 1 (dq: 2 t & 3, ...) whose sums this lane holds
+    const float l2[2] = {__shfl_sync(0xffffffffu, l, 8 * t), __shfl_sync(0xffffffffu, l, 8 * t + 4)};
     const bool writes = D >= 64 || n8 < D / 8;
     if constexpr (M == kForward) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int h = h0 + 2 * t + j;
         if (2 * t + j >= live) continue;
-        const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+        const float inv = l2[j] == 0.f ? 0.f : 1.f / l2[j];
 #pragma unroll
         for (int i = 0; i < VT; ++i) {
           float f[8];
@@ -342,17 +333,18 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
             RowVec<T, 8>::st((T *)a.out.p + (int64_t)row * a.out.row + (int64_t)h * a.out.head + col, f);
           }
         }
-        if (n8 == 0) {
-          if (cut) a.slot_ml[2 * (slot * a.heads + h)] = m[j], a.slot_ml[2 * (slot * a.heads + h) + 1] = l[j];
-          else if (a.lse) a.lse[(int64_t)row * a.heads + h] = l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * kLn2;
-        }
+      }
+      if (t == 0 && n8 < live) {
+        const int64_t at = slot * a.heads + h0 + n8;
+        if (cut) a.slot_ml[2 * at] = m, a.slot_ml[2 * at + 1] = l;
+        else if (a.lse) a.lse[(int64_t)row * a.heads + h0 + n8] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
       }
     } else if constexpr (M == kDq) {
       // x of heads 2 t, 2 t + 1 in lanes t < 2, their y in lanes t + 2
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        const int h = h0 + head_of(j);
-        const bool own = head_of(j) < live && writes;
+        const int hh = (2 * t + j) & 3, h = h0 + hh;
+        const bool own = hh < live && writes;
 #pragma unroll
         for (int i = 0; i < VT; ++i) {
           float f[8], g[8];
@@ -368,14 +360,14 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
             st_f32<8>(a.slots + (slot * a.heads + h) * 2 * D + (t < 2 ? 0 : D) + col, f);
           } else if (t < 2) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) f[c] = (f[c] - l[j] * g[c]) * a.scale;
+            for (int c = 0; c < 8; ++c) f[c] = (f[c] - l2[j] * g[c]) * a.scale;
             RowVec<T, 8>::st((T *)a.dq.p + (int64_t)row * a.dq.row + (int64_t)h * a.dq.head + col, f);
           }
         }
-        if (n8 == 0 && t < 2 && head_of(j) < live) {
-          if (cut) a.slot_ml[slot * a.heads + h] = l[j];
-          else a.delta[(int64_t)row * a.heads + h] = l[j];
-        }
+      }
+      if (t == 0 && n8 < live) {
+        if (cut) a.slot_ml[slot * a.heads + h0 + n8] = l;
+        else a.stats[(int64_t)row * a.heads + h0 + n8] = make_float2(lse2, l);
       }
     } else {
 #pragma unroll

@@ -78,6 +78,37 @@ __device__ __forceinline__ void load_column(uint32_t (&q)[D / 16][2], const T *r
     q[2 * i][0] = w.x, q[2 * i][1] = w.y, q[2 * i + 1][0] = w.z, q[2 * i + 1][1] = w.w;
   }
 }
+// The other way round: 16 gathered rows as the 8 columns of two products, so that a row's vectors are operands as they are
+// loaded. Of A, rows 0 to 7 are `low`, rows 8 to 15 `high` (one row per lane group n8 each).
+template <class T, int D>
+__device__ __forceinline__ void load_pair(uint32_t (&q)[D / 16][4], const T *low, bool low_on, const T *high, bool high_on) {
+  const int t = threadIdx.x & 3;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const uint4 w = low_on ? __ldg(reinterpret_cast<const uint4 *>(low + t * 8 + 32 * i)) : zero;
+    const uint4 v = high_on ? __ldg(reinterpret_cast<const uint4 *>(high + t * 8 + 32 * i)) : zero;
+    q[2 * i][0] = w.x, q[2 * i][2] = w.y, q[2 * i + 1][0] = w.z, q[2 * i + 1][2] = w.w;
+    q[2 * i][1] = v.x, q[2 * i][3] = v.y, q[2 * i + 1][1] = v.z, q[2 * i + 1][3] = v.w;
+  }
+}
+// s[0], s[1]: row n8 of low (HIGH: high) . gathered rows 2 t, 2 t + 1; s[2], s[3]: . rows 2 t + 8, 2 t + 9.
+template <class T, int D, bool HIGH>
+__device__ __forceinline__ void pair_times(float (&s)[4], const uint32_t (&q)[D / 16][4], const uint4 (&k)[2][D / 32]) {
+  float c[2][4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[j][i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      mma16816<T>(c[j], q[2 * i], k[j][i].x, k[j][i].y);
+      mma16816<T>(c[j], q[2 * i + 1], k[j][i].z, k[j][i].w);
+    }
+    s[2 * j] = c[j][HIGH ? 2 : 0], s[2 * j + 1] = c[j][HIGH ? 3 : 1];
+  }
+}
+
 // vectors of a turned row per lane, result tiles
 template <int D>
 constexpr int kTurned = D >= 64 ? D / 64 : 1;

@@ -19,7 +19,7 @@ namespace dsp {
 // 2c + 1 of the chunk it starts in, in slot 2c of every later one. split_row lists the cut rows, those of more than
 // kLongSlots partials first (n_long of them).
 constexpr int kRowUnits = 8;
-constexpr int kLongSlots = 16;
+constexpr int kLongSlots = 12;
 constexpr int kMaxUnits = 512;  // of a chunk
 DSP_HD int64_t row_start(int64_t r, int64_t p) { return r * kRowUnits + p; }
 

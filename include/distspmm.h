@@ -400,7 +400,7 @@ int dsp_spmm_act_grad(const dsp_pattern *p, const dsp_act_grad_desc *d, void *wo
  * first row, say). Rows without entries give out = 0, lse = -infinity. Entries that A does not list are not part of a row,
  * whatever k and v hold there.
  * q, out: rows x heads x dim; k, v: cols x kv_heads x dim; dtype; strides in elements (row, head), dim contiguous; addresses
- * and strides multiples of 16 bytes (INVALID otherwise). dim: a multiple of 8 up to 256 (UNSUPPORTED otherwise). lse: rows x
+ * and strides multiples of 16 bytes, none negative (INVALID otherwise), row strides < 2^30 (UNSUPPORTED otherwise). dim: a multiple of 8 up to 256 (UNSUPPORTED otherwise). lse: rows x
  * heads fp32, contiguous, or NULL. No output may overlap an input. Workspace, device, stream and order of sums as for
  * dsp_spmm_act. The pattern needs DSP_PATTERN_ATTENTION, for gradients DSP_PATTERN_GRAD too (STATE otherwise). */
 typedef struct dsp_attn_desc {

@@ -77,7 +77,7 @@ def decode_desc(**kw):
 @pytest.mark.parametrize("bad,code", [
     (dict(dtype=3), -1), (dict(heads=0), -1), (dict(kv_heads=3), -1), (dict(kv_heads=0), -1), (dict(dim=0), -6), (dict(dim=20), -6),
     (dict(dim=264), -6), (dict(softcap=-1.0), -1), (dict(softcap=float("inf")), -1), (dict(scale=float("nan")), -1), (dict(q=None), -1),
-    (dict(q=(1 << 12) + 2), -1), (dict(k_row=129), -1), (dict(out=None), -1), (dict(indptr=None), -1), (dict(indices=None), -1),
+    (dict(q=(1 << 12) + 2), -1), (dict(k_row=129), -1), (dict(k_row=-128), -1), (dict(v_row=1 << 30), -6), (dict(out=None), -1), (dict(indptr=None), -1), (dict(indices=None), -1),
     (dict(rows=-1), -1), (dict(nnz=-1), -1), (dict(rows=1 << 25), -6), (dict(nnz=1 << 31), -6), (dict(), -1)])
 def test_decode_refuses(bad, code):
     """Bad arguments, and (last) a missing workspace: all refused before anything reaches a device."""
