@@ -66,10 +66,13 @@ __device__ __forceinline__ float group_sum(float x) {
   return x;
 }
 
-// u_ij in units of log 2, and the capped score's tanh.
-__device__ __forceinline__ float score2(const AttnArgs &a, float dot, float inv_cap2, float slope, float dist, float &th) {
+// u_ij in units of log 2, and the capped score's tanh (tanhf: fp32 results are held to fp32's rounding).
+__device__ __forceinline__ float score2(const AttnArgs &a, float dot, float inv_cap, float slope, float dist, float &th) {
   float s = dot * a.scale;
-  if (a.cap > 0.f) s = capped(s, a.cap, inv_cap2, th);
+  if (a.cap > 0.f) {
+    th = tanhf(s * inv_cap);
+    s = a.cap * th;
+  }
   return (s - slope * dist) * kLog2e;
 }
 
@@ -80,7 +83,7 @@ __device__ __forceinline__ void attend(const Rows &d, const AttnArgs &a, int64_t
                                        float &m, float &l, float (&acc)[VPL][VE]) {
   constexpr int G = 32 / LPR, U = 4;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
-  const float slope = a.slopes ? __ldg(a.slopes + h) : 0.f, inv_cap2 = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+  const float slope = a.slopes ? __ldg(a.slopes + h) : 0.f, inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
   float q[VPL][VE];
   typename H::Raw raw[VPL];
   H::fetch(a.q, row, h, lane, a.dim, true, raw);
@@ -106,7 +109,7 @@ __device__ __forceinline__ void attend(const Rows &d, const AttnArgs &a, int64_t
     for (int u = 0; u < U; ++u) {
       const int64_t at = b + u * G + g;
       float th;
-      s[u] = score2(a, group_sum<LPR>(H::dot(q, k[u])), inv_cap2, slope, d.distance(a, row, end, at, c[u]), th);
+      s[u] = score2(a, group_sum<LPR>(H::dot(q, k[u])), inv_cap, slope, d.distance(a, row, end, at, c[u]), th);
       if (!d.in_range(c[u])) s[u] = NAN;  // a key that does not exist: the row shows it
       if (at >= pe) s[u] = -INFINITY;
       top = fmaxf(top, s[u]);
@@ -163,7 +166,7 @@ __device__ __forceinline__ void attend_dq(const PlanRows &d, const AttnArgs &a, 
                                           float &delta, float (&x)[VPL][VE], float (&y)[VPL][VE]) {
   constexpr int G = 32 / LPR, U = 4;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
-  const float slope = a.slopes ? __ldg(a.slopes + h) : 0.f, inv_cap2 = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+  const float slope = a.slopes ? __ldg(a.slopes + h) : 0.f, inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
   float q[VPL][VE], dout[VPL][VE];
   typename H::Raw raw[VPL];
   H::fetch(a.q, row, h, lane, a.dim, true, raw);
@@ -189,7 +192,7 @@ __device__ __forceinline__ void attend_dq(const PlanRows &d, const AttnArgs &a, 
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float th = 0.f;
-      const float s = score2(a, group_sum<LPR>(H::dot(q, k[u])), inv_cap2, slope, d.distance(a, row, 0, 0, c[u]), th);
+      const float s = score2(a, group_sum<LPR>(H::dot(q, k[u])), inv_cap, slope, d.distance(a, row, 0, 0, c[u]), th);
       const float dp = group_sum<LPR>(H::dot(dout, v[u]));
       if (b + u * G + g < pe) {
         const float w = lse2 == -INFINITY ? 0.f : exp2_approx(s - lse2), wc = w * (1.f - th * th);
@@ -219,7 +222,7 @@ __device__ __forceinline__ void attend_dkv(const PlanRows &d, const AttnArgs &a,
                                            float (&dk)[VPL][VE], float (&dv)[VPL][VE]) {
   constexpr int G = 32 / LPR, U = 4;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
-  const float inv_cap2 = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f;
+  const float inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
   float k[VPL][VE], v[VPL][VE];
   typename H::Raw raw[VPL];
   H::fetch(a.k, row, hk, lane, a.dim, true, raw);
@@ -248,7 +251,7 @@ __device__ __forceinline__ void attend_dkv(const PlanRows &d, const AttnArgs &a,
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         float th = 0.f;
-        const float s = score2(a, group_sum<LPR>(H::dot(k, q[u])), inv_cap2, slope,
+        const float s = score2(a, group_sum<LPR>(H::dot(k, q[u])), inv_cap, slope,
                                fabsf((float)(c[u] + a.row_offset - row)), th);
         const float dp = group_sum<LPR>(H::dot(v, dout[u]));
         if (b + u * G + g < pe) {

@@ -17,7 +17,8 @@
 // causal mask with a distance bias scores fall along that way, and the maximum stands after one tile.
 //
 // Rounding: weights enter the second product in the operands' 16-bit type (half a step each; the sum l is of unrounded
-// weights). fp16 has few exponents: weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is
+// weights), the score gradients of dq as hi + lo (delta comes from a rounded out; both errors together would be 1.5 times the
+// result's own rounding). fp16 has few exponents: weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is
 // scaled by a power of two that brings the largest |dout| near 16; both come off in the epilogue.
 //
 // Masks and values that are not finite: an entry that is not listed has weight 0, but 0 x NaN in the product is NaN. So a row
@@ -32,6 +33,7 @@
 
 #include "attn_row.cuh"
 #include "attn_tile.h"
+#include "frag.cuh"
 #include "tcgen05.cuh"
 
 namespace dsp {
@@ -113,17 +115,6 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 constexpr int kAccBars = 4;
 __device__ __forceinline__ bool wait_acc(uint32_t bars, int it, volatile int *dead, int *err, int code) {
   return warp_wait(bars + 8 * (it % kAccBars), (it / kAccBars) & 1, dead, err, code);
-}
-
-template <class T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    const __nv_bfloat162 x = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&x);
-  } else {
-    const __half2 x = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&x);
-  }
 }
 
 // s -> cap tanh(k s), k = scale / cap, of N columns of this thread's row. Where no score of the warp's rows is above half the cap, as
@@ -375,6 +366,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
 #pragma unroll
         for (int k = 0; k < 4; ++k)  // 16 streamed rows each: 8 columns of weights, 2048 bytes of the stream's image
           mma_ts(tm_acc0, tm_s + b * 64 + k * 8, desc_mn_major((M == kDq ? x0 : x1) + k * 2048, 8192), id_second, it > 0 || k > 0);
+        if (M == kDq) {  // what rounding took from the score gradients
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_ts(tm_acc0, tm_r + b * 64 + k * 8, desc_mn_major(x0 + k * 2048, 8192), id_second, true);
+        }
         if (M == kDkv) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
@@ -650,9 +645,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             }
           }
           uint32_t v[16];
+          if constexpr (M == kDq) {
+            uint32_t lo[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) v[c / 2] = pack2<T>(e[c], e[c + 1]);
-          tmem_st16((M == kDkv ? tm_r : tm_s) + lanes + b * 64 + half * 16, v);
+            for (int c = 0; c < 32; c += 2) split2<T>(e[c], e[c + 1], v[c / 2], lo[c / 2]);
+            tmem_st16(tm_s + lanes + b * 64 + half * 16, v);
+            tmem_st16(tm_r + lanes + b * 64 + half * 16, lo);
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) v[c / 2] = pack2<T>(e[c], e[c + 1]);
+            tmem_st16(tm_r + lanes + b * 64 + half * 16, v);
+          }
         }
         tmem_wait_st();
         tc_fence_before();

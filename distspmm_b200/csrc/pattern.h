@@ -76,8 +76,10 @@ struct HostTiles {
   std::vector<uint64_t> words;
   int32_t max_tiles = 0;
 };
-// Entries per tile from which the tile form is built and used (see tiles_pay in pattern.cu).
-constexpr int64_t kTileFill = 192;
+// Entries per tile from which the tile form is built and used. A tile costs the same however many entries it has, a row's entry
+// by itself; 8 heads of 64, training step, tiles / rows in us: R-MAT 11 (92 entries a tile) 176 / 150, 4096 rows of 60 random
+// columns (120) 371 / 463, R-MAT 10 (167) 108 / 100, 2048 rows of 60 (240) 176 / 252, a window of 8 over 4096 rows (345) 72 / 119.
+constexpr int64_t kTileFill = 160;
 // False (and out untouched) where tiles would hold fewer than kTileFill entries on average.
 bool build_tiles(int32_t n, int32_t n_cols, const HostDir &d, bool always, HostTiles *out);
 
