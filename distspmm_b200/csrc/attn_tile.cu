@@ -17,7 +17,7 @@
 // causal mask with a distance bias scores fall along that way, and the maximum stands after one tile.
 //
 // Rounding: weights enter the second product in the operands' 16-bit type (half a step each; the sum l is of unrounded
-// weights), the score gradients of dq as hi + lo (delta comes from a rounded out; both errors together would be 1.5 times the
+// weights), the score gradients as hi + lo (delta comes from a rounded out; both errors together would be 1.5 times the
 // result's own rounding). fp16 has few exponents: weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is
 // scaled by a power of two that brings the largest |dout| near 16; both come off in the epilogue.
 //
@@ -363,17 +363,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         if (M == kFwd && !wait(bar_x1_full + 8 * s, (it / ST) & 1, dead, x.err, 6)) return false;
         tc_fence_after();
         const uint32_t x0 = sm_x0 + s * C::kStreamBytes, x1 = sm_x1 + s * C::kStreamBytes;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)  // 16 streamed rows each: 8 columns of weights, 2048 bytes of the stream's image
-          mma_ts(tm_acc0, tm_s + b * 64 + k * 8, desc_mn_major((M == kDq ? x0 : x1) + k * 2048, 8192), id_second, it > 0 || k > 0);
-        if (M == kDq) {  // what rounding took from the score gradients
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mma_ts(tm_acc0, tm_r + b * 64 + k * 8, desc_mn_major(x0 + k * 2048, 8192), id_second, true);
-        }
-        if (M == kDkv) {
+        // 16 streamed rows each: 8 columns of weights, 2048 bytes of the stream's image
+        if (M == kFwd) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            mma_ts(tm_acc1, tm_r + b * 64 + k * 8, desc_mn_major(x0 + k * 2048, 8192), id_second, it > 0 || k > 0);
+            mma_ts(tm_acc0, tm_s + b * 64 + k * 8, desc_mn_major(x1 + k * 2048, 8192), id_second, it > 0 || k > 0);
+        } else {
+          // each half of a score tile (32 columns) holds: of S the weights (dk, dv) and the low parts, of R the high parts
+          const uint32_t grads = M == kDq ? tm_acc0 : tm_acc1;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t at = b * 64 + (k / 2) * 32 + (k % 2) * 8;
+            const uint64_t d0 = desc_mn_major(x0 + k * 2048, 8192);
+            if (M == kDkv) mma_ts(tm_acc0, tm_s + at, desc_mn_major(x1 + k * 2048, 8192), id_second, it > 0 || k > 0);
+            mma_ts(grads, tm_r + at, d0, id_second, it > 0 || k > 0);
+            mma_ts(grads, tm_s + at + 16, d0, id_second, true);
+          }
         }
         if (M != kFwd) mma_commit(bar_x0_free + 8 * s);
         if (M != kDq) mma_commit(bar_x1_free + 8 * s);
@@ -620,7 +625,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             uint32_t w[16];
 #pragma unroll
             for (int c = 0; c < 32; c += 2) w[c / 2] = pack2<T>(p[c], p[c + 1]);
-            tmem_st16(tm_s + lanes + b * 64 + half * 16, w);
+            tmem_st16(tm_s + lanes + b * 64 + half * 32, w);
           }
           // score gradients: p (dp - delta) (1 - tanh^2), up to the scale
 #pragma unroll
@@ -644,18 +649,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
               mul2(e[c], e[c + 1], e[c], e[c + 1], z0, z1);
             }
           }
-          uint32_t v[16];
-          if constexpr (M == kDq) {
-            uint32_t lo[16];
+          uint32_t v[16], lo[16];
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) split2<T>(e[c], e[c + 1], v[c / 2], lo[c / 2]);
-            tmem_st16(tm_s + lanes + b * 64 + half * 16, v);
-            tmem_st16(tm_r + lanes + b * 64 + half * 16, lo);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 32; c += 2) v[c / 2] = pack2<T>(e[c], e[c + 1]);
-            tmem_st16(tm_r + lanes + b * 64 + half * 16, v);
-          }
+          for (int c = 0; c < 32; c += 2) split2<T>(e[c], e[c + 1], v[c / 2], lo[c / 2]);
+          tmem_st16(tm_r + lanes + b * 64 + half * 32, v);
+          tmem_st16(tm_s + lanes + b * 64 + half * 32 + 16, lo);
         }
         tmem_wait_st();
         tc_fence_before();
