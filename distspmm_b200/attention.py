@@ -15,26 +15,30 @@ from ._lib import call, dsp_attn_decode_desc, dsp_attn_desc, dsp_attn_grad_desc,
 from .pattern import DTYPES, SparsePattern, need, on_device, ptr, stream_of, wants_grad, workspace
 
 
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels can read it in place (dim contiguous, address and strides multiples of 16 bytes, no axis
-    expanded), else a contiguous copy."""
+def _heads(t: torch.Tensor):
+    """(tensor, (address, row stride, head stride)): t itself where the kernels can read it in place (dim contiguous, address
+    and strides multiples of 16 bytes, no axis expanded), else a contiguous copy. Strides of axes of length one are free and
+    are set to what the alignment rule accepts."""
+    n, h, w = t.shape
+    at = t.data_ptr()
+    if t.is_contiguous() and at % 16 == 0:
+        return t, (at, h * w, w)
+    rs, hs, ws = t.stride()
     e = t.element_size()
-    (n, h, w), (rs, hs, ws) = t.shape, t.stride()
-    ok = (ws == 1 or w == 1) and t.data_ptr() % 16 == 0 and (n <= 1 or (rs > 0 and rs * e % 16 == 0)) and (
-        h <= 1 or (hs > 0 and hs * e % 16 == 0))
-    return t if ok else t.contiguous()
-
-
-def _at(t: torch.Tensor):
-    """(address, row stride, head stride); strides of axes of length one are free and are set to what the alignment rule
-    accepts."""
-    (n, h, w), (rs, hs, _) = t.shape, t.stride()
-    return t.data_ptr(), rs if n > 1 else h * w, hs if h > 1 else w
+    if (ws == 1 or w == 1) and at % 16 == 0 and (n <= 1 or (rs > 0 and rs * e % 16 == 0)) and (
+            h <= 1 or (hs > 0 and hs * e % 16 == 0)):
+        return t, (at, rs if n > 1 else h * w, hs if h > 1 else w)
+    t = t.contiguous()
+    if t.data_ptr() % 16:  # contiguous already, at an odd address
+        t = t.clone()
+    return t, (t.data_ptr(), h * w, w)
 
 
 def _desc(q, k, v, out, lse, scale, softcap, slopes, row_offset):
-    return dsp_attn_desc(DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], scale, softcap, ptr(slopes), row_offset, *_at(q),
-                         *_at(k), *_at(v), *_at(out), ptr(lse))
+    """q, k, v, out: as _heads gives them."""
+    (n, heads, dim), kv_heads = q[0].shape, k[0].shape[1]
+    return dsp_attn_desc(DTYPES[q[0].dtype], heads, kv_heads, dim, scale, softcap, ptr(slopes), row_offset, *q[1], *k[1], *v[1],
+                         *out[1], ptr(lse))
 
 
 def _check(device, rows, keys, q, k, v, scale, softcap, slopes):
@@ -71,11 +75,11 @@ def sparse_attention_forward(p: SparsePattern, q, k, v, scale=None, softcap=0.0,
     """(out, lse): out [rows, heads, dim] in q's type, lse [rows, heads] fp32."""
     _pattern(p)
     q, k, v, scale, softcap, slopes = _check(p.device, p.rows, p.cols, q, k, v, scale, softcap, slopes)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-    d = _desc(q, k, v, out, lse, scale, softcap, slopes, row_offset)
+    out = torch.empty(q[0].shape, dtype=q[0].dtype, device=q[0].device)
+    lse = torch.empty(out.shape[:2], dtype=torch.float32, device=out.device)
+    d = _desc(q, k, v, _heads(out), lse, scale, softcap, slopes, row_offset)
     nbytes = lib().dsp_attn_workspace(p._h, ctypes.byref(d))
-    ws = workspace(nbytes, q.device)
+    ws = workspace(nbytes, out.device)
     call("dsp_attn", p._h, ctypes.byref(d), ptr(ws), nbytes, stream_of(p.device))
     return out, lse
 
@@ -86,15 +90,16 @@ def sparse_attention_backward(p: SparsePattern, dout, q, k, v, out, lse, scale=N
     took them."""
     _pattern(p, grad=True)
     q, k, v, scale, softcap, slopes = _check(p.device, p.rows, p.cols, q, k, v, scale, softcap, slopes)
-    on_device("dout", dout, p.device, q.dtype, q.shape)
-    on_device("out", out, p.device, q.dtype, q.shape)
-    on_device("lse", lse, p.device, torch.float32, q.shape[:2])
+    shape, t = q[0].shape, q[0].dtype
+    on_device("dout", dout, p.device, t, shape)
+    on_device("out", out, p.device, t, shape)
+    on_device("lse", lse, p.device, torch.float32, shape[:2])
     dout, out, lse = _heads(dout), _heads(out), lse.contiguous()
-    res = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-    g = dsp_attn_grad_desc(_desc(q, k, v, out, lse, scale, softcap, slopes, row_offset), *_at(dout), *_at(res[0]), *_at(res[1]),
-                           *_at(res[2]))
+    res = [torch.empty(x.shape, dtype=t, device=lse.device) for x, _ in (q, k, v)]
+    g = dsp_attn_grad_desc(_desc(q, k, v, out, lse, scale, softcap, slopes, row_offset), *dout[1], *_heads(res[0])[1],
+                           *_heads(res[1])[1], *_heads(res[2])[1])
     nbytes = lib().dsp_attn_grad_workspace(p._h, ctypes.byref(g.fwd))
-    ws = workspace(nbytes, q.device)
+    ws = workspace(nbytes, lse.device)
     call("dsp_attn_grad", p._h, ctypes.byref(g), ptr(ws), nbytes, stream_of(p.device))
     return tuple(res)
 
@@ -149,11 +154,11 @@ def sparse_attention_decode(q, k_cache, v_cache, indptr, indices, scale=None, so
         need(False, f"indptr must have {rows + 1} entries, has {tuple(indptr.shape)}")
     q, k, v, scale, softcap, slopes = _check(dev, rows, None, q, k_cache, v_cache, scale, softcap, slopes)
     indptr, indices = indptr.contiguous(), indices.contiguous()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device) if return_lse else None
-    g = dsp_attn_decode_desc(_desc(q, k, v, out, lse, scale, softcap, slopes, 0), rows, indices.numel(), k.shape[0],
+    out = torch.empty(q[0].shape, dtype=q[0].dtype, device=q[0].device)
+    lse = torch.empty(out.shape[:2], dtype=torch.float32, device=out.device) if return_lse else None
+    g = dsp_attn_decode_desc(_desc(q, k, v, _heads(out), lse, scale, softcap, slopes, 0), rows, indices.numel(), k[0].shape[0],
                              indptr.data_ptr(), indices.data_ptr(), dev)
     nbytes = lib().dsp_attn_decode_workspace(ctypes.byref(g))
-    ws = workspace(nbytes, q.device)
+    ws = workspace(nbytes, out.device)
     call("dsp_attn_decode", ctypes.byref(g), ptr(ws), nbytes, stream_of(dev))
     return (out, lse) if return_lse else out
