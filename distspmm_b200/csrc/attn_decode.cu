@@ -195,26 +195,29 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
 }
 
 // Rows cut across chunks: a block per row and head. The partials' weights 2^(m - max) first, each by a thread, then the
-// weighted sums in chunk order, a thread per column.
+// weighted sums: groups of dim threads, a thread per column, take every groups-th partial, and their sums are added in order.
+constexpr int kJoin = 512;
 template <class T>
-__global__ void __launch_bounds__(kThreads) attn_decode_join_kernel(const ListRows d, const AttnArgs a) {
-  __shared__ float weight[kThreads], red[4];
+__global__ void __launch_bounds__(kJoin) attn_decode_join_kernel(const ListRows d, const AttnArgs a) {
+  __shared__ float weight[kJoin], red[kJoin / 32], part[kJoin];
   const int64_t r = blockIdx.x;
   const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t c0 = row_start(r, d.ptr(r)) / d.L, c1 = min(row_start(r, d.ptr(r + 1)) / d.L, (int64_t)d.n_chunks - 1);
   if (c0 >= c1) return;  // not cut
   auto slot = [&](int64_t c) { return (c == c0 ? 2 * c + 1 : 2 * c) * a.heads + h; };
   float m = -INFINITY;
-  for (int64_t c = c0 + tid; c <= c1; c += kThreads) m = fmaxf(m, a.slot_ml[2 * slot(c)]);
+  for (int64_t c = c0 + tid; c <= c1; c += kJoin) m = fmaxf(m, a.slot_ml[2 * slot(c)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (lane == 0) red[warp] = m;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int w = 0; w < kJoin / 32; ++w) m = fmaxf(m, red[w]);
   const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, acc[2] = {0.f, 0.f};
-  for (int64_t b = c0; b <= c1; b += kThreads) {
-    const int n = (int)min((int64_t)kThreads, c1 - b + 1);
+  const int groups = kJoin / a.dim, g = tid / a.dim, col = tid - g * a.dim;  // dim <= 256
+  float l = 0.f, acc = 0.f;
+  for (int64_t b = c0; b <= c1; b += kJoin) {
+    const int n = (int)min((int64_t)kJoin, c1 - b + 1);
     float w = 0.f;
     if (tid < n) {
       const int64_t s = slot(b + tid);
@@ -224,25 +227,24 @@ __global__ void __launch_bounds__(kThreads) attn_decode_join_kernel(const ListRo
     __syncthreads();
     weight[tid] = w;
     __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int col = tid + k * kThreads;
-      if (col >= a.dim) continue;
+    if (g < groups) {
 #pragma unroll 8
-      for (int i = 0; i < n; ++i) acc[k] = fmaf(weight[i], a.slots[slot(b + i) * a.dim + col], acc[k]);
+      for (int i = g; i < n; i += groups) acc = fmaf(weight[i], a.slots[slot(b + i) * a.dim + col], acc);
     }
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   __syncthreads();
   if (lane == 0) red[warp] = l;
+  part[tid] = acc;
   __syncthreads();
-  l = (red[0] + red[1]) + (red[2] + red[3]);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *dst = (T *)a.out.p + r * a.out.row + (int64_t)h * a.out.head;
+  l = 0.f;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (tid + k * kThreads < a.dim) dst[tid + k * kThreads] = T(acc[k] * inv);
+  for (int w = 0; w < kJoin / 32; ++w) l += red[w];
+  if (tid < a.dim) {
+    for (int k = 1; k < groups; ++k) acc += part[k * a.dim + tid];
+    ((T *)a.out.p)[r * a.out.row + h * a.out.head + tid] = T(l == 0.f ? 0.f : acc / l);
+  }
   if (a.lse && tid == 0) a.lse[r * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
@@ -271,9 +273,9 @@ int32_t decode_units(int64_t rows, int64_t nnz, int heads, int kv_heads, bool te
 int decode_join(const ListRows &d, const AttnArgs &a, int dtype, cudaStream_t s) {
   if (d.n_chunks > 1) {
     const dim3 grid((unsigned)d.rows, (unsigned)a.heads);
-    if (dtype == DSP_F32) attn_decode_join_kernel<float><<<grid, kThreads, 0, s>>>(d, a);
-    else if (dtype == DSP_BF16) attn_decode_join_kernel<__nv_bfloat16><<<grid, kThreads, 0, s>>>(d, a);
-    else attn_decode_join_kernel<__half><<<grid, kThreads, 0, s>>>(d, a);
+    if (dtype == DSP_F32) attn_decode_join_kernel<float><<<grid, kJoin, 0, s>>>(d, a);
+    else if (dtype == DSP_BF16) attn_decode_join_kernel<__nv_bfloat16><<<grid, kJoin, 0, s>>>(d, a);
+    else attn_decode_join_kernel<__half><<<grid, kJoin, 0, s>>>(d, a);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_attn_decode: %s", cudaGetErrorString(e));
