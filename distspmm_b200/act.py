@@ -112,6 +112,8 @@ def spmm_act(p: SparsePattern, B: torch.Tensor, values=None, bias=None, residual
     type; act: None, "relu", "silu" or "gelu" (erf form). Runs on the current stream."""
     if not wants_grad(B, values, bias, residual):
         return spmm_act_forward(p, B, values, bias, residual, act)[0]
+    need(isinstance(p, SparsePattern), "the first argument must be a SparsePattern")
+    need(p.grad or not B.requires_grad, "a gradient of B needs a SparsePattern(..., grad=True)")
     if values is None:
         values = p.values
     return _SpmmAct.apply(p, act, B, values, bias, residual)

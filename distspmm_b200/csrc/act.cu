@@ -680,6 +680,7 @@ int check_type(const char *who, int dtype, int act, int N) {
   DSP_TRY_ARG(dtype >= DSP_F32 && dtype <= DSP_F16, "%s: dtype %d", who, dtype);
   DSP_TRY_ARG(act >= DSP_ACT_NONE && act <= DSP_ACT_GELU, "%s: act %d", who, act);
   DSP_TRY_ARG(N >= 0, "%s: N = %d", who, N);
+  if (N > (1 << 22)) return fail(DSP_ERR_UNSUPPORTED, "%s: N = %d: up to 2^22 is wanted", who, N);
   return DSP_OK;
 }
 

@@ -400,7 +400,8 @@ int check_attn(const char *who, const dsp_attn_desc *d, int64_t rows, int64_t ke
               "%s: %d query heads, %d key/value heads", who, d->heads, d->kv_heads);
   if (d->dim <= 0 || d->dim > 256 || d->dim % 8)
     return fail(DSP_ERR_UNSUPPORTED, "%s: dim %d: a multiple of 8 up to 256 is wanted", who, d->dim);
-  DSP_TRY_ARG(d->scale == d->scale && d->softcap >= 0.f && d->softcap < INFINITY, "%s: scale %g, softcap %g", who, d->scale, d->softcap);
+  DSP_TRY_ARG(fabsf(d->scale) < INFINITY && (d->softcap == 0.f || (d->softcap >= 1e-6f && d->softcap < INFINITY)),
+              "%s: scale %g, softcap %g", who, d->scale, d->softcap);
   int rc;
   if (rows > 0 && ((rc = check_heads(who, "q", d->q, d->q_row, d->q_head, d->dtype)) ||
                    (rc = check_heads(who, "out", d->out, d->out_row, d->out_head, d->dtype))))

@@ -124,7 +124,7 @@ struct CapPoly {
   float limit, c[5];  // of s^2; s (c0 + c1 s^2 + ...)
   __device__ __forceinline__ CapPoly(float scale, float cap) {
     const float k = cap > 0.f ? scale / cap : 0.f, k2 = k * k;
-    limit = k2 > 0.f ? 0.25f / k2 : INFINITY;
+    limit = k2 < 1e20f ? 0.25f / fmaxf(k2, 1e-20f) : -1.f;  // beyond, the coefficients overflow
     float f = k * cap;
     c[0] = 0.999999987f * f;
     c[1] = -0.333330719f * (f *= k2);

@@ -43,7 +43,8 @@ class SparsePattern:
 
     @property
     def values(self) -> torch.Tensor:
-        """A's own values on the device (fp32, CSR order), uploaded on first use."""
+        """A's own values on the device (fp32, CSR order), uploaded on first use (so use it once
+        before capturing a graph that relies on it)."""
         if self._values is None:
             self._values = torch.from_numpy(self._host_values).to(torch.device("cuda", self.device))
         return self._values

@@ -342,6 +342,7 @@ int dsp_pattern_check_error(dsp_pattern *p);
 #define DSP_ACT_GELU 3 /* z * Phi(z), the erf form */
 
 /* out = act(A*B + bias) + residual, row by row:
+ *   N         up to 2^22
  *   values    [nnz] fp32, device, in A's CSR order
  *   B         cols x N, dtype, leading dimension ldb (elements; ldb and lddo < 2^30)
  *   bias      [N] fp32, or NULL
@@ -396,7 +397,7 @@ int dsp_spmm_act_grad(const dsp_pattern *p, const dsp_act_grad_desc *d, void *wo
  * documents, prefix, the edges of a graph), for each query head h (key/value head h / (heads / kv_heads)):
  *   u_ij = softcap * tanh(scale * q_i.k_j / softcap) - slopes[h] * |i + row_offset - j|
  *   out_i = sum_j exp(u_ij - lse_i) v_j,   lse_i = log sum_j exp(u_ij)   (natural logarithm)
- * softcap = 0: no cap. slopes [heads] fp32 (device) or NULL: no distance bias. row_offset: the position of row 0 (a rank's
+ * softcap = 0: no cap (else at least 1e-6). slopes [heads] fp32 (device) or NULL: no distance bias. row_offset: the position of row 0 (a rank's
  * first row, say). Rows without entries give out = 0, lse = -infinity. Entries that A does not list are not part of a row,
  * whatever k and v hold there.
  * q, out: rows x heads x dim; k, v: cols x kv_heads x dim; dtype; strides in elements (row, head), dim contiguous; addresses

@@ -352,6 +352,8 @@ def test_refusals(gpu):
         d.spmm_act(p, B, residual=dy.to(BF16))
     with pytest.raises(ValueError, match="grad=True"):
         d.spmm_act_backward(p, dy, B, None)
+    with pytest.raises(ValueError, match="grad=True"):
+        d.spmm_act(p, B.clone().requires_grad_())
     with pytest.raises(ValueError, match="needs pre"):
         d.spmm_act_backward(p, dy, B, None, act="silu", need_B=False)
     ok = (0, 0, 64, p.values.data_ptr(), B.data_ptr(), 64, None, None, 0, dy.data_ptr(), 64, None, 0)

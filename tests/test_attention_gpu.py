@@ -115,6 +115,9 @@ def test_large_scores(gpu, t):
     check(positional("window", 150, window=64), 2, 2, 64, t, scale=2.0)
     check(positional("window", 150, window=64), 2, 2, 64, t, scale=2.0, cap=5.0)
     check(positional("window", 150, window=64), 2, 2, 64, t, scale=0.0)
+    check(positional("window", 150, window=64), 2, 2, 64, t, scale=0.0, cap=5.0)
+    check(positional("window", 150, window=64), 2, 2, 64, t, scale=0.125, cap=0.01)
+    check(positional("window", 150, window=64), 2, 2, 64, t, scale=-0.125, cap=7.0, bias=True)
 
 
 @pytest.mark.parametrize("t", [F32, BF16, F16])

@@ -76,9 +76,15 @@ def decode_desc(**kw):
 
 @pytest.mark.parametrize("bad,code", [
     (dict(dtype=3), -1), (dict(heads=0), -1), (dict(kv_heads=3), -1), (dict(kv_heads=0), -1), (dict(dim=0), -6), (dict(dim=20), -6),
-    (dict(dim=264), -6), (dict(softcap=-1.0), -1), (dict(softcap=float("inf")), -1), (dict(scale=float("nan")), -1), (dict(q=None), -1),
+    (dict(dim=264), -6), (dict(softcap=-1.0), -1), (dict(softcap=float("inf")), -1), (dict(softcap=1e-9), -1), (dict(scale=float("inf")), -1), (dict(scale=float("nan")), -1), (dict(q=None), -1),
     (dict(q=(1 << 12) + 2), -1), (dict(k_row=129), -1), (dict(k_row=-128), -1), (dict(v_row=1 << 30), -6), (dict(out=None), -1), (dict(indptr=None), -1), (dict(indices=None), -1),
     (dict(rows=-1), -1), (dict(nnz=-1), -1), (dict(rows=1 << 25), -6), (dict(nnz=1 << 31), -6), (dict(), -1)])
 def test_decode_refuses(bad, code):
     """Bad arguments, and (last) a missing workspace: all refused before anything reaches a device."""
     assert status("dsp_attn_decode", ctypes.byref(decode_desc(**bad)), None, 0, None) == code
+
+
+def test_act_refuses_wide_products():
+    d1 = dsp_act_desc(0, 0, (1 << 22) + 1)
+    p = 1 << 12  # never read: the check comes first
+    assert status("dsp_spmm_act", p, ctypes.byref(d1), None, 0, None) == -6
