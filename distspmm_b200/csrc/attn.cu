@@ -23,21 +23,18 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <class Rows, class T, int VE, int LPR, int VPL>
-__global__ void __launch_bounds__(kThreads) attn_rows_kernel(const Rows d, const AttnArgs a) {
+// Rows r0 .. r1 and entries p0 .. p1 of a chunk, for head h.
+template <class T, int VE, int LPR, int VPL, class Rows>
+__device__ __forceinline__ void chunk_rows(const Rows &d, const AttnArgs &a, int64_t chunk, int h, typename Rows::Index r0,
+                                           typename Rows::Index r1, typename Rows::Index p0, typename Rows::Index p1) {
   using H = HeadRow<T, VE, LPR, VPL>;
-  const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
-  const int64_t chunk = item / a.heads;
-  const int h = (int)(item - chunk * a.heads);
-  if (chunk >= d.chunks()) return;
+  using I = typename Rows::Index;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
-  int64_t r0, r1, p0, p1;
-  d.chunk(chunk, r0, r1, p0, p1);
   const bool head_cut = p0 > d.ptr(r0);
-  int64_t p = p0;
-  for (int64_t row = r0; row <= r1; ++row) {
+  I p = p0;
+  for (I row = r0; row <= r1; ++row) {
     if (row == r1 && (p >= p1 || row >= d.n())) break;
-    const int64_t end = d.ptr(row + 1), pe = row < r1 ? end : p1;
+    const I end = d.ptr(row + 1), pe = row < r1 ? end : p1;
     float acc[VPL][VE], m, l;
     attend<H, LPR>(d, a, row, h, p, pe, end, m, l, acc);
     const bool cut_head = row == r0 && head_cut;
@@ -52,21 +49,40 @@ __global__ void __launch_bounds__(kThreads) attn_rows_kernel(const Rows d, const
   }
 }
 
-// dq and delta of the pattern's rows.
-template <class T, int VE, int LPR, int VPL>
-__global__ void __launch_bounds__(kThreads) attn_dq_kernel(const PlanRows d, const AttnArgs a) {
-  using H = HeadRow<T, VE, LPR, VPL>;
+template <class Rows, class T, int VE, int LPR, int VPL>
+__global__ void __launch_bounds__(kThreads, VPL == 1 ? 3 : 2) attn_rows_kernel(const Rows d, const AttnArgs a) {
   const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
   const int64_t chunk = item / a.heads;
   const int h = (int)(item - chunk * a.heads);
   if (chunk >= d.chunks()) return;
+  if constexpr (std::is_same<Rows, PlanRows>::value) {
+    __shared__ ChunkLists lists[kThreads / 32];
+    const StagedRows s(d, chunk, lists[threadIdx.x >> 5]);
+    chunk_rows<T, VE, LPR, VPL>(s, a, chunk, h, s.r0, s.r1, s.p0, s.p1);
+  } else {
+    int64_t r0, r1, p0, p1;
+    d.chunk(chunk, r0, r1, p0, p1);
+    chunk_rows<T, VE, LPR, VPL>(d, a, chunk, h, r0, r1, p0, p1);
+  }
+}
+
+// dq and delta of the pattern's rows.
+template <class T, int VE, int LPR, int VPL>
+__global__ void __launch_bounds__(kThreads, VPL == 1 ? 3 : 2) attn_dq_kernel(const PlanRows rows, const AttnArgs a) {
+  using H = HeadRow<T, VE, LPR, VPL>;
+  const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
+  const int64_t chunk = item / a.heads;
+  const int h = (int)(item - chunk * a.heads);
+  if (chunk >= rows.chunks()) return;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
-  int64_t r0, r1, p, p1;
-  d.chunk(chunk, r0, r1, p, p1);
+  __shared__ ChunkLists lists[kThreads / 32];
+  const StagedRows d(rows, chunk, lists[threadIdx.x >> 5]);
+  const int32_t r0 = d.r0, r1 = d.r1, p1 = d.p1;
+  int32_t p = d.p0;
   const bool head_cut = p > d.ptr(r0);
-  for (int64_t row = r0; row <= r1; ++row) {
+  for (int32_t row = r0; row <= r1; ++row) {
     if (row == r1 && p >= p1) break;
-    const int64_t pe = row < r1 ? d.ptr(row + 1) : p1;
+    const int32_t pe = row < r1 ? d.ptr(row + 1) : p1;
     float delta, x[VPL][VE], y[VPL][VE];
     attend_dq<H, LPR>(d, a, row, h, p, pe, delta, x, y);
     const bool cut_head = row == r0 && head_cut;
@@ -83,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) attn_dq_kernel(const PlanRows d, con
 #pragma unroll
         for (int i = 0; i < VE; ++i) x[w][i] = (x[w][i] - delta * y[w][i]) * a.scale;
       if (g == 0) H::store(a.dq, row, h, lane, a.dim, x);
-      if ((threadIdx.x & 31) == 0) a.delta[row * a.heads + h] = delta;
+      if ((threadIdx.x & 31) == 0) a.delta[(int64_t)row * a.heads + h] = delta;
     }
     p = pe;
   }
@@ -91,20 +107,22 @@ __global__ void __launch_bounds__(kThreads) attn_dq_kernel(const PlanRows d, con
 
 // dk and dv of the pattern's columns (d: the transposed pattern), one key/value head.
 template <class T, int VE, int LPR, int VPL>
-__global__ void __launch_bounds__(kThreads) attn_dkv_kernel(const PlanRows d, const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, VPL == 1 ? 3 : 2) attn_dkv_kernel(const PlanRows rows, const AttnArgs a) {
   using H = HeadRow<T, VE, LPR, VPL>;
   const int kv_heads = a.heads / a.group;
   const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
   const int64_t chunk = item / kv_heads;
   const int hk = (int)(item - chunk * kv_heads);
-  if (chunk >= d.chunks()) return;
+  if (chunk >= rows.chunks()) return;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
-  int64_t r0, r1, p, p1;
-  d.chunk(chunk, r0, r1, p, p1);
+  __shared__ ChunkLists lists[kThreads / 32];
+  const StagedRows d(rows, chunk, lists[threadIdx.x >> 5]);
+  const int32_t r0 = d.r0, r1 = d.r1, p1 = d.p1;
+  int32_t p = d.p0;
   const bool head_cut = p > d.ptr(r0);
-  for (int64_t row = r0; row <= r1; ++row) {  // a row here is a column of A
+  for (int32_t row = r0; row <= r1; ++row) {  // a row here is a column of A
     if (row == r1 && p >= p1) break;
-    const int64_t pe = row < r1 ? d.ptr(row + 1) : p1;
+    const int32_t pe = row < r1 ? d.ptr(row + 1) : p1;
     float dk[VPL][VE], dv[VPL][VE];
     attend_dkv<H, LPR>(d, a, row, hk, p, pe, dk, dv);
     const bool cut_head = row == r0 && head_cut;

@@ -7,6 +7,7 @@ namespace dsp {
 // Rows listed by a CSR in device memory that nothing has validated: every value read from it is bounded before it is used,
 // so that no list can make the kernel leave its operands.
 struct ListRows {
+  using Index = int64_t;
   const int64_t *indptr, *indices;
   int64_t rows, nnz, keys;
   int32_t n_chunks, L;

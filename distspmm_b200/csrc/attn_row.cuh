@@ -7,6 +7,7 @@ namespace dsp {
 
 // Rows and entries of a prepared pattern.
 struct PlanRows {
+  using Index = int32_t;
   DirView d;
   __device__ int64_t chunks() const { return d.n_chunks; }
   __device__ void chunk(int64_t c, int64_t &r0, int64_t &r1, int64_t &p0, int64_t &p1) const {
@@ -20,6 +21,28 @@ struct PlanRows {
   }
   __device__ bool in_range(int64_t) const { return true; }
   __device__ int32_t units() const { return d.L; }
+};
+
+// A chunk of a prepared pattern with its lists in shared memory: one coalesced read instead of a wait for each step.
+struct ChunkLists {
+  int32_t cols[kMaxUnits];
+  int32_t ptr[kMaxUnits / kRowUnits + 4];
+};
+struct StagedRows : PlanRows {
+  const int32_t *cols_, *ptr_;
+  int32_t r0, r1, p0, p1;
+  __device__ __forceinline__ StagedRows(const PlanRows &rows, int64_t c, ChunkLists &list) : PlanRows(rows) {
+    const int lane = threadIdx.x & 31;
+    r0 = __ldg(d.row0 + c), r1 = __ldg(d.row0 + c + 1), p0 = __ldg(d.nz0 + c), p1 = __ldg(d.nz0 + c + 1);
+    for (int i = lane; i <= r1 - r0 + 1; i += 32)
+      if (r0 + i <= d.n) list.ptr[i] = __ldg(d.ptr + r0 + i);
+#pragma unroll 4
+    for (int i = lane; i < p1 - p0; i += 32) list.cols[i] = __ldg(d.cols + p0 + i);
+    __syncwarp();
+    cols_ = list.cols - p0, ptr_ = list.ptr - r0;
+  }
+  __device__ int32_t ptr(int32_t r) const { return ptr_[r]; }
+  __device__ int32_t col(int32_t p) const { return cols_[p]; }
 };
 
 // A head's row in the lanes of a group: VPL vectors of VE elements.
@@ -79,7 +102,8 @@ __device__ __forceinline__ float score2(const AttnArgs &a, float dot, float inv_
 // The entries [p, pe) of a row (which ends at `end`) for head h: running maximum m, sum l and weighted sum acc, over all
 // lanes of the warp. q: the row's query in the lanes of each group.
 template <class H, int LPR, class Rows, int VPL, int VE>
-__device__ __forceinline__ void attend(const Rows &d, const AttnArgs &a, int64_t row, int h, int64_t p, int64_t pe, int64_t end,
+__device__ __forceinline__ void attend(const Rows &d, const AttnArgs &a, int64_t row, int h, typename Rows::Index p,
+                                       typename Rows::Index pe, typename Rows::Index end,
                                        float &m, float &l, float (&acc)[VPL][VE]) {
   constexpr int G = 32 / LPR, U = 4;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
@@ -93,12 +117,12 @@ __device__ __forceinline__ void attend(const Rows &d, const AttnArgs &a, int64_t
   for (int w = 0; w < VPL; ++w)
 #pragma unroll
     for (int i = 0; i < VE; ++i) acc[w][i] = 0.f;
-  for (int64_t b = p; b < pe; b += G * U) {
+  for (typename Rows::Index b = p; b < pe; b += G * U) {
     typename H::Raw k[U][VPL], v[U][VPL];
-    int64_t c[U];
+    typename Rows::Index c[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = b + u * G + g;
+      const typename Rows::Index at = b + u * G + g;
       c[u] = at < pe ? d.col(at) : -1;
       const bool on = at < pe && d.in_range(c[u]);
       H::fetch(a.k, on ? c[u] : 0, h / a.group, lane, a.dim, on, k[u]);
@@ -107,7 +131,7 @@ __device__ __forceinline__ void attend(const Rows &d, const AttnArgs &a, int64_t
     float s[U], top = m;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = b + u * G + g;
+      const typename Rows::Index at = b + u * G + g;
       float th;
       s[u] = score2(a, group_sum<LPR>(H::dot(q, k[u])), inv_cap, slope, d.distance(a, row, end, at, c[u]), th);
       if (!d.in_range(c[u])) s[u] = NAN;  // a key that does not exist: the row shows it
@@ -161,8 +185,8 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, int64_t row, int h, f
 // The entries [p, pe) of a row for head h, for dq. With c = 1 - tanh^2: delta = sum p dp, x = sum p c dp k, y = sum p c k, so
 // that dq = scale (x - delta y) needs one pass, and delta is not that of a rounded out (in a row of one entry the two parts
 // cancel exactly, as they should).
-template <class H, int LPR, int VPL, int VE>
-__device__ __forceinline__ void attend_dq(const PlanRows &d, const AttnArgs &a, int64_t row, int h, int64_t p, int64_t pe,
+template <class H, int LPR, class Rows, int VPL, int VE>
+__device__ __forceinline__ void attend_dq(const Rows &d, const AttnArgs &a, int64_t row, int h, int32_t p, int32_t pe,
                                           float &delta, float (&x)[VPL][VE], float (&y)[VPL][VE]) {
   constexpr int G = 32 / LPR, U = 4;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
@@ -179,12 +203,12 @@ __device__ __forceinline__ void attend_dq(const PlanRows &d, const AttnArgs &a, 
   for (int w = 0; w < VPL; ++w)
 #pragma unroll
     for (int i = 0; i < VE; ++i) x[w][i] = y[w][i] = 0.f;
-  for (int64_t b = p; b < pe; b += G * U) {
+  for (int32_t b = p; b < pe; b += G * U) {
     typename H::Raw k[U][VPL], v[U][VPL];
-    int64_t c[U];
+    int32_t c[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int64_t at = b + u * G + g;
+      const int32_t at = b + u * G + g;
       c[u] = at < pe ? d.col(at) : 0;
       H::fetch(a.k, c[u], h / a.group, lane, a.dim, at < pe, k[u]);
       H::fetch(a.v, c[u], h / a.group, lane, a.dim, at < pe, v[u]);
@@ -217,8 +241,8 @@ __device__ __forceinline__ void attend_dq(const PlanRows &d, const AttnArgs &a, 
 
 // The entries [p, pe) of key `row` (d: the transposed pattern) for key/value head hk: dk and dv over the query heads of its
 // group, one after another in the same sums.
-template <class H, int LPR, int VPL, int VE>
-__device__ __forceinline__ void attend_dkv(const PlanRows &d, const AttnArgs &a, int64_t row, int hk, int64_t p, int64_t pe,
+template <class H, int LPR, class Rows, int VPL, int VE>
+__device__ __forceinline__ void attend_dkv(const Rows &d, const AttnArgs &a, int64_t row, int hk, int32_t p, int32_t pe,
                                            float (&dk)[VPL][VE], float (&dv)[VPL][VE]) {
   constexpr int G = 32 / LPR, U = 4;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
@@ -235,18 +259,18 @@ __device__ __forceinline__ void attend_dkv(const PlanRows &d, const AttnArgs &a,
     for (int i = 0; i < VE; ++i) dk[w][i] = dv[w][i] = 0.f;
   for (int h = hk * a.group; h < (hk + 1) * a.group; ++h) {
     const float slope = a.slopes ? __ldg(a.slopes + h) : 0.f;
-    for (int64_t b = p; b < pe; b += G * U) {
+    for (int32_t b = p; b < pe; b += G * U) {
       typename H::Raw q[U][VPL], dout[U][VPL];
-      int64_t c[U];
+      int32_t c[U];
       float lse2[U], delta[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t at = b + u * G + g;
+        const int32_t at = b + u * G + g;
         c[u] = at < pe ? d.col(at) : 0;
         H::fetch(a.q, c[u], h, lane, a.dim, at < pe, q[u]);
         H::fetch(a.dout, c[u], h, lane, a.dim, at < pe, dout[u]);
-        lse2[u] = at < pe ? a.lse[c[u] * a.heads + h] * kLog2e : -INFINITY;
-        delta[u] = at < pe ? a.delta[c[u] * a.heads + h] : 0.f;
+        lse2[u] = at < pe ? a.lse[(int64_t)c[u] * a.heads + h] * kLog2e : -INFINITY;
+        delta[u] = at < pe ? a.delta[(int64_t)c[u] * a.heads + h] : 0.f;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
