@@ -7,7 +7,8 @@
 // are bound by how fast rows come out of L2 (or HBM, once B is larger than the 126 MB L2). What the design does about it:
 // 16-bit rows stay 16-bit until they are in registers, the epilogue adds no pass over the result, and work is cut into
 // chunks of equal entries + row ends, so that hub rows and runs of empty rows are spread evenly. A warp owns a chunk; a row
-// is read in 16-byte vectors by as many lanes as it has, several rows side by side where it has fewer than 32.
+// is read in 16-byte vectors by as many lanes as it has, several rows side by side where it has fewer than 32. Measured, R-MAT
+// 18 (7.6 M entries), N = 128, bf16: 199 us without an epilogue (9.8 TB/s gathered), 234 with bias, gelu and residual.
 #include <algorithm>
 #include <type_traits>
 
@@ -17,11 +18,7 @@
 namespace dsp {
 namespace {
 
-#ifndef ACT_T
-#define ACT_T 256
-#define ACT_G 4
-#endif
-constexpr int kThreads = 256, kWalk = ACT_T;  // kWalk: threads of the kernels that walk chunks
+constexpr int kThreads = 256;
 
 struct ActArgs {
   int act, N;
@@ -175,8 +172,8 @@ struct Spread {
 };
 
 // A warp's chunk in shared memory: its entries (column, value) and row pointers. One coalesced read per list brings them in, so
-// that a step waits for rows of B only, not for ids first (with ids read step by step the kernel spent 42 % of its time on
-// that chain: 352 us instead of the figure below).
+// that a step waits for rows of B only, not for ids first (ids read step by step: 352 us instead of 275 on R-MAT 18, bf16,
+// N = 128).
 struct ChunkLists {
   int2 entry[kMaxUnits];
   int32_t ptr[kMaxUnits / kRowUnits + 4];
@@ -202,13 +199,13 @@ __device__ __forceinline__ Chunk load_chunk(const DirView &d, int64_t chunk, Chu
 // epilogue, a cut one to its slot. The residual of the running row is requested when the row begins, so that its end does not
 // wait; rows without entries need no more than act(bias), worked out once.
 template <class T, int VE, int LPR, int VPL, int U, int MINB, bool PERM>
-__global__ void __launch_bounds__(kWalk, MINB) act_product_kernel(const DirView d, const ActArgs a) {
+__global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirView d, const ActArgs a) {
   using V = RowVec<T, VE>;
   using S = Spread<VE, LPR>;
   constexpr int G = S::G, FE = S::FE;
   using F = RowVec<T, FE>;
-  __shared__ ChunkLists lists[kWalk / 32];
-  const int64_t chunk = ((int64_t)blockIdx.x * kWalk + threadIdx.x) >> 5;
+  __shared__ ChunkLists lists[kThreads / 32];
+  const int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
   if (chunk >= d.n_chunks) return;
   ChunkLists &list = lists[threadIdx.x >> 5];
   const Chunk k = load_chunk(d, chunk, list, [&](int32_t p) { return __ldg(a.values + (PERM ? __ldg(d.perm + p) : p)); });
@@ -428,7 +425,7 @@ __device__ __forceinline__ float group_sums(float (&s)[U], int lane, uint32_t ma
 // product with A transposed, whose sums over many rows are rounded to T anyway), dvalues, and the block's share of dbias. The
 // walk is the product kernel's; dout and z of the next row are requested when a row begins.
 template <class T, int VE, int LPR, int VPL, int U, int MINB>
-__global__ void __launch_bounds__(kWalk, MINB) act_grad_rows_kernel(const DirView d, const GradArgs a) {
+__global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const DirView d, const GradArgs a) {
   using V = RowVec<T, VE>;
   using S = Spread<VE, LPR>;
   constexpr int G = S::G, FE = S::FE;
@@ -436,8 +433,8 @@ __global__ void __launch_bounds__(kWalk, MINB) act_grad_rows_kernel(const DirVie
   static_assert(LPR >= U, "a group holds a step's sums");
   constexpr int cols = LPR * VE * VPL;
   __shared__ union {
-    ChunkLists lists[kWalk / 32];
-    float sums[kWalk / 32][cols];
+    ChunkLists lists[kThreads / 32];
+    float sums[kThreads / 32][cols];
   } sm;
   ChunkLists &list = sm.lists[threadIdx.x >> 5];
   const int lane = threadIdx.x % LPR, g = S::part();
@@ -453,9 +450,9 @@ __global__ void __launch_bounds__(kWalk, MINB) act_grad_rows_kernel(const DirVie
   for (int w = 0; w < VPL; ++w)
 #pragma unroll
     for (int i = 0; i < FE; ++i) bsum[w][i] = z[w][i] = 0.f;
-  const int64_t warps = (int64_t)gridDim.x * (kWalk / 32);
+  const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
 #pragma unroll 1
-  for (int64_t chunk = ((int64_t)blockIdx.x * kWalk + threadIdx.x) >> 5; chunk < d.n_chunks; chunk += warps) {
+  for (int64_t chunk = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5; chunk < d.n_chunks; chunk += warps) {
     const Chunk k = load_chunk(d, chunk, list, [](int32_t) { return 0.f; });
     const int2 *entry = list.entry - k.p0;
     auto request = [&](int32_t row) {  // dout and z of a row
@@ -529,12 +526,12 @@ __global__ void __launch_bounds__(kWalk, MINB) act_grad_rows_kernel(const DirVie
 #pragma unroll
     for (int i = 0; i < FE; ++i) sm.sums[threadIdx.x >> 5][w * LPR * VE + lane * VE + g * FE + i] = bsum[w][i];
   __syncthreads();
-  for (int c = threadIdx.x; c < cols; c += kWalk) {
+  for (int c = threadIdx.x; c < cols; c += kThreads) {
     const int col = blockIdx.y * cols + c;
     if (col >= a.N) continue;
     float s = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWalk / 32; ++w) s += sm.sums[w][c];
+    for (int w = 0; w < kThreads / 32; ++w) s += sm.sums[w][c];
     a.dbias[(int64_t)blockIdx.x * a.N + col] = s;
   }
 }
@@ -585,25 +582,22 @@ Shape shape_of(int N, int ve, int size) {
   return {ve, lpr, lpr == 32 && N > 32 * ve ? 2 : 1};
 }
 
-#ifndef ACT_U
-#define ACT_U 4
-#define ACT_B 4
-#define GR_U 4
-#define GR_B 4
-#endif
+// Entries a step and blocks an SM: 4 and 4 measured best (R-MAT 18 forward / R-MAT 16 fp32 training / R-MAT 18 training, us: 4, 4:
+// 275 / 296 / 830; 4, 3: 276 / 377 / 895; 8, 3: 326 / 388 / 1007; 4, 5: 328 / 330 / 1044, spilling).
+constexpr int kSteps = 4, kBlocks = 4;
 template <class T, int VE, int LPR, int VPL, bool PERM>
 void run_product(const DirView &d, const ActArgs &a, cudaStream_t s) {
-  constexpr int U = VE * VPL >= 16 ? 4 : VE == 4 && VPL == 2 ? 4 : ACT_U, minb = VE * VPL >= 16 ? 2 : ACT_B;
-  const dim3 grid((unsigned)((d.n_chunks + kWalk / 32 - 1) / (kWalk / 32)),
+  constexpr int U = kSteps, minb = VE * VPL >= 16 ? 2 : kBlocks;  // two vectors a lane take the registers of four blocks
+  const dim3 grid((unsigned)((d.n_chunks + kThreads / 32 - 1) / (kThreads / 32)),
                   (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL)));
-  act_product_kernel<T, VE, LPR, VPL, U, minb * 256 / kWalk, PERM><<<grid, kWalk, 0, s>>>(d, a);
+  act_product_kernel<T, VE, LPR, VPL, U, minb, PERM><<<grid, kThreads, 0, s>>>(d, a);
 }
 
 template <class T, int VE, int LPR, int VPL>
 void run_rows(const DirView &d, const GradArgs &a, int blocks, cudaStream_t s) {
-  constexpr int U = GR_U < LPR ? GR_U : 4, minb = VE * VPL >= 16 ? 2 : GR_B;
-  act_grad_rows_kernel<T, VE, LPR, VPL, U, minb * 256 / kWalk>
-      <<<dim3((unsigned)blocks, (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL))), kWalk, 0, s>>>(d, a);
+  constexpr int U = kSteps, minb = VE * VPL >= 16 ? 2 : kBlocks;
+  act_grad_rows_kernel<T, VE, LPR, VPL, U, minb>
+      <<<dim3((unsigned)blocks, (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL))), kThreads, 0, s>>>(d, a);
 }
 
 // f.template operator()<VE, LPR, VPL>() of a shape.
@@ -716,7 +710,7 @@ GradPlan grad_plan(const dsp_pattern *p, const dsp_act_grad_desc *d) {
   g.shape = shape_of(d->N, al.ve, esize(d->dtype));
   g.col_blocks = (d->N + g.shape.cols() - 1) / g.shape.cols();
   g.blocks = (int)std::max<int64_t>(
-      1, std::min<int64_t>((int64_t)ACT_G * 256 / kWalk * p->sms, (p->a.n_chunks + kWalk / 32 - 1) / (kWalk / 32)));
+      1, std::min<int64_t>((int64_t)kBlocks * p->sms, (p->a.n_chunks + kThreads / 32 - 1) / (kThreads / 32)));
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
