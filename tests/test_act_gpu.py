@@ -364,3 +364,20 @@ def test_refusals(gpu):
     g = dsp_act_grad_desc(0, 0, 64, p.values.data_ptr(), B.data_ptr(), 64, None, 0, dy.data_ptr(), 64, B.data_ptr(), 64, None, None)
     assert d.lib().dsp_spmm_act_grad(p._h, ctypes.byref(g), None, 0, None) == -8
     assert torch.cuda.current_device() == 0
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_offsets_past_32_bits(gpu, t):
+    """Rows of B and gradients behind 2^32 bytes (untouched rows in between are never read)."""
+    n, cols = 256, (1 << 32) // 256 // (4 if t == F32 else 2) + 5000
+    a = csr_of([[0, 7, cols - 1], [cols - 2], []], cols, [1.0, 2.0, 3.0, 4.0])
+    p = d.SparsePattern(a)
+    B = torch.empty(cols, n, dtype=t, device="cuda")
+    used = {c: torch.randint(-4, 5, (n,)).float() for c in (0, 7, cols - 2, cols - 1)}
+    for c, x in used.items():
+        B[c] = x.to(t).cuda()
+    out = d.spmm_act(p, B).cpu().float()
+    assert torch.equal(out[0], used[0] + 2 * used[7] + 3 * used[cols - 1])
+    assert torch.equal(out[1], 4 * used[cols - 2]) and (out[2] == 0).all()
+    dv = d.spmm_act_backward(p, torch.ones(3, n, dtype=t, device="cuda"), B, None, need_B=False)[1].cpu()
+    assert torch.equal(dv, torch.stack([used[0], used[7], used[cols - 1], used[cols - 2]]).sum(1))

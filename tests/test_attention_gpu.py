@@ -544,3 +544,41 @@ def test_a_graph_transformer_layer(gpu):
     # are larger than the result by cancellation; held to 1e-4 of each result's largest value
     for x, z in zip((y,) + got, (y64.detach(),) + want):
         assert (x.detach().cpu().double() - z).abs().max() <= 1e-4 * z.abs().max()
+
+
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_decode_offsets_past_32_bits(gpu, t):
+    """A cache whose last rows lie behind 2^32 bytes: the same tokens at its front and at its end give the same result."""
+    dim, kv = 128, 4
+    keys = (1 << 32) // (dim * kv * (4 if t == F32 else 2)) + 3000
+    k, v = (torch.empty(keys, kv, dim, dtype=t, device="cuda") for _ in range(2))
+    q, ks, vs, _ = (x.cuda() for x in inputs(2, 200, 8, kv, dim, t, 3))
+    for cache, x in ((k, ks), (v, vs)):
+        cache[:200] = x
+        cache[-200:] = x
+    idx = torch.cat([torch.arange(200), torch.arange(keys - 200, keys)]).cuda()
+    both = torch.cat([q[:1], q[:1]])
+    out = d.sparse_attention_decode(both, k, v, torch.tensor([0, 200, 400], device="cuda"), idx)
+    want = d.sparse_attention_decode(q[:1], ks, vs, torch.tensor([0, 200], device="cuda"), torch.arange(200, device="cuda"))
+    # chunk borders fall elsewhere: sums in another order
+    torch.testing.assert_close(out, torch.cat([want, want]), rtol=0, atol=2 ** -8 if t == BF16 else 1e-6)
+
+
+def test_tiles_of_rows_past_32_bits(gpu):
+    """q, k and v as strided rows that reach past 2^32 bytes, by tiles and by rows."""
+    n, stride = 300, (1 << 32) // 2 // 256
+    base = torch.empty(n * stride + 8192, dtype=BF16, device="cuda")
+    a = positional("window", n, window=90)
+    q, k, v, dout = (x.cuda() for x in inputs(n, n, 2, 2, 64, BF16, 5))
+    far = []
+    for i, x in enumerate((q, k, v)):
+        w = base.as_strided((n, 2, 64), (stride, 64, 1), i * 1024)
+        w.copy_(x)
+        far.append(w)
+    for form in FORMS:
+        p = d.SparsePattern(a, grad=True, attention=True, form=form)
+        near_out = d.sparse_attention_forward(p, q, k, v)
+        far_out = d.sparse_attention_forward(p, *far)
+        for x, y in zip(near_out + d.sparse_attention_backward(p, dout, q, k, v, *near_out),
+                        far_out + d.sparse_attention_backward(p, dout, *far, *far_out)):
+            assert torch.equal(x, y)
