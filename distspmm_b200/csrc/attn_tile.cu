@@ -4,7 +4,7 @@
 // lists), with products of 128 x 64 x dim and 128 x dim x 64 per tile:
 //
 //             stationary   stream    first products            weights (16-bit, in tensor memory)   second products
-//   forward   Q            K, V      S = Q K^T                 P = exp(u - m)                       O += P V
+//   forward   Q            K, V      S = Q K^T                 P = exp(u - m), in two parts         O += P V
 //   dq        Q, dO        K, V      S = Q K^T, R = dO V^T     dS = P (R - delta) c                 dQ += dS K
 //   dk, dv    K, V         Q, dO     S^T = K Q^T, R^T = V dO^T P^T, dS^T                            dV += P^T dO, dK += dS^T Q
 //
@@ -16,20 +16,23 @@
 // the result the same (weights and their sum share the stale maximum). It takes the tiles from the last to the first: under a
 // causal mask with a distance bias scores fall along that way, and the maximum stands after one tile.
 //
-// Rounding: weights enter the second product in the operands' 16-bit type (half a step each; the sum l is of unrounded
-// weights), the score gradients as hi + lo (delta comes from a rounded out; both errors together would be 1.5 times the
-// result's own rounding). fp16 has few exponents: weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is
-// scaled by a power of two that brings the largest |dout| near 16; both come off in the epilogue.
+// Rounding: in the forward pass weights enter the second product as hi + lo, two parts of the operands' 16-bit type (2^-16 of a
+// weight is lost at most; one part alone put a second rounding of the result's size into it, at 218 instead of 257 us in the window case
+// below). dk, dv: weights in the 16-bit type (half a step each; the sum l is of unrounded weights). The score gradients enter as hi +
+// lo (delta comes from a rounded out; both errors together would be 1.5 times the result's own rounding). fp16 has few exponents:
+// weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is scaled by a power of two that brings the
+// largest |dout| near 16; both come off in the epilogue.
 //
 // Masks and values that are not finite: an entry that is not listed has weight 0, but 0 x NaN in the product is NaN. So a row
 // whose result is not finite is computed again by attn_row.cuh's gather, which reads listed entries only. A NaN that belongs
 // there stays, one that leaked in does not.
 //
-// Bounds: on the tensor cores a tile of dim 128 takes 256 cycles for each product, the first 384 since 128 x 64 x 16 steps read
-// shared memory 1.5 times as fast as it delivers; its exponentials take 512 on the special function units, and the weights'
-// warps some 1000 with their waits. Two CTAs on an SM (tensor memory and registers allow no third) overlap one's weights with
-// the other's products. Measured: 8192 rows, window 1024 with 64 first keys, 32 query heads over 8 of 128, distance bias:
-// 218 us, 627 TFLOP/s of listed entries; documents, 6001 rows, 16 heads of 64, cap: 65 us forward, 100 dq, 115 dk and dv.
+// Bounds: on the tensor cores a tile of dim 128 takes 256 cycles for each product (the forward's second: twice, for two parts), the
+// first 384 since 128 x 64 x 16 steps read shared memory 1.5 times as fast as it delivers; its exponentials take 512 on the special
+// function units. The forward takes some 1900 cycles a tile and SM: neither of the two bounds it, but the chain of waits from scores
+// to weights to products, which two CTAs on an SM (tensor memory and registers allow no third) overlap only in part. Measured: 8192
+// rows, window 1024 with 64 first keys, 32 query heads over 8 of 128, distance bias: 257 us, 531 TFLOP/s of listed entries; documents,
+// 6001 rows, 16 heads of 64, cap: 68 us forward, 100 dq, 115 dk and dv.
 #include <algorithm>
 #include <type_traits>
 
@@ -368,8 +371,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         // 16 streamed rows each: 8 columns of weights, 2048 bytes of the stream's image
         if (M == kFwd) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_ts(tm_acc0, tm_s + b * 64 + k * 8, desc_mn_major(x1 + k * 2048, 8192), id_second, it > 0 || k > 0);
+          for (int k = 0; k < 4; ++k) {  // high parts in the first 32 columns, low parts in the others
+            const uint64_t v = desc_mn_major(x1 + k * 2048, 8192);
+            mma_ts(tm_acc0, tm_s + b * 64 + k * 8, v, id_second, it > 0 || k > 0);
+            mma_ts(tm_acc0, tm_s + b * 64 + 32 + k * 8, v, id_second, true);
+          }
         } else {
           // each half of a score tile (32 columns) holds: of S the weights (dk, dv) and the low parts, of R the high parts
           const uint32_t grads = M == kDq ? tm_acc0 : tm_acc1;
@@ -489,18 +495,22 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         }
         const float base = m == -INFINITY ? 0.f : -m;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        uint32_t w[32];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          float p0, p1;
-          fma2(p0, p1, u[2 * c], u[2 * c + 1], fu, fu, base, base);
-          p0 = exp2_approx(p0), p1 = exp2_approx(p1);
-          const int k = 2 * (c & 1);
-          add2(sum[k], sum[k + 1], sum[k], sum[k + 1], p0, p1);
-          w[c] = pack2<T>(p0, p1);
+        for (int half = 0; half < 2; ++half) {
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int c = 0; c < 16; ++c) {
+            const int at = half * 32 + 2 * c, k = 2 * (c & 1);
+            float p0, p1;
+            fma2(p0, p1, u[at], u[at + 1], fu, fu, base, base);
+            p0 = exp2_approx(p0), p1 = exp2_approx(p1);
+            add2(sum[k], sum[k + 1], sum[k], sum[k + 1], p0, p1);
+            split2<T>(p0, p1, hi[c], lo[c]);
+          }
+          tmem_st16(tm_s + lanes + b * 64 + half * 16, hi);
+          tmem_st16(tm_s + lanes + b * 64 + 32 + half * 16, lo);
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        tmem_st32(tm_s + lanes + b * 64, w);
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(bar_weights + 8 * b);

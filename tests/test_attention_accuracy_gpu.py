@@ -1,0 +1,62 @@
+"""What 16-bit attention keeps of fp32: weights and score gradients in two parts, gradients of any size in fp16, caps of any size,
+infinite values (bounds: derived in attention_bounds.bounds)."""
+import math
+
+import pytest
+import torch
+
+import distspmm_b200 as d
+from attention_bounds import bounds
+from sparse_reference import attention64, csr_of, mask_of, matrix, positional
+from test_attention_gpu import FORMS, inputs, lists, near, slopes_of
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def check(form, a, q, k, v, dout, cap=0.0, scale=None, slopes=None, names=("out", "lse", "dq", "dk", "dv"), depth=None):
+    t, dim = q.dtype, q.shape[2]
+    p = d.SparsePattern(a, grad=True, attention=True, form=form)
+    opt = dict(scale=scale, softcap=cap, slopes=None if slopes is None else slopes.cuda())
+    qc, kc, vc, dc = (x.cuda() for x in (q, k, v, dout))
+    out, lse = d.sparse_attention_forward(p, qc, kc, vc, **opt)
+    got = dict(out=out, lse=lse)
+    got.update(zip(("dq", "dk", "dv"), d.sparse_attention_backward(p, dc, qc, kc, vc, out, lse, **opt)))
+    w = [x.double().requires_grad_() for x in (q, k, v)]
+    s = dim ** -0.5 if scale is None else scale
+    mask = mask_of(a)
+    o, l, pr = attention64(mask, *w, s, cap, slopes)
+    grads = torch.autograd.grad(o, w, dout.double())
+    want = dict(out=o.detach(), lse=l.detach(), **dict(zip(("dq", "dk", "dv"), grads)))
+    tol = bounds(mask, *(x.detach() for x in (*w, o, l, pr)), t, s, cap, slopes, dout=dout.double(), grads=grads, depth=depth, once=form == "tiles")
+    for name in names:
+        near(got[name], want[name], tol[name], name)
+    p.check_error()
+
+
+MASKS = {"window": lambda: positional("window", 300, window=120, first=3), "docs": lambda: positional("docs", 260, cuts=[0, 90, 91, 250]),
+         "rmat": lambda: d.gen_rmat(8, seed=3)}
+
+
+def forms(dim):
+    return FORMS if dim in (64, 128) else FORMS[1:]
+
+
+@pytest.mark.parametrize("what", [("out", "lse")])
+@pytest.mark.parametrize("cap,scale", [(0.0, None), (8.0, None), (0.0, 1.0)])
+@pytest.mark.parametrize("heads,kv,dim,t", [(2, 1, 64, BF16), (4, 2, 128, BF16), (2, 2, 64, F16), (2, 1, 128, F16), (2, 1, 32, BF16)])
+@pytest.mark.parametrize("mask", list(MASKS))
+@pytest.mark.parametrize("form", FORMS)
+def test_weights_keep_16_bits(gpu, form, mask, heads, kv, dim, t, cap, scale, what):
+    """A scale of 1 saturates the softmax: score gradients are small differences then."""
+    if form not in forms(dim):
+        pytest.skip("dims 64 and 128 have tiles")
+    a = MASKS[mask]()
+    check(form, a, *inputs(a.num_rows, a.num_cols, heads, kv, dim, t, 5), cap=cap, scale=scale, names=what)
+
+
+def rows_of_sizes():
+    """Rows of 1, 2 and 100 entries, one cut across chunks, rows without any."""
+    rows = [[i] for i in range(20)] + [[i, i + 30] for i in range(20)] + [list(range(i, i + 100)) for i in range(20)] + [[]] * 3
+    rows[25] = list(range(0, 1100))
+    return csr_of(rows, 1100)
