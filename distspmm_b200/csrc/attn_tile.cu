@@ -4,9 +4,10 @@
 // lists), with products of 128 x 64 x dim and 128 x dim x 64 per tile:
 //
 //             stationary   stream    first products            weights (16-bit, in tensor memory)   second products
-//   forward   Q            K, V      S = Q K^T                 P = exp(u - m), in two parts         O += P V
+//   forward   Q            K, V      S = Q K^T                 P = exp(u - m)                       O += P V
 //   dq        Q, dO        K, V      S = Q K^T, R = dO V^T     dS = P (R - delta) c                 dQ += dS K
 //   dk, dv    K, V         Q, dO     S^T = K Q^T, R^T = V dO^T P^T, dS^T                            dV += P^T dO, dK += dS^T Q
+// All weights are in two parts.
 //
 // A CTA: four warps of weights (a thread owns one of the 128 rows: the running maximum, sum and all masks are its own
 // registers, no shuffles), one warp of TMA loads, one that issues the products. Scores arrive in tensor memory, weights go
@@ -16,10 +17,9 @@
 // the result the same (weights and their sum share the stale maximum). It takes the tiles from the last to the first: under a
 // causal mask with a distance bias scores fall along that way, and the maximum stands after one tile.
 //
-// Rounding: in the forward pass weights enter the second product as hi + lo, two parts of the operands' 16-bit type (2^-16 of a
-// weight is lost at most; one part alone put a second rounding of the result's size into it, at 218 instead of 257 us in the window case
-// below). dk, dv: weights in the 16-bit type (half a step each; the sum l is of unrounded weights). The score gradients enter as hi +
-// lo (delta comes from a rounded out; both errors together would be 1.5 times the result's own rounding). fp16 has few exponents:
+// Rounding: weights enter the second products as hi + lo, two parts of the operands' 16-bit type, and so do the score gradients (2^-16
+// of a value is lost at most). One part alone put a second rounding of the result's size into out and dv (window case below: 218
+// instead of 257 us forward; documents: 115 instead of 126 us dk and dv). delta comes from a rounded out. fp16 has few exponents:
 // weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is scaled by a power of two that brings the
 // largest |dout| near 16; both come off in the epilogue.
 //
@@ -32,7 +32,7 @@
 // function units. The forward takes some 1900 cycles a tile and SM: neither of the two bounds it, but the chain of waits from scores
 // to weights to products, which two CTAs on an SM (tensor memory and registers allow no third) overlap only in part. Measured: 8192
 // rows, window 1024 with 64 first keys, 32 query heads over 8 of 128, distance bias: 257 us, 531 TFLOP/s of listed entries; documents,
-// 6001 rows, 16 heads of 64, cap: 68 us forward, 100 dq, 115 dk and dv.
+// 6001 rows, 16 heads of 64, cap: 67 us forward, 96 dq, 126 dk and dv.
 #include <algorithm>
 #include <type_traits>
 
@@ -377,13 +377,18 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             mma_ts(tm_acc0, tm_s + b * 64 + 32 + k * 8, v, id_second, true);
           }
         } else {
-          // each half of a score tile (32 columns) holds: of S the weights (dk, dv) and the low parts, of R the high parts
+          // each half of a score tile (32 columns) holds: of S the weights (dk, dv) and the score gradients' low parts, of R the score
+          // gradients and the weights' low parts (dk, dv)
           const uint32_t grads = M == kDq ? tm_acc0 : tm_acc1;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t at = b * 64 + (k / 2) * 32 + (k % 2) * 8;
             const uint64_t d0 = desc_mn_major(x0 + k * 2048, 8192);
-            if (M == kDkv) mma_ts(tm_acc0, tm_s + at, desc_mn_major(x1 + k * 2048, 8192), id_second, it > 0 || k > 0);
+            if (M == kDkv) {
+              const uint64_t d1 = desc_mn_major(x1 + k * 2048, 8192);
+              mma_ts(tm_acc0, tm_s + at, d1, id_second, it > 0 || k > 0);
+              mma_ts(tm_acc0, tm_r + at + 16, d1, id_second, true);
+            }
             mma_ts(grads, tm_r + at, d0, id_second, it > 0 || k > 0);
             mma_ts(grads, tm_s + at + 16, d0, id_second, true);
           }
@@ -634,10 +639,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             for (int c = 0; c < 32; ++c) p[c] = bit & (1u << c) ? p[c] : 0.f;
           }
           if (M == kDkv) {
-            uint32_t w[16];
+            uint32_t w[16], lo[16];
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) w[c / 2] = pack2<T>(p[c], p[c + 1]);
+            for (int c = 0; c < 32; c += 2) split2<T>(p[c], p[c + 1], w[c / 2], lo[c / 2]);
             tmem_st16(tm_s + lanes + b * 64 + half * 32, w);
+            tmem_st16(tm_r + lanes + b * 64 + half * 32 + 16, lo);
           }
           // score gradients: p (dp - delta) (1 - tanh^2), up to the scale
 #pragma unroll

@@ -42,7 +42,7 @@ def forms(dim):
     return FORMS if dim in (64, 128) else FORMS[1:]
 
 
-@pytest.mark.parametrize("what", [("out", "lse")])
+@pytest.mark.parametrize("what", [("out", "lse"), ("dv",)])
 @pytest.mark.parametrize("cap,scale", [(0.0, None), (8.0, None), (0.0, 1.0)])
 @pytest.mark.parametrize("heads,kv,dim,t", [(2, 1, 64, BF16), (4, 2, 128, BF16), (2, 2, 64, F16), (2, 1, 128, F16), (2, 1, 32, BF16)])
 @pytest.mark.parametrize("mask", list(MASKS))
