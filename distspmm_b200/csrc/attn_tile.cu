@@ -5,9 +5,9 @@
 //
 //             stationary   stream    first products            weights (16-bit, in tensor memory)   second products
 //   forward   Q            K, V      S = Q K^T                 P = exp(u - m)                       O += P V
-//   dq        Q, dO        K, V      S = Q K^T, R = dO V^T     dS = P (R - delta) c                 dQ += dS K
+//   dq        Q, dO        K, V      S = Q K^T, R = dO V^T     dS = P (R - delta0) c, P c           dQ += dS K, Y += P c K
 //   dk, dv    K, V         Q, dO     S^T = K Q^T, R^T = V dO^T P^T, dS^T                            dV += P^T dO, dK += dS^T Q
-// All weights are in two parts.
+// All weights but P c are in two parts.
 //
 // A CTA: four warps of weights (a thread owns one of the 128 rows: the running maximum, sum and all masks are its own
 // registers, no shuffles), one warp of TMA loads, one that issues the products. Scores arrive in tensor memory, weights go
@@ -19,7 +19,9 @@
 //
 // Rounding: weights enter the second products as hi + lo, two parts of the operands' 16-bit type, and so do the score gradients (2^-16
 // of a value is lost at most). One part alone put a second rounding of the result's size into out and dv (window case below: 218
-// instead of 257 us forward; documents: 115 instead of 126 us dk and dv). delta comes from a rounded out. fp16 has few exponents:
+// instead of 257 us forward; documents: 115 instead of 126 us dk and dv). The first delta0 = dout . out has a rounded
+// out; so dq = sum p c (dp - delta0) k - g sum p c k with g = sum p (dp - delta0) = delta - delta0, whose weights p c may be rounded once, as g is
+// but a rounding itself; delta0 + g is what dk takes. fp16 has few exponents:
 // weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is scaled by a power of two that brings the
 // largest |dout| near 16; both come off in the epilogue.
 //
@@ -32,7 +34,7 @@
 // function units. The forward takes some 1900 cycles a tile and SM: neither of the two bounds it, but the chain of waits from scores
 // to weights to products, which two CTAs on an SM (tensor memory and registers allow no third) overlap only in part. Measured: 8192
 // rows, window 1024 with 64 first keys, 32 query heads over 8 of 128, distance bias: 257 us, 531 TFLOP/s of listed entries; documents,
-// 6001 rows, 16 heads of 64, cap: 67 us forward, 96 dq, 126 dk and dv.
+// 6001 rows, 16 heads of 64, cap: 67 us forward, 106 dq, 126 dk and dv.
 #include <algorithm>
 #include <type_traits>
 
@@ -70,7 +72,7 @@ struct Cfg {
   static constexpr int NB = M == kFwd || D == 128 ? 2 : 1;  // score buffers
   static constexpr int ST = 2;                                 // stages of each streamed operand
   static constexpr int kAcc = kScores * NB * 64;               // first accumulator column
-  static constexpr int kUsed = kAcc + (M == kDkv ? 2 : 1) * D;
+  static constexpr int kUsed = kAcc + (M == kFwd ? 1 : 2) * D;
   static constexpr int kCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static constexpr int kStaticBytes = 128 * D * 2, kStreamBytes = 64 * D * 2;
   static constexpr int kSmemUsed = kStatic * kStaticBytes + 2 * ST * kStreamBytes + 1024;
@@ -215,6 +217,7 @@ __device__ __noinline__ void redo(const TileArgs &x, int64_t row0, int head, uin
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[0][i] = (y[0][i] - m * z[0][i]) * x.a.scale;
       if (g == 0) H::store(x.a.dq, row, head, lane, D, y);
+      if ((threadIdx.x & 31) == 0) x.a.delta[row * x.a.heads + head] = m;
     } else {
       attend_dkv<H, D / 8>(x.rows, x.a, row, head, p, pe, y, z);
       if (g == 0) {
@@ -225,23 +228,31 @@ __device__ __noinline__ void redo(const TileArgs &x, int64_t row0, int head, uin
   }
 }
 
-// D columns of this thread's row at `addr`, times f, to the row's place in global memory; whether all were finite.
-template <class T, int D>
-__device__ __forceinline__ bool put_acc(uint32_t addr, float f, const HeadsOut &o, int64_t row, int head, bool store) {
+// D columns of this thread's row at `addr`, times f (TWO: plus those at `addr2` times f2), to the row's place in global memory; whether
+// all were finite.
+template <class T, int D, bool TWO = false>
+__device__ __forceinline__ bool put_acc(uint32_t addr, float f, const HeadsOut &o, int64_t row, int head, bool store, uint32_t addr2 = 0,
+                                        float f2 = 0.f) {
   bool fine = true;
   T *dst = (T *)o.p + row * o.row + (int64_t)head * o.head;
 #pragma unroll 1
   for (int c = 0; c < D; c += 32) {
-    uint32_t r[32];
+    uint32_t r[32], r2[TWO ? 32 : 1];
     tmem_ld32(addr + c, r);
+    if constexpr (TWO) tmem_ld32(addr2 + c, r2);
     tmem_wait_ld();
+    auto value = [&](int i) {
+      const float x = __uint_as_float(r[i]) * f;
+      if constexpr (TWO) return fmaf(__uint_as_float(r2[i]), f2, x);
+      else return x;
+    };
 #pragma unroll
     for (int i = 0; i < 32; i += 8) {
       uint4 w;
       uint32_t *w4 = &w.x;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float lo = __uint_as_float(r[i + 2 * j]) * f, hi = __uint_as_float(r[i + 2 * j + 1]) * f;
+        const float lo = value(i + 2 * j), hi = value(i + 2 * j + 1);
         fine &= isfinite(lo) && isfinite(hi);
         w4[j] = pack2<T>(lo, hi);
       }
@@ -377,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             mma_ts(tm_acc0, tm_s + b * 64 + 32 + k * 8, v, id_second, true);
           }
         } else {
-          // each half of a score tile (32 columns) holds: of S the weights (dk, dv) and the score gradients' low parts, of R the score
+          // each half of a score tile (32 columns) holds: of S the weights (dq: p c) and the score gradients' low parts, of R the score
           // gradients and the weights' low parts (dk, dv)
           const uint32_t grads = M == kDq ? tm_acc0 : tm_acc1;
 #pragma unroll
@@ -388,6 +399,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
               const uint64_t d1 = desc_mn_major(x1 + k * 2048, 8192);
               mma_ts(tm_acc0, tm_s + at, d1, id_second, it > 0 || k > 0);
               mma_ts(tm_acc0, tm_r + at + 16, d1, id_second, true);
+            } else {
+              mma_ts(tm_acc1, tm_s + at, d0, id_second, it > 0 || k > 0);
             }
             mma_ts(grads, tm_r + at, d0, id_second, it > 0 || k > 0);
             mma_ts(grads, tm_s + at + 16, d0, id_second, true);
@@ -556,7 +569,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
       if (M == kDkv && !kBf16) up *= 0x1p-12f;  // the weights of dk, dv are 2^12 up themselves
       constexpr float kUp = kBf16 ? 0.f : 12.f;
       const bool live = row < n_rows;
-      float lse2 = INFINITY, delta = 0.f;
+      float lse2 = INFINITY, delta = 0.f, gap[2] = {0.f, 0.f};  // gap: sum of p (dp - delta), times up
       if (M == kDq && live) {
         lse2 = x.a.lse[row * x.a.heads + head] * kLog2e;
         if (lse2 == -INFINITY) lse2 = INFINITY;  // a row without entries: weights of 0
@@ -656,6 +669,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             add2(e[c], e[c + 1], e[c], e[c + 1], d0, d1);
             if (!kBf16) mul2(e[c], e[c + 1], e[c], e[c + 1], up, up);
             mul2(e[c], e[c + 1], e[c], e[c + 1], p[c], p[c + 1]);
+            if (M == kDq) add2(gap[0], gap[1], gap[0], gap[1], e[c], e[c + 1]);
           }
           if (cap > 0.f) {
             const float inv = -1.f / (cap * cap);
@@ -665,7 +679,17 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
               mul2(y0, y1, s[c], s[c + 1], s[c], s[c + 1]);
               fma2(z0, z1, y0, y1, inv, inv, 1.f, 1.f);
               mul2(e[c], e[c + 1], e[c], e[c + 1], z0, z1);
+              if (M == kDq) mul2(p[c], p[c + 1], p[c], p[c + 1], z0, z1);
             }
+          }
+          if (M == kDq) {  // p c, for the correction of delta
+            uint32_t w[16];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              if (!kBf16) mul2(p[c], p[c + 1], p[c], p[c + 1], 4096.f, 4096.f);
+              w[c / 2] = pack2<T>(p[c], p[c + 1]);
+            }
+            tmem_st16(tm_s + lanes + b * 64 + half * 32, w);
           }
           uint32_t v[16], lo[16];
 #pragma unroll
@@ -682,7 +706,9 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
       if (ok && iters > 0) {
         bool fine;
         if constexpr (M == kDq) {
-          fine = put_acc<T, D>(tm_acc0 + lanes, down, x.a.dq, row, head, live);
+          const float g = gap[0] + gap[1];
+          fine = put_acc<T, D, true>(tm_acc0 + lanes, down, x.a.dq, row, head, live, tm_acc1 + lanes, -g * down * (kBf16 ? 1.f : 0x1p-12f));
+          if (live) x.a.delta[row * x.a.heads + head] = delta + g / up;
         } else {
           fine = put_acc<T, D>(tm_acc0 + lanes, kBf16 ? 1.f : 0x1p-12f, x.a.dv, row, head, live);
           fine = put_acc<T, D>(tm_acc1 + lanes, down, x.a.dk, row, head, live) && fine;
@@ -743,7 +769,7 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const __grid_consta
   if (__any_sync(0xffffffffu, !fine)) redo<T, D, kFwd>(x, row, h, 1u);
 }
 
-// delta_i = dout_i . out_i of each row and head, a warp each (fp16: and the largest finite |dout|).
+// delta0_i = dout_i . out_i of each row and head, a warp each (fp16: and the largest finite |dout|).
 template <class T, int D>
 __global__ void __launch_bounds__(256) attn_delta_kernel(int64_t rows, const AttnArgs a, uint32_t *dout_max) {
   const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
