@@ -204,6 +204,7 @@ template <class T, int D, Mode M>
 __device__ __noinline__ void redo(const TileArgs &x, int64_t row0, int head, uint32_t bad) {
   using H = HeadRow<T, 8, D / 8, 1>;
   const int lane = threadIdx.x % (D / 8), g = (threadIdx.x & 31) / (D / 8);
+  __syncwarp();  // the rows' first results were written by other lanes than will write them now
   while (bad) {
     const int64_t row = row0 + __ffs(bad) - 1;
     bad &= bad - 1;
