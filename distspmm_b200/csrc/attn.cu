@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kThreads, VPL == 1 ? 3 : 2) attn_dq_kernel(con
         H::store_f32(a.slots + slot * 2 * a.dim, lane, a.dim, x);
         H::store_f32(a.slots + slot * 2 * a.dim + a.dim, lane, a.dim, y);
       }
-      if ((threadIdx.x & 31) == 0) a.slot_ml[slot] = delta;
+      if ((threadIdx.x & 31) == 0) a.slot_ml[2 * slot] = delta, a.slot_ml[2 * slot + 1] = 0.f;
     } else {
 #pragma unroll
       for (int w = 0; w < VPL; ++w)
@@ -197,8 +197,8 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const DirView d, co
   if (a.lse && lane == 0) a.lse[r.row * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
-// Partials of cut rows (gradients), 2 dim floats per slot and head, summed in a fixed order. DQ: the sums x and y of a row and
-// its delta (attend_dq); else dk and dv of a key.
+// Partials of cut rows (gradients), 2 dim floats per slot and head, summed in a fixed order. DQ: the sums x and y of a row, its
+// delta - delta0 and delta0 (attn_graph.cu; attend_dq: 0); else dk and dv of a key.
 template <class T, bool DQ>
 __global__ void __launch_bounds__(kThreads) attn_sum_kernel(const DirView d, int n_heads, const AttnArgs a) {
   __shared__ float part[8][512], part_delta[8];
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) attn_sum_kernel(const DirView d, int
   for (int64_t c = first; c <= r.c1; c += step) {
     const int64_t slot = r.slot(c) * n_heads + h;
     const float *src = a.slots + slot * 2 * a.dim + lane;
-    if (DQ) delta += a.slot_ml[slot];
+    if (DQ) delta += a.slot_ml[2 * slot];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (lane + 32 * i < a.dim) x[i] += src[32 * i], y[i] += src[a.dim + 32 * i];
@@ -234,9 +234,9 @@ __global__ void __launch_bounds__(kThreads) attn_sum_kernel(const DirView d, int
     }
   }
   if (DQ && lane == 0) {
-    const float lse = a.lse[r.row * a.heads + h];
-    if (a.stats) a.stats[r.row * a.heads + h] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, delta);
-    else a.delta[r.row * a.heads + h] = delta;
+    const float lse = a.lse[r.row * a.heads + h], whole = delta + a.slot_ml[2 * (r.slot(r.c0) * n_heads + h) + 1];
+    if (a.stats) a.stats[r.row * a.heads + h] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, whole);
+    else a.delta[r.row * a.heads + h] = whole;
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -322,7 +322,7 @@ GradPlan grad_plan(const dsp_pattern *p, const dsp_attn_desc *d) {
   const int64_t q = p->a.n_split ? 16ll * p->a.n_chunks * d->heads * d->dim : 0;
   const int64_t kv = p->t.n_split ? 16ll * p->t.n_chunks * d->kv_heads * d->dim : 0;
   g.ml = g.slots + up256(std::max(q, kv));  // dq's partials are joined before dk's and dv's are written
-  g.total = g.ml + (p->a.n_split ? up256(8ll * p->a.n_chunks * d->heads) : 0);
+  g.total = g.ml + (p->a.n_split ? up256(16ll * p->a.n_chunks * d->heads) : 0);
   return g;
 }
 

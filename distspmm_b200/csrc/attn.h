@@ -27,7 +27,7 @@ struct AttnArgs {
   float2 *stats;     // [rows][heads] lse in base 2 (+infinity: a row without entries) and delta, for attn_graph.cu's dk, dv
   const uint32_t *dout_max;  // bits of the largest finite |dout| (fp16 gradients)
   float *slots;      // partials of cut rows: [2 n_chunks][heads][width]
-  float *slot_ml;    // [2 n_chunks][heads][2] running maximum and sum (forward)
+  float *slot_ml;    // [2 n_chunks][heads][2] running maximum and sum (forward), delta - delta0 and delta0 (dq)
 };
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

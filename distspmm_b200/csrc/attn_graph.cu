@@ -3,18 +3,20 @@
 // For patterns too thin for tiles (a graph's edges). The formulas are those of attn.cu; what bounds both is the gather of a row
 // of k and one of v (q and dout, by columns) for each entry and head out of L2. Here the arithmetic is given to mma.sync, though
 // an entry has but one query for each head to be multiplied with (of m16n8k16 products, 8 columns are entries and 1 to 8 rows
-// query heads): R-MAT 15, 8 heads of 64, bf16: forward 577 -> 375 us, dq 632 -> 445,
-// dk and dv 681 -> 595 against dot products by shuffles.
+// query heads): R-MAT 15, 8 heads of 64, bf16: forward 577 -> 367 us, dq 632 -> 469,
+// dk and dv 681 -> 581 against dot products by shuffles.
 //
 //   pass      16 entries as columns   rows                         then, entries turned
 //   forward   k                       q of up to 8 heads           v   x weights
-//   dq        k, v                    q, dout of up to 4 heads,    k   x [p c dp | p c]   (x and y of attn_row.cuh)
+//   dq        k, v                    q, dout of up to 4 heads,    k   x [p c (dp - delta0) | p c]   (x and y of attn_row.cuh)
 //                                     twice
 //   dk, dv    q, dout of one head     k, v (one key, twice)        dout x p, q x p c (dp - delta): hi and lo parts in the columns
 //
 // A warp owns a chunk (pattern.h) and a head or group; its column ids and row pointers are staged in shared memory, and the walk
 // over 16-entry steps runs on across rows: the next step's rows are requested as soon as the present ones are in the products,
-// so a short row costs no wait. Weights enter the second product as hi + lo, as exact as fp32.
+// so a short row costs no wait. Weights enter the second product as hi + lo (2^-16 of a weight is lost at most). So dq takes its
+// differences dp - delta from delta0 = dout . out, within out's rounding of delta, before they are split, and the rest off after the
+// products: dq = scale (x - g y) with g = delta - delta0 = sum p (dp - delta0).
 #include <algorithm>
 #include <type_traits>
 
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
           constexpr int width = M == kForward ? D : 2 * D;
           for (int i = lane; i < width / 4; i += 32) reinterpret_cast<uint4 *>(a.slots + slot * width)[i] = zero;
           if (lane == 0 && M == kForward) a.slot_ml[2 * slot] = -INFINITY, a.slot_ml[2 * slot + 1] = 0.f;
-          if (lane == 0 && M == kDq) a.slot_ml[slot] = 0.f;
+          if (lane == 0 && M == kDq) a.slot_ml[2 * slot] = a.slot_ml[2 * slot + 1] = 0.f;
         } else {
           const HeadsOut &o = M == kForward ? a.out : a.dq;
           if (lane < D / 8) *reinterpret_cast<uint4 *>((T *)o.p + (int64_t)row * o.row + (int64_t)h * o.head + 8 * lane) = zero;
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
   int32_t row = -1;
   uint32_t pair[D / 16][4];  // q over dout (dk, dv: k over v)
   float acc[NT][4], acc2[M == kDkv ? NT : 1][4];
-  float m = -INFINITY, l = 0.f, lse2 = 0.f;  // forward: maximum, sum; dq: l is delta
+  float m = -INFINITY, l = 0.f, lse2 = 0.f, delta0 = 0.f;  // forward: maximum, sum; dq: l is delta - delta0
 
 #pragma unroll 1
   while (true) {
@@ -190,6 +192,21 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
         if constexpr (M == kDq) {
           lse2 = head < live ? __ldg(a.lse + (int64_t)row * a.heads + h0 + head) * kLog2e : 0.f;
           if (lse2 == -INFINITY) lse2 = INFINITY;
+          delta0 = 0.f;
+          if (head < live) {
+            const T *o = (const T *)a.o.p + (int64_t)row * a.o.row + (int64_t)(h0 + head) * a.o.head + t * 8;
+#pragma unroll
+            for (int i = 0; i < VR; ++i) {
+              const uint4 w = __ldg(reinterpret_cast<const uint4 *>(o + 32 * i));
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                const float2 x = unpack2<T>(word(w, c)), y = unpack2<T>(pair[2 * i + c / 2][1 + 2 * (c & 1)]);
+                delta0 = fmaf(x.x, y.x, fmaf(x.y, y.y, delta0));
+              }
+            }
+          }
+          delta0 += __shfl_xor_sync(0xffffffffu, delta0, 1);
+          delta0 += __shfl_xor_sync(0xffffffffu, delta0, 2);
         }
       }
 #pragma unroll
@@ -271,9 +288,9 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
       float v[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float w = on[j] ? exp2_approx(s[j] - lse2) : 0.f, wc = w * (1.f - th[j] * th[j]);
-        l = fmaf(w, dp[j], l);
-        v[j] = n8 < 4 ? wc * dp[j] * up : wc;
+        const float w = on[j] ? exp2_approx(s[j] - lse2) : 0.f, wc = w * (1.f - th[j] * th[j]), gap = dp[j] - delta0;
+        l = fmaf(w, gap, l);
+        v[j] = n8 < 4 ? wc * gap * up : wc;
       }
       split2<T>(v[0], v[1], parts[0][0], parts[1][0]);
       split2<T>(v[2], v[3], parts[0][1], parts[1][1]);
@@ -367,8 +384,9 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
         }
       }
       if (t == 0 && n8 < live) {
-        if (cut) a.slot_ml[slot * a.heads + h0 + n8] = l;
-        else a.stats[(int64_t)row * a.heads + h0 + n8] = make_float2(lse2, l);
+        const int64_t at = 2 * (slot * a.heads + h0 + n8);
+        if (cut) a.slot_ml[at] = l, a.slot_ml[at + 1] = delta0;
+        else a.stats[(int64_t)row * a.heads + h0 + n8] = make_float2(lse2, delta0 + l);
       }
     } else {
 #pragma unroll

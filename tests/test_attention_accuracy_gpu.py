@@ -82,3 +82,26 @@ def test_long_row_of_equal_weights(gpu, form, t):
     v = (1 + torch.randn((n, 1, 64), generator=g)).to(t)
     dout = (1 + torch.randn((2, 1, 64), generator=g)).to(t)
     check(form, a, q, k, v, dout, names=("out", "lse", "dq"), depth=540 + n // 4096 if form == "rows" else 64 + n // 16)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_one_entry_has_no_score_gradient(gpu, form, t):
+    """dp of 18 bits, exact in fp32: dp - delta is 0, and what is left of dq has fp32's size, not that of dp in two 16-bit parts."""
+    if t == F32 and form == "tiles":
+        pytest.skip("16-bit operands have tiles")
+    n = 70
+    q, k, _, _ = inputs(n, n, 2, 2, 64, t, 12)
+    v, dout = torch.zeros_like(q), torch.zeros_like(q)
+    v[..., 0], dout[..., 0] = 256, 1
+    v[..., 1], dout[..., 1] = (torch.arange(n)[:, None] % 7 + 1) / 512, 1
+    v[..., 2], dout[..., 2] = 1, 1
+    p = d.SparsePattern(csr_of([[i] for i in range(n)], n), grad=True, attention=True, form=form)
+    qc, kc, vc, dc = (x.cuda() for x in (q, k, v, dout))
+    out, lse = d.sparse_attention_forward(p, qc, kc, vc)
+    assert torch.equal(out, vc)
+    dq, dk, dv = d.sparse_attention_backward(p, dc, qc, kc, vc, out, lse)
+    # p is 1 within the exponential's 2^-21, once or twice in a product
+    zero, size = torch.zeros(q.shape, dtype=torch.float64), 258 * 64 ** -0.5 * 2.0 ** -20
+    near(dq, zero, size * k.double().abs() + 1e-37, "dq")
+    near(dk, zero, size * q.double().abs() + 1e-37, "dk")
