@@ -313,12 +313,11 @@ ForwardPlan forward_plan(int64_t n_chunks, bool cut, int heads, int dim) {
 }
 
 struct GradPlan {
-  int64_t dout_max, slots, ml, total;
+  int64_t slots, ml, total;
 };
 GradPlan grad_plan(const dsp_pattern *p, const dsp_attn_desc *d) {
   GradPlan g = {};
-  g.dout_max = up256(8 * p->rows * d->heads);  // delta, or stats, lie before it
-  g.slots = g.dout_max + 256;
+  g.slots = up256(8 * p->rows * d->heads);  // delta, or stats, lie before them
   const int64_t q = p->a.n_split ? 16ll * p->a.n_chunks * d->heads * d->dim : 0;
   const int64_t kv = p->t.n_split ? 16ll * p->t.n_chunks * d->kv_heads * d->dim : 0;
   g.ml = g.slots + up256(std::max(q, kv));  // dq's partials are joined before dk's and dv's are written
@@ -360,11 +359,6 @@ int gradients(const dsp_pattern *p, const dsp_attn_grad_desc *g, char *ws, cudaS
   const PlanRows ra = {view(p->a)}, rt = {view(p->t)};
   const bool tensor = graph_on_tensor_cores(d->dtype, d->dim);
   if (tensor) a.stats = (float2 *)ws;
-  if (tensor && d->dtype == DSP_F16) {
-    a.dout_max = (uint32_t *)(ws + f.dout_max);
-    const int rc = graph_dout_max(a.dout, p->rows, d->heads, d->dim, (uint32_t *)(ws + f.dout_max), s);
-    if (rc) return rc;
-  }
   if (tensor) graph_pass(kDq, ra.d, a, d->dtype, s);
   else launch_pass<PlanRows, T>(kDq, ra, a, ra.d.n_chunks, s);
   if (ra.d.n_split)

@@ -25,7 +25,7 @@ struct AttnArgs {
   float *lse;        // [rows][heads]
   float *delta;      // [rows][heads] dout . out
   float2 *stats;     // [rows][heads] lse in base 2 (+infinity: a row without entries) and delta, for attn_graph.cu's dk, dv
-  const uint32_t *dout_max;  // bits of the largest finite |dout| (fp16 gradients)
+  const uint32_t *dout_max;  // bits of the largest finite |dout| (fp16 gradients by tiles)
   float *slots;      // partials of cut rows: [2 n_chunks][heads][width]
   float *slot_ml;    // [2 n_chunks][heads][2] running maximum and sum (forward), delta - delta0 and delta0 (dq)
 };

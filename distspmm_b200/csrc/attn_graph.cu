@@ -39,6 +39,25 @@ struct Step {
   int32_t row, b, pe, h;
 };
 
+// fp16 has few exponents: a column of the second product's weights is carried with a power of two, the same from one step to the next
+// while the largest weight stays between 2^0 (in a row's first step that has any) and 2^15, else that which brings it to 2^10 (what the sums
+// hold is then scaled by the same). So nothing overflows, and hi + lo are within 2^-25 where the largest is 1 or more.
+__device__ __forceinline__ bool out_of_place(float top, float carry, bool fresh) {
+  const float x = top * carry;
+  return x > 32768.f || (fresh && x < 1.f && top > 0.f);
+}
+// The new carry, and what the sums are to be multiplied with.
+__device__ __forceinline__ float renew(float top, float &carry, bool fresh) {
+  const int e = (int)(__float_as_uint(top) >> 23);  // 255: not finite, and nothing will help
+  if (!out_of_place(top, carry, fresh) || e == 255) return 1.f;
+  const float now = __uint_as_float((uint32_t)min(max(127 + 10 - (e - 127), 1), 254) << 23), keep = fresh ? 1.f : now / carry;
+  carry = now;
+  return keep;
+}
+__device__ __forceinline__ float largest(const float (&x)[4]) {
+  return fmaxf(max3(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])), fabsf(x[3]));
+}
+
 template <class T, int D, AttnPass M>
 __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M == kDkv ? 3 : 4))
     attn_graph_kernel(const DirView d, const AttnArgs a, int head_tiles) {
@@ -62,13 +81,13 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
   const int32_t *cols = list.cols - p0;
   const bool head_cut = p0 > list.ptr[0];
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  // fp16: score gradients carry the factor up, weights of dk, dv 2^12; both come off at the row's end
-  const float up = kHalf && M != kForward ? dout_scale(a.dout_max) : 1.f, down = 1.f / up;
-  constexpr float kUp = kHalf && M == kDkv ? 4096.f : 1.f;
+  // fp16: what the columns of the second products carry (dq: this lane's column; dk, dv: the weights, the score gradients)
+  float carry = 1.f, carry2 = 1.f;
   const float inv_cap2 = a.cap > 0.f ? 2.f * kLog2e / a.cap : 0.f, scale2 = a.scale * kLog2e;
 
   // a lane has the scores of column n8, a query head (dk, dv: the key, in columns 0 and 1), for the entries 2 t, 2 t + 1, 2 t + 8,
   // 2 t + 9 of a step: as they enter the second product
+  bool fresh = false, fresh2 = false;  // the row's sums are still 0
   const int head = M == kForward ? n8 : M == kDq ? n8 & 3 : 0;
   const float slope2 = M != kDkv && a.slopes && head < live ? __ldg(a.slopes + h0 + head) * kLog2e : 0.f;
   auto entry = [&](int j) { return 2 * t + (j & 1) + 8 * (j >> 1); };
@@ -217,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
           if constexpr (M == kDkv) acc2[i][j] = 0.f;
         }
       m = -INFINITY, l = 0.f;
+      fresh = fresh2 = true;
     }
     const Step next = next_of(now);
     const bool more = next.row <= r1;
@@ -290,7 +310,22 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
       for (int j = 0; j < 4; ++j) {
         const float w = on[j] ? exp2_approx(s[j] - lse2) : 0.f, wc = w * (1.f - th[j] * th[j]), gap = dp[j] - delta0;
         l = fmaf(w, gap, l);
-        v[j] = n8 < 4 ? wc * gap * up : wc;
+        v[j] = n8 < 4 ? wc * gap : wc;
+      }
+      if constexpr (kHalf) {
+        float top = largest(v);
+        const uint32_t filled = __ballot_sync(0xffffffffu, top > 0.f) >> (lane & 28) & 15;  // of this lane's column
+        if (__any_sync(0xffffffffu, out_of_place(top, carry, fresh))) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const float keep = renew(top, carry, fresh);
+          const float k0 = __shfl_sync(0xffffffffu, keep, 8 * t), k1 = __shfl_sync(0xffffffffu, keep, 8 * t + 4);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) acc[i][0] *= k0, acc[i][2] *= k0, acc[i][1] *= k1, acc[i][3] *= k1;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] *= carry;
+        fresh = fresh && filled == 0;
       }
       split2<T>(v[0], v[1], parts[0][0], parts[1][0]);
       split2<T>(v[2], v[3], parts[0][1], parts[1][1]);
@@ -302,8 +337,26 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         w[j] = on[j] ? exp2_approx(s[j] - stat[j].x) : 0.f;
-        g[j] = w[j] * (dp[j] - stat[j].y) * (1.f - th[j] * th[j]) * up;
-        w[j] *= kUp;
+        g[j] = w[j] * (dp[j] - stat[j].y) * (1.f - th[j] * th[j]);
+      }
+      if constexpr (kHalf) {
+        float top = n8 == 0 ? largest(w) : 0.f, top2 = n8 == 0 ? largest(g) : 0.f;
+        const bool filled = __any_sync(0xffffffffu, top > 0.f), filled2 = __any_sync(0xffffffffu, top2 > 0.f);
+        if (__any_sync(0xffffffffu, out_of_place(top, carry, fresh) || out_of_place(top2, carry2, fresh2))) {
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            top2 = fmaxf(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+          }
+          const float keep = renew(top, carry, fresh), keep2 = renew(top2, carry2, fresh2);
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] *= keep, acc2[i][j] *= keep2;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] *= carry, g[j] *= carry2;
+        fresh = fresh && !filled, fresh2 = fresh2 && !filled2;
       }
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -363,13 +416,14 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
       for (int j = 0; j < 2; ++j) {
         const int hh = (2 * t + j) & 3, h = h0 + hh;
         const bool own = hh < live && writes;
+        const float down = kHalf ? 1.f / __shfl_sync(0xffffffffu, carry, 8 * t + 4 * j) : 1.f;
 #pragma unroll
         for (int i = 0; i < VT; ++i) {
           float f[8], g[8];
           elements(acc, i, j, f);
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
-            if (t < 2) f[c] *= down;
+            if (kHalf) f[c] *= down;
             g[c] = __shfl_xor_sync(0xffffffffu, f[c], 2);
           }
           const int col = (n8 + 8 * i) * 8;
@@ -397,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
         elements(acc, i, 0, g);
         elements(acc, i, 1, g1);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) f[c] = (f[c] + f1[c]) * (a.scale * down), g[c] = (g[c] + g1[c]) * (1.f / kUp);
+        for (int c = 0; c < 8; ++c) f[c] = (f[c] + f1[c]) * (a.scale / carry2), g[c] = (g[c] + g1[c]) * (1.f / carry);
         const int col = (n8 + 8 * i) * 8;
         if (t != 0 || !writes) continue;
         if (cut) {
@@ -414,22 +468,6 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
     if (!more) break;
     now = next;
   }
-}
-
-__global__ void __launch_bounds__(256) dout_max_kernel(Heads x, int64_t rows, int heads, int dim, uint32_t *out) {
-  const int per = dim / 8;
-  const int64_t n = rows * heads * per;
-  float top = 0.f;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    const int64_t item = i / per, row = item / heads;
-    float f[8];
-    RowVec<__half, 8>::widen(RowVec<__half, 8>::ldg((const __half *)x.p + row * x.row + (item - row * heads) * x.head + (i - item * per) * 8), f);
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-      if (isfinite(f[c])) top = fmaxf(top, fabsf(f[c]));
-  }
-  const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-  if ((threadIdx.x & 31) == 0 && bits > 0) atomicMax(out, bits);  // a maximum does not depend on the order
 }
 
 template <class T, int D>
@@ -452,14 +490,6 @@ void pick(AttnPass pass, const DirView &d, const AttnArgs &a, cudaStream_t s) {
 }  // namespace
 
 bool graph_on_tensor_cores(int dtype, int dim) { return dtype != DSP_F32 && (dim == 32 || dim == 64 || dim == 128); }
-
-int graph_dout_max(const Heads &dout, int64_t rows, int heads, int dim, uint32_t *out, cudaStream_t s) {
-  const cudaError_t e = cudaMemsetAsync(out, 0, 4, s);
-  if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_attn_grad: %s", cudaGetErrorString(e));
-  const int64_t n = rows * heads * (dim / 8);
-  if (n > 0) dout_max_kernel<<<(unsigned)std::min<int64_t>(148 * 8, (n + 255) / 256), 256, 0, s>>>(dout, rows, heads, dim, out);
-  return DSP_OK;
-}
 
 void graph_pass(AttnPass pass, const DirView &d, const AttnArgs &a, int dtype, cudaStream_t s) {
   if (d.n_chunks == 0) return;

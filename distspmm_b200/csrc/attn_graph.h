@@ -8,7 +8,5 @@ enum AttnPass { kForward, kDq, kDkv };
 bool graph_on_tensor_cores(int dtype, int dim);
 // The pass's kernel over the chunks of d (A for forward and dq, A transposed for dk, dv); cut rows are left in slots as by
 // attn.cu's kernels.
-// *out = the bits of the largest finite |dout| (fp16), for AttnArgs::dout_max.
-int graph_dout_max(const Heads &dout, int64_t rows, int heads, int dim, uint32_t *out, cudaStream_t s);
 void graph_pass(AttnPass pass, const DirView &d, const AttnArgs &a, int dtype, cudaStream_t s);
 }  // namespace dsp

@@ -49,7 +49,7 @@ def forms(dim):
 @pytest.mark.parametrize("form", FORMS)
 def test_weights_keep_16_bits(gpu, form, mask, heads, kv, dim, t, cap, scale, what):
     """A scale of 1 saturates the softmax: score gradients are small differences then."""
-    if form not in forms(dim) or (form == "rows" and t == F16):
+    if form not in forms(dim):
         pytest.skip("dims 64 and 128 have tiles")
     a = MASKS[mask]()
     check(form, a, *inputs(a.num_rows, a.num_cols, heads, kv, dim, t, 5), cap=cap, scale=scale, names=what)
@@ -67,21 +67,6 @@ def rows_of_sizes():
 def test_score_gradients_of_rows_with_few_entries(gpu, form, t):
     """A row of one entry has no score gradient: what is left is rounding of fp32, not of the type."""
     check(form, rows_of_sizes(), *inputs(63, 1100, 2, 1, 64, t, 6))
-
-
-@pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("t", [BF16, F16])
-def test_long_row_of_equal_weights(gpu, form, t):
-    """Weights of 2^-18 are subnormal in fp16; keys of nonzero mean add up their errors. Sums: by rows 512 entries of a chunk, then
-    the chunks' in eight interleaved sums; by tiles 16 entries a step."""
-    n = 300_000 if form == "rows" else 100_000
-    a = csr_of([list(range(n)), [0, 1]], n)
-    g = torch.Generator().manual_seed(3)
-    q = (torch.randn((2, 1, 64), generator=g) / 16).to(t)
-    k = (1 + torch.randn((n, 1, 64), generator=g) / 4).to(t)
-    v = (1 + torch.randn((n, 1, 64), generator=g)).to(t)
-    dout = (1 + torch.randn((2, 1, 64), generator=g)).to(t)
-    check(form, a, q, k, v, dout, names=("out", "lse", "dq"), depth=540 + n // 4096 if form == "rows" else 64 + n // 16)
 
 
 @pytest.mark.parametrize("form", FORMS)
@@ -105,3 +90,47 @@ def test_one_entry_has_no_score_gradient(gpu, form, t):
     zero, size = torch.zeros(q.shape, dtype=torch.float64), 258 * 64 ** -0.5 * 2.0 ** -20
     near(dq, zero, size * k.double().abs() + 1e-37, "dq")
     near(dk, zero, size * q.double().abs() + 1e-37, "dk")
+
+
+@pytest.mark.parametrize("size", [100.0, 1000.0])
+@pytest.mark.parametrize("heads,kv,dim", [(2, 1, 64), (3, 3, 128), (4, 1, 32)])
+@pytest.mark.parametrize("form", FORMS)
+def test_fp16_gradients_with_large_values(gpu, form, heads, kv, dim, size):
+    """dout . v leaves fp16's range where neither dout nor v does, nor the results."""
+    if form not in forms(dim):
+        pytest.skip("dims 64 and 128 have tiles")
+    a = rows_of_sizes()
+    q, k, v, _ = inputs(63, 1100, heads, kv, dim, F16, 7)
+    for values in (torch.full_like(v, size), (v.float() * size).to(F16)):
+        dout = torch.ones_like(q)
+        dout[5:] = 0.25
+        check(form, a, (q.float() / 4).to(F16), k, values, dout)
+
+
+@pytest.mark.parametrize("form", FORMS[1:])
+@pytest.mark.parametrize("high", [1.0, 2.0 ** 11])
+def test_fp16_gradients_of_different_sizes(gpu, form, high):
+    """Rows whose gradient is small beside another's, documents apart and in one: each is right for itself."""
+    a = positional("docs", 400, cuts=[0, 60, 190, 400])
+    q, k, v, dout = inputs(400, 400, 2, 1, 64, F16, 8)
+    dout = dout.float() * 2.0 ** -10
+    dout[70] = high
+    dout[300] = high * torch.randn(2, 64)
+    check(form, a, q, k, v, dout.to(F16))
+    dout[60:100] = 0  # the first rows that many keys see
+    check(form, a, q, k, v, dout.to(F16))
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t", [BF16, F16])
+def test_long_row_of_equal_weights(gpu, form, t):
+    """Weights of 2^-18 are subnormal in fp16; keys of nonzero mean add up their errors. Sums: by rows 512 entries of a chunk, then
+    the chunks' in eight interleaved sums; by tiles 16 entries a step."""
+    n = 300_000 if form == "rows" else 100_000
+    a = csr_of([list(range(n)), [0, 1]], n)
+    g = torch.Generator().manual_seed(3)
+    q = (torch.randn((2, 1, 64), generator=g) / 16).to(t)
+    k = (1 + torch.randn((n, 1, 64), generator=g) / 4).to(t)
+    v = (1 + torch.randn((n, 1, 64), generator=g)).to(t)
+    dout = (1 + torch.randn((2, 1, 64), generator=g)).to(t)
+    check(form, a, q, k, v, dout, names=("out", "lse", "dq"), depth=540 + n // 4096 if form == "rows" else 64 + n // 16)
