@@ -156,9 +156,27 @@ struct CutRow {
   __device__ __forceinline__ int64_t slot(int64_t c) const { return c == c0 ? 2 * c + 1 : 2 * c; }
 };
 
+// Where attn_graph.cu left the partials of type T, an infinity in them may have become NaN: the row, or key, again by gather.
+template <class T>
+__device__ __forceinline__ void row_again(const DirView &d, const AttnArgs &a, int64_t row, int h) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.dim == 32) attend_again<T, 32>(PlanRows{d}, a, row, h);
+    else if (a.dim == 64) attend_again<T, 64>(PlanRows{d}, a, row, h);
+    else if (a.dim == 128) attend_again<T, 128>(PlanRows{d}, a, row, h);
+  }
+}
+template <class T>
+__device__ __forceinline__ void key_again(const DirView &d, const AttnArgs &a, int64_t row, int hk) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.dim == 32) attend_dkv_again<T, 32>(PlanRows{d}, a, row, hk);
+    else if (a.dim == 64) attend_dkv_again<T, 64>(PlanRows{d}, a, row, hk);
+    else if (a.dim == 128) attend_dkv_again<T, 128>(PlanRows{d}, a, row, hk);
+  }
+}
+
 // Partials of cut rows (forward), merged in a fixed order. blockIdx.y: head. Lane l holds columns l, l + 32, ...
 template <class T>
-__global__ void __launch_bounds__(kThreads) attn_join_kernel(const DirView d, const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 5) attn_join_kernel(const __grid_constant__ DirView d, const __grid_constant__ AttnArgs a) {
   __shared__ float part[8][256], part_ml[8][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
   CutRow r;
@@ -190,17 +208,22 @@ __global__ void __launch_bounds__(kThreads) attn_join_kernel(const DirView d, co
     for (int w = 1; w < 8; ++w) merge(part_ml[w][0], part_ml[w][1], part[w]);
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
+  float zero = 0.f;
   T *dst = (T *)a.out.p + r.row * a.out.row + h * a.out.head;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (lane + 32 * i < a.dim) dst[lane + 32 * i] = T(acc[i] * inv);
+    if (lane + 32 * i < a.dim) {
+      dst[lane + 32 * i] = T(acc[i] * inv);
+      zero = fmaf(acc[i] * inv, 0.f, zero);
+    }
   if (a.lse && lane == 0) a.lse[r.row * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (__any_sync(0xffffffffu, zero != 0.f) && l == l) row_again<T>(d, a, r.row, h);
 }
 
 // Partials of cut rows (gradients), 2 dim floats per slot and head, summed in a fixed order. DQ: the sums x and y of a row, its
 // delta - delta0 and delta0 (attn_graph.cu; attend_dq: 0); else dk and dv of a key.
 template <class T, bool DQ>
-__global__ void __launch_bounds__(kThreads) attn_sum_kernel(const DirView d, int n_heads, const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) attn_sum_kernel(const __grid_constant__ DirView d, int n_heads, const __grid_constant__ AttnArgs a) {
   __shared__ float part[8][512], part_delta[8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, h = blockIdx.y;
   CutRow r;
@@ -238,16 +261,21 @@ __global__ void __launch_bounds__(kThreads) attn_sum_kernel(const DirView d, int
     if (a.stats) a.stats[r.row * a.heads + h] = make_float2(lse == -INFINITY ? INFINITY : lse * kLog2e, whole);
     else a.delta[r.row * a.heads + h] = whole;
   }
+  float zero = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int col = lane + 32 * i;
     if (col >= a.dim) continue;
+    zero = fmaf(x[i], 0.f, fmaf(y[i], 0.f, zero));
     if (DQ) {
       ((T *)a.dq.p)[r.row * a.dq.row + h * a.dq.head + col] = T((x[i] - delta * y[i]) * a.scale);
     } else {
       ((T *)a.dk.p)[r.row * a.dk.row + h * a.dk.head + col] = T(x[i]);
       ((T *)a.dv.p)[r.row * a.dv.row + h * a.dv.head + col] = T(y[i]);
     }
+  }
+  if constexpr (!DQ) {
+    if (__any_sync(0xffffffffu, zero != 0.f)) key_again<T>(d, a, r.row, h);
   }
 }
 

@@ -9,17 +9,21 @@
 //
 // Rows go from global memory to fragments without a stop (frag.cuh). The next 16 keys are requested as soon as the products
 // have read the present ones, so each warp keeps about 8 KB in flight. Weights are split in two 16-bit parts, p = hi + lo, with a product
-// for each: the tensor cores are idle anyway, and the result is then as exact as with fp32 weights.
+// for each: the tensor cores are idle anyway, and no more than 2^-16 of a weight (fp16: 2^-22) is lost. An infinity that is listed
+// would meet lo parts of 0 or of the other sign: rows whose result is not finite, though their weights are, are done again by
+// attn_row.cuh's gather.
 #include <algorithm>
 #include <type_traits>
 
 #include "attn_decode.h"
+#include "attn_row.cuh"
 #include "frag.cuh"
 
 namespace dsp {
 namespace {
 
 constexpr int kThreads = 128;
+constexpr int kMaxList = 1024, kBadRows = kMaxList / kRowUnits + 4;  // units of a chunk; its rows
 
 // A row is read once: past L1, and as DRAM delivers it (240 -> 231 us on 64 x ~4800 tokens, 8 heads of 128, against plain loads).
 __device__ __forceinline__ uint4 ld_row(const void *p) {
@@ -63,7 +67,7 @@ struct Tile {
 };
 
 template <class T, int D>
-__global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows d, const AttnArgs a, int head_tiles) {
+__global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const __grid_constant__ ListRows d, const __grid_constant__ AttnArgs a, int head_tiles) {
   const int lane = threadIdx.x & 31, t = lane & 3, n8 = lane >> 2;
   const int kv_heads = a.heads / a.group, per_chunk = kv_heads * head_tiles;
   const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
@@ -78,6 +82,10 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
   for (int j = 0; j < 2; ++j) slope2[j] = a.slopes && 2 * t + j < live ? __ldg(a.slopes + h0 + 2 * t + j) * kLog2e : 0.f;
   int64_t r0, r1, p, p1;
   d.chunk(chunk, r0, r1, p, p1);
+  // heads of the chunk's rows to be done again (lists that are no CSR may give a chunk more rows than kBadRows)
+  __shared__ uint8_t all_bad[kThreads / 32][kBadRows];
+  for (int i = lane; i < kBadRows; i += 32) all_bad[threadIdx.x >> 5][i] = 0;
+  __syncwarp();
   const bool head_cut = p > d.ptr(r0);
   for (int64_t row = r0; row <= r1; ++row) {
     if (row == r1 && (p >= p1 || row >= d.n())) break;
@@ -165,11 +173,13 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
     }
     const bool cut_head = row == r0 && head_cut, cut = cut_head || row == r1;
     const int64_t slot = (cut_head ? 2 * chunk : 2 * chunk + 1) * a.heads;
+    uint32_t bad = 0;  // heads with a result that is not finite, though the weights are
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int h = h0 + 2 * t + j;
       if (2 * t + j >= live) continue;
       const float inv = l[j] == 0.f ? 0.f : 1.f / l[j];
+      float zero = 0.f;
 #pragma unroll
       for (int i = 0; i < D / 64; ++i) {
         // elements 2 c (acc[.][j]) and 2 c + 1 (acc[.][2 + j]) of vector n8 + 8 i
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
           st_f32<8>(a.slots + (slot + h) * D + col, f);
         } else {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) f[c] *= inv;
+          for (int c = 0; c < 8; ++c) f[c] *= inv, zero = fmaf(f[c], 0.f, zero);
           RowVec<T, 8>::st((T *)a.out.p + row * a.out.row + (int64_t)h * a.out.head + col, f);
         }
       }
@@ -189,16 +199,28 @@ __global__ void __launch_bounds__(kThreads, 3) attn_decode_kernel(const ListRows
         if (cut) a.slot_ml[2 * (slot + h)] = m[j], a.slot_ml[2 * (slot + h) + 1] = l[j];
         else if (a.lse) a.lse[row * a.heads + h] = l[j] == 0.f ? -INFINITY : (m[j] + log2f(l[j])) * kLn2;
       }
+      if (zero != 0.f && l[j] == l[j]) bad |= 1u << (2 * t + j);
     }
+    if (__any_sync(0xffffffffu, bad != 0) && row - r0 < kBadRows)
+      all_bad[threadIdx.x >> 5][row - r0] = (uint8_t)__reduce_or_sync(0xffffffffu, bad);
     p = pe;
   }
+  __syncwarp();
+  const uint8_t *bad_rows = all_bad[threadIdx.x >> 5];
+  uint32_t any = 0;
+  for (int i = lane; i < kBadRows; i += 32) any |= bad_rows[i];
+  if (!__any_sync(0xffffffffu, any != 0)) return;
+#pragma unroll 1
+  for (int i = 0; i < kBadRows; ++i)  // after the loop: a call within it would cost its registers
+#pragma unroll 1
+    for (uint32_t bad = bad_rows[i]; bad; bad &= bad - 1) attend_again<T, D>(d, a, r0 + i, h0 + __ffs(bad) - 1);
 }
 
 // Rows cut across chunks: a block per row and head. The partials' weights 2^(m - max) first, each by a thread, then the
 // weighted sums: groups of dim threads, a thread per column, take every groups-th partial, and their sums are added in order.
 constexpr int kJoin = 512;
 template <class T>
-__global__ void __launch_bounds__(kJoin) attn_decode_join_kernel(const ListRows d, const AttnArgs a) {
+__global__ void __launch_bounds__(kJoin, 2) attn_decode_join_kernel(const __grid_constant__ ListRows d, const __grid_constant__ AttnArgs a) {
   __shared__ float weight[kJoin], red[kJoin / 32], part[kJoin];
   const int64_t r = blockIdx.x;
   const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -241,11 +263,20 @@ __global__ void __launch_bounds__(kJoin) attn_decode_join_kernel(const ListRows 
   l = 0.f;
 #pragma unroll
   for (int w = 0; w < kJoin / 32; ++w) l += red[w];
+  bool bad = false;
   if (tid < a.dim) {
     for (int k = 1; k < groups; ++k) acc += part[k * a.dim + tid];
-    ((T *)a.out.p)[r * a.out.row + h * a.out.head + tid] = T(l == 0.f ? 0.f : acc / l);
+    acc = l == 0.f ? 0.f : acc / l;
+    bad = !isfinite(acc);
+    ((T *)a.out.p)[r * a.out.row + h * a.out.head + tid] = T(acc);
   }
   if (a.lse && tid == 0) a.lse[r * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if constexpr (sizeof(T) == 2) {
+    if (__syncthreads_or(bad && l == l) && warp == 0) {  // the barrier: other warps' results are written
+      if (a.dim == 64) attend_again<T, 64>(d, a, r, h);
+      else if (a.dim == 128) attend_again<T, 128>(d, a, r, h);
+    }
+  }
 }
 
 template <class T>
@@ -267,7 +298,7 @@ int32_t decode_units(int64_t rows, int64_t nnz, int heads, int kv_heads, bool te
   // 24 / 36 / 48 warps an SM: 250 / 231 / 240 us.
   const int64_t width = tensor ? (int64_t)kv_heads * ((heads / kv_heads + 7) / 8) : heads;
   const int64_t l = (row_start(rows, nnz) * width + 148 * 36 - 1) / (148 * 36);
-  return (int32_t)std::min<int64_t>(1024, std::max<int64_t>(32, (l + 15) / 16 * 16));
+  return (int32_t)std::min<int64_t>(kMaxList, std::max<int64_t>(32, (l + 15) / 16 * 16));
 }
 
 int decode_join(const ListRows &d, const AttnArgs &a, int dtype, cudaStream_t s) {

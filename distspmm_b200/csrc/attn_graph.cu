@@ -3,8 +3,8 @@
 // For patterns too thin for tiles (a graph's edges). The formulas are those of attn.cu; what bounds both is the gather of a row
 // of k and one of v (q and dout, by columns) for each entry and head out of L2. Here the arithmetic is given to mma.sync, though
 // an entry has but one query for each head to be multiplied with (of m16n8k16 products, 8 columns are entries and 1 to 8 rows
-// query heads): R-MAT 15, 8 heads of 64, bf16: forward 577 -> 367 us, dq 632 -> 469,
-// dk and dv 681 -> 581 against dot products by shuffles.
+// query heads): R-MAT 15, 8 heads of 64, bf16: forward 577 -> 377 us, dq 632 -> 468,
+// dk and dv 681 -> 597 against dot products by shuffles.
 //
 //   pass      16 entries as columns   rows                         then, entries turned
 //   forward   k                       q of up to 8 heads           v   x weights
@@ -16,11 +16,13 @@
 // over 16-entry steps runs on across rows: the next step's rows are requested as soon as the present ones are in the products,
 // so a short row costs no wait. Weights enter the second product as hi + lo (2^-16 of a weight is lost at most). So dq takes its
 // differences dp - delta from delta0 = dout . out, within out's rounding of delta, before they are split, and the rest off after the
-// products: dq = scale (x - g y) with g = delta - delta0 = sum p (dp - delta0).
+// products: dq = scale (x - g y) with g = delta - delta0 = sum p (dp - delta0). An infinity that is listed would meet lo parts of 0 or of
+// the other sign: rows whose result is not finite are done again by attn_row.cuh's gather (dq: any such row is NaN by the formula).
 #include <algorithm>
 #include <type_traits>
 
 #include "attn_graph.h"
+#include "attn_row.cuh"
 #include "frag.cuh"
 
 namespace dsp {
@@ -28,11 +30,6 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr float kSlack = 8.f;
-
-struct Lists {
-  int32_t cols[kMaxUnits];
-  int32_t ptr[kMaxUnits / kRowUnits + 4];
-};
 
 // A step: 16 entries from b on, of a row whose entries in this chunk end at pe, for query head number h of the group (dk, dv).
 struct Step {
@@ -60,10 +57,11 @@ __device__ __forceinline__ float largest(const float (&x)[4]) {
 
 template <class T, int D, AttnPass M>
 __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M == kDkv ? 3 : 4))
-    attn_graph_kernel(const DirView d, const AttnArgs a, int head_tiles) {
+    attn_graph_kernel(const __grid_constant__ DirView d, const __grid_constant__ AttnArgs a, int head_tiles) {
   constexpr int VR = D / 32, VT = kTurned<D>, NT = kTiles<D>;
   constexpr int kWidth = M == kForward ? 8 : M == kDq ? 4 : 1;  // query heads of a warp's columns
-  __shared__ Lists all_lists[kThreads / 32];
+  __shared__ ChunkLists all_lists[kThreads / 32];
+  __shared__ uint8_t all_bad[kThreads / 32][kMaxUnits / kRowUnits + 4];  // heads of the chunk's rows to be done again
   const int lane = threadIdx.x & 31, t = lane & 3, n8 = lane >> 2;
   const int kv_heads = a.heads / a.group, per_chunk = kv_heads * head_tiles;
   const int64_t item = ((int64_t)blockIdx.x * kThreads + threadIdx.x) >> 5;
@@ -71,10 +69,13 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
   if (chunk >= d.n_chunks) return;
   const int hk = (int)(item - chunk * per_chunk) / head_tiles, h0 = hk * a.group + (int)(item % head_tiles) * kWidth;
   const int live = M == kDkv ? 1 : min(kWidth, (hk + 1) * a.group - h0);  // query heads h0 .. h0 + live - 1
-  Lists &list = all_lists[threadIdx.x >> 5];
+  ChunkLists &list = all_lists[threadIdx.x >> 5];
   const int32_t r0 = __ldg(d.row0 + chunk), r1 = __ldg(d.row0 + chunk + 1), p0 = __ldg(d.nz0 + chunk), p1 = __ldg(d.nz0 + chunk + 1);
-  for (int i = lane; i <= r1 - r0 + 1; i += 32)
+  uint8_t *bad_rows = all_bad[threadIdx.x >> 5];
+  for (int i = lane; i <= r1 - r0 + 1; i += 32) {
     if (r0 + i <= d.n) list.ptr[i] = __ldg(d.ptr + r0 + i);
+    bad_rows[i] = 0;
+  }
 #pragma unroll 4
   for (int i = lane; i < p1 - p0; i += 32) list.cols[i] = __ldg(d.cols + p0 + i);
   __syncwarp();
@@ -385,11 +386,13 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
     const float l2[2] = {__shfl_sync(0xffffffffu, l, 8 * t), __shfl_sync(0xffffffffu, l, 8 * t + 4)};
     const bool writes = D >= 64 || n8 < D / 8;
     if constexpr (M == kForward) {
+      uint32_t bad = 0;  // heads with a result that is not finite, though the weights are
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int h = h0 + 2 * t + j;
         if (2 * t + j >= live) continue;
         const float inv = l2[j] == 0.f ? 0.f : 1.f / l2[j];
+        float zero = 0.f;
 #pragma unroll
         for (int i = 0; i < VT; ++i) {
           float f[8];
@@ -400,16 +403,18 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
             st_f32<8>(a.slots + (slot * a.heads + h) * D + col, f);
           } else {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) f[c] *= inv;
+            for (int c = 0; c < 8; ++c) f[c] *= inv, zero = fmaf(f[c], 0.f, zero);
             RowVec<T, 8>::st((T *)a.out.p + (int64_t)row * a.out.row + (int64_t)h * a.out.head + col, f);
           }
         }
+        if (zero != 0.f && l2[j] == l2[j]) bad |= 1u << (2 * t + j);
       }
       if (t == 0 && n8 < live) {
         const int64_t at = slot * a.heads + h0 + n8;
         if (cut) a.slot_ml[2 * at] = m, a.slot_ml[2 * at + 1] = l;
         else if (a.lse) a.lse[(int64_t)row * a.heads + h0 + n8] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
       }
+      if (__any_sync(0xffffffffu, bad != 0)) bad_rows[row - r0] = (uint8_t)__reduce_or_sync(0xffffffffu, bad);
     } else if constexpr (M == kDq) {
       // x of heads 2 t, 2 t + 1 in lanes t < 2, their y in lanes t + 2
 #pragma unroll
@@ -443,6 +448,7 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
         else a.stats[(int64_t)row * a.heads + h0 + n8] = make_float2(lse2, delta0 + l);
       }
     } else {
+      float zero = 0.f;
 #pragma unroll
       for (int i = 0; i < VT; ++i) {
         float f[8], f1[8], g[8], g1[8];
@@ -461,12 +467,27 @@ __global__ void __launch_bounds__(kThreads, D == 128 ? (M == kDkv ? 2 : 3) : (M 
         } else {
           RowVec<T, 8>::st((T *)a.dk.p + (int64_t)row * a.dk.row + (int64_t)hk * a.dk.head + col, f);
           RowVec<T, 8>::st((T *)a.dv.p + (int64_t)row * a.dv.row + (int64_t)hk * a.dv.head + col, g);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) zero = fmaf(f[c], 0.f, fmaf(g[c], 0.f, zero));
         }
       }
+      if (__any_sync(0xffffffffu, zero != 0.f)) bad_rows[row - r0] = 1;
     }
     idle(row + 1, more ? next.row : r1);
     if (!more) break;
     now = next;
+  }
+  if constexpr (M != kDq) {
+    __syncwarp();
+#pragma unroll 1
+    for (int i = 0; i < r1 - r0; ++i) {  // after the loop: a call within it would cost its registers
+      if constexpr (M == kDkv) {
+        if (bad_rows[i]) attend_dkv_again<T, D>(PlanRows{d}, a, r0 + i, hk);
+      } else {
+#pragma unroll 1
+        for (uint32_t bad = bad_rows[i]; bad; bad &= bad - 1) attend_again<T, D>(PlanRows{d}, a, r0 + i, h0 + __ffs(bad) - 1);
+      }
+    }
   }
 }
 

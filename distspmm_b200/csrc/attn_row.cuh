@@ -182,6 +182,17 @@ __device__ __forceinline__ void put_row(const AttnArgs &a, int64_t row, int h, f
   if (a.lse && (threadIdx.x & 31) == 0) a.lse[row * a.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
+// A whole row once more, for head h: where products of hi + lo parts met an infinity (lo x infinity), which here stays one.
+template <class T, int D, class Rows>
+__device__ __noinline__ void attend_again(const Rows &d, const AttnArgs &a, int64_t row, int h) {
+  using H = HeadRow<T, 8, D / 8, 1>;
+  float y[1][8], m, l;
+  const typename Rows::Index p = d.ptr(row), pe = d.ptr(row + 1);
+  __syncwarp();  // the first result was written by other lanes than will write it now
+  attend<H, D / 8>(d, a, row, h, p, pe, pe, m, l, y);
+  put_row<H, D / 8>(a, row, h, m, l, y);
+}
+
 // The entries [p, pe) of a row for head h, for dq. With c = 1 - tanh^2: delta = sum p dp, x = sum p c dp k, y = sum p c k, so
 // that dq = scale (x - delta y) needs one pass, and delta is not that of a rounded out (in a row of one entry the two parts
 // cancel exactly, as they should).
@@ -270,7 +281,7 @@ __device__ __forceinline__ void attend_dkv(const Rows &d, const AttnArgs &a, int
         H::fetch(a.q, c[u], h, lane, a.dim, at < pe, q[u]);
         H::fetch(a.dout, c[u], h, lane, a.dim, at < pe, dout[u]);
         lse2[u] = at < pe ? a.lse[(int64_t)c[u] * a.heads + h] * kLog2e : -INFINITY;
-        delta[u] = at < pe ? a.delta[(int64_t)c[u] * a.heads + h] : 0.f;
+        delta[u] = at >= pe ? 0.f : a.stats ? a.stats[(int64_t)c[u] * a.heads + h].y : a.delta[(int64_t)c[u] * a.heads + h];
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -295,6 +306,19 @@ __device__ __forceinline__ void attend_dkv(const Rows &d, const AttnArgs &a, int
         dk[w][i] += __shfl_xor_sync(0xffffffffu, dk[w][i], o);
         dv[w][i] += __shfl_xor_sync(0xffffffffu, dv[w][i], o);
       }
+}
+
+// As attend_again, of a key.
+template <class T, int D>
+__device__ __noinline__ void attend_dkv_again(const PlanRows &d, const AttnArgs &a, int64_t row, int hk) {
+  using H = HeadRow<T, 8, D / 8, 1>;
+  float dk[1][8], dv[1][8];
+  __syncwarp();
+  attend_dkv<H, D / 8>(d, a, row, hk, (int32_t)d.ptr(row), (int32_t)d.ptr(row + 1), dk, dv);
+  if ((threadIdx.x & 31) < D / 8) {
+    H::store(a.dk, row, hk, threadIdx.x & 31, D, dk);
+    H::store(a.dv, row, hk, threadIdx.x & 31, D, dv);
+  }
 }
 
 }  // namespace dsp

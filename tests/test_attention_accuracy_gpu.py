@@ -134,3 +134,75 @@ def test_long_row_of_equal_weights(gpu, form, t):
     v = (1 + torch.randn((n, 1, 64), generator=g)).to(t)
     dout = (1 + torch.randn((2, 1, 64), generator=g)).to(t)
     check(form, a, q, k, v, dout, names=("out", "lse", "dq"), depth=540 + n // 4096 if form == "rows" else 64 + n // 16)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t,dim", [(BF16, 64), (F16, 128), (BF16, 32), (F16, 96), (F32, 64)])
+def test_infinite_values_that_are_listed(gpu, form, t, dim):
+    """An infinity in a listed value is the row's result in that place (both signs: NaN), in short and in cut rows."""
+    if form not in forms(dim):
+        pytest.skip("dims 64 and 128 have tiles")
+    a = rows_of_sizes()
+    q, k, v, _ = inputs(63, 1100, 2, 1, dim, t, 10)
+    v[5, :, 3] = math.inf  # row 5, row 25 and others
+    v[31, :, 4] = -math.inf
+    v[900, :, 5] = math.inf  # row 25 alone
+    v[901, :, 5] = -math.inf
+    want, lse, p = attention64(mask_of(a), q.double(), k.double(), v.double().nan_to_num(posinf=0, neginf=0), dim ** -0.5)
+    tol = bounds(mask_of(a), q.double(), k.double(), v.double().nan_to_num(posinf=0, neginf=0), want, lse, p, t, dim ** -0.5)
+    mask = mask_of(a)
+    want[mask[:, 5], :, 3] = math.inf
+    want[mask[:, 31], :, 4] = -math.inf
+    got, got_lse = d.sparse_attention_forward(d.SparsePattern(a, attention=True, form=form), *(x.cuda() for x in (q, k, v)))
+    got = got.cpu()
+    assert torch.isnan(got[25, :, 5]).all()
+    want[25, :, 5] = 0
+    got[25, :, 5] = 0
+    near(got, want, tol["out"], "out")
+    near(got_lse, lse, tol["lse"], "lse")
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("t,dim", [(BF16, 64), (F16, 128), (BF16, 32), (F16, 96), (F32, 64)])
+def test_infinite_gradients(gpu, form, t, dim):
+    """An infinity in dout is dv's in that place for every key of its row; row 25 is cut, and by columns key 5 is long."""
+    if form not in forms(dim):
+        pytest.skip("dims 64 and 128 have tiles")
+    a = rows_of_sizes()
+    q, k, v, dout = inputs(63, 1100, 2, 1, dim, t, 13)
+    dout[25, :, 3] = math.inf
+    dout[45, :, 4] = -math.inf
+    mask = mask_of(a)
+    w = [x.double().requires_grad_() for x in (q, k, v)]
+    o, l, p = attention64(mask, *w, dim ** -0.5)
+    fine = dout.double().nan_to_num(posinf=0, neginf=0)
+    grads = torch.autograd.grad(o, w, fine)
+    tol = bounds(mask, *(x.detach() for x in (*w, o, l, p)), t, dim ** -0.5, dout=fine, grads=grads)
+    want = grads[2].clone()
+    want[mask[25], :, 3] = math.inf
+    want[mask[45], :, 4] = -math.inf
+    pat = d.SparsePattern(a, grad=True, attention=True, form=form)
+    qc, kc, vc, dc = (x.cuda() for x in (q, k, v, dout))
+    dv = d.sparse_attention_backward(pat, dc, qc, kc, vc, *d.sparse_attention_forward(pat, qc, kc, vc))[2]
+    near(dv, want, tol["dv"], "dv")
+
+
+@pytest.mark.parametrize("t,dim", [(BF16, 64), (F16, 128), (BF16, 96), (F32, 64)])
+def test_infinite_values_in_a_cache(gpu, t, dim):
+    q, k, v, _ = inputs(3, 700, 8, 2, dim, t, 11)
+    ptr, idx = lists([3, 600, 90], 700, 2)
+    v[idx[1], :, 3] = math.inf
+    v[idx[500], :, 4] = -math.inf
+    fine = v.double().nan_to_num(posinf=0, neginf=0)
+    got = d.sparse_attention_decode(*(x.cuda() for x in (q, k, v, ptr, idx)))
+    for r in range(3):
+        at = idx[ptr[r]:ptr[r + 1]]
+        mask = torch.ones(1, at.numel(), dtype=torch.bool)
+        args = q[r:r + 1].double(), k[at].double(), fine[at]
+        o, l, p = attention64(mask, *args, dim ** -0.5)
+        tol = bounds(mask, *args, o, l, p, t, dim ** -0.5)
+        if (at == idx[1]).any():
+            o[:, :, 3] = math.inf
+        if (at == idx[500]).any():
+            o[:, :, 4] = -math.inf
+        near(got[r:r + 1], o, tol["out"], "out")
