@@ -133,11 +133,11 @@ struct CapPoly {
     const float k = cap > 0.f ? scale / cap : 0.f, k2 = k * k;
     limit = k2 < 1e20f ? 0.25f / fmaxf(k2, 1e-20f) : -1.f;  // beyond, the coefficients overflow
     float f = k * cap;
-    c[0] = 0.999999987f * f;
-    c[1] = -0.333330719f * (f *= k2);
-    c[2] = 0.13324829f * (f *= k2);
-    c[3] = -0.0529892412f * (f *= k2);
-    c[4] = 0.017141319f * (f *= k2);
+    c[0] = kTanh0 * f;
+    c[1] = kTanh1 * (f *= k2);
+    c[2] = kTanh2 * (f *= k2);
+    c[3] = kTanh3 * (f *= k2);
+    c[4] = kTanh4 * (f *= k2);
   }
 };
 template <int N>

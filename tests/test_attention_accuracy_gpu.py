@@ -136,6 +136,30 @@ def test_long_row_of_equal_weights(gpu, form, t):
     check(form, a, q, k, v, dout, names=("out", "lse", "dq"), depth=540 + n // 4096 if form == "rows" else 64 + n // 16)
 
 
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e8, 1e30])
+@pytest.mark.parametrize("form,t,dim", [("tiles", BF16, 64), ("tiles", F16, 128), ("rows", BF16, 64), ("rows", F16, 32), ("rows", F32, 64)])
+def test_large_caps(gpu, form, t, dim, cap):
+    """A cap far above the scores leaves them as they are."""
+    a = MASKS["window"]()
+    check(form, a, *inputs(300, 300, 2, 1, dim, t, 9), cap=cap)
+
+
+@pytest.mark.parametrize("cap", [1e3, 1e5, 1e8, 1e30])
+@pytest.mark.parametrize("t,dim", [(BF16, 64), (F16, 128), (BF16, 96), (F32, 64)])
+def test_large_caps_of_decode(gpu, t, dim, cap):
+    q, k, v, _ = inputs(2, 500, 4, 2, dim, t, 9)
+    ptr, idx = lists([333, 41], 500)
+    out, lse = d.sparse_attention_decode(*(x.cuda() for x in (q, k, v, ptr, idx)), softcap=cap, return_lse=True)
+    for r in range(2):
+        at = idx[ptr[r]:ptr[r + 1]]
+        mask = torch.ones(1, at.numel(), dtype=torch.bool)
+        args = [x.double() for x in (q[r:r + 1], k[at], v[at])]
+        o, l, p = attention64(mask, *args, dim ** -0.5, cap)
+        tol = bounds(mask, *args, o, l, p, t, dim ** -0.5, cap)
+        near(out[r:r + 1], o, tol["out"], "out")
+        near(lse[r:r + 1], l, tol["lse"], "lse")
+
+
 @pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("t,dim", [(BF16, 64), (F16, 128), (BF16, 32), (F16, 96), (F32, 64)])
 def test_infinite_values_that_are_listed(gpu, form, t, dim):
