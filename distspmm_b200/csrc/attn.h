@@ -25,7 +25,7 @@ struct AttnArgs {
   float *lse;        // [rows][heads]
   float *delta;      // [rows][heads] dout . out
   float2 *stats;     // [rows][heads] lse in base 2 (+infinity: a row without entries) and delta, for attn_graph.cu's dk, dv
-  const uint32_t *dout_max;  // bits of the largest finite |dout| (fp16 gradients by tiles)
+  const uint32_t *dout_max;  // [heads][rows] bits of the largest finite |dout| (fp16 gradients by tiles)
   float *slots;      // partials of cut rows: [2 n_chunks][heads][width]
   float *slot_ml;    // [2 n_chunks][heads][2] running maximum and sum (forward), delta - delta0 and delta0 (dq)
 };
@@ -52,8 +52,8 @@ __device__ __forceinline__ float capped(float s, float cap, float inv_cap2, floa
 }
 
 // fp16 has few exponents: gradients of scores are carried with a power of two that brings the largest |dout| near 16.
-__device__ __forceinline__ float dout_scale(const uint32_t *dout_max) {
-  const int e = (int)(__ldg(dout_max) >> 23);  // biased exponent; 255: not finite
+__device__ __forceinline__ float dout_scale(uint32_t dout_max) {
+  const int e = (int)(dout_max >> 23);  // biased exponent; 255: not finite
   return e > 0 && e < 255 ? __uint_as_float((uint32_t)min(max(127 + 4 - (e - 127), 1), 254) << 23) : 1.f;
 }
 

@@ -23,7 +23,8 @@
 // out; so dq = sum p c (dp - delta0) k - g sum p c k with g = sum p (dp - delta0) = delta - delta0, whose weights p c may be rounded once, as g is
 // but a rounding itself; delta0 + g is what dk takes. fp16 has few exponents:
 // weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is scaled by a power of two that brings the
-// largest |dout| near 16; both come off in the epilogue.
+// largest |dout| (of the row for dq, of the streamed rows for dk and dv) near 16; both come off in the epilogue. Rows whose largest dS
+// still leaves fp16's range, or comes so low that its parts lose bits, are computed again as below.
 //
 // Masks and values that are not finite: an entry that is not listed has weight 0, but 0 x NaN in the product is NaN. So a row
 // whose result is not finite is computed again by attn_row.cuh's gather, which reads listed entries only. A NaN that belongs
@@ -275,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
   __shared__ uint64_t bars[1 + 4 * ST + 2 * NB + kAccBars + 1];
   __shared__ uint32_t tmem_result;
   __shared__ int dead_flag;
+  __shared__ uint32_t tops[4];
   __shared__ __align__(16) float row_lse[2][64], row_delta[2][64];  // dk, dv: -lse (base 2) and -delta of the streamed rows
   volatile int *dead = &dead_flag;
 
@@ -565,11 +567,30 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         if (x.a.lse) x.a.lse[row * x.a.heads + head] = -INFINITY;
       }
     } else {
-      float up = kBf16 ? 1.f : dout_scale(x.a.dout_max);
+      const bool live = row < n_rows;
+      float up = 1.f, dout_top = 0.f;
+      if (!kBf16) {  // the largest |dout|: dq: of this thread's row, dk, dv: of the rows that are streamed
+        uint32_t bits = 0;
+        if (M == kDq) {
+          if (live) bits = __ldg(x.a.dout_max + (int64_t)head * n_rows + row);
+        } else {
+          for (int i = r; i < iters * kTileCols; i += kWeightThreads) {
+            const int it = i / kTileCols;
+            const int64_t q = (int64_t)__ldg(x.t.col + t0 + it % nt) * kTileCols + i % kTileCols;
+            if (q < x.a.n_queries) bits = max(bits, __ldg(x.a.dout_max + (int64_t)(head * x.a.group + it / nt) * x.a.n_queries + q));
+          }
+          bits = __reduce_max_sync(0xffffffffu, bits);
+          if ((threadIdx.x & 31) == 0) tops[warp] = bits;
+          asm volatile("bar.sync 1, 128;" ::: "memory");  // the weights' warps
+          bits = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+        }
+        dout_top = __uint_as_float(bits);
+        up = dout_scale(bits);
+      }
       const float down = x.a.scale / up;
       if (M == kDkv && !kBf16) up *= 0x1p-12f;  // the weights of dk, dv are 2^12 up themselves
       constexpr float kUp = kBf16 ? 0.f : 12.f;
-      const bool live = row < n_rows;
+      float most = 0.f, most_p = 0.f;  // fp16: the largest score gradient and weight as they are carried
       float lse2 = INFINITY, delta = 0.f, gap[2] = {0.f, 0.f};  // gap: sum of p (dp - delta), times up
       if (M == kDq && live) {
         lse2 = x.a.lse[row * x.a.heads + head] * kLog2e;
@@ -655,7 +676,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
           if (M == kDkv) {
             uint32_t w[16], lo[16];
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) split2<T>(p[c], p[c + 1], w[c / 2], lo[c / 2]);
+            for (int c = 0; c < 32; c += 2) {
+              if (!kBf16) most_p = max3(most_p, p[c], p[c + 1]);
+              split2<T>(p[c], p[c + 1], w[c / 2], lo[c / 2]);
+            }
             tmem_st16(tm_s + lanes + b * 64 + half * 32, w);
             tmem_st16(tm_r + lanes + b * 64 + half * 32 + 16, lo);
           }
@@ -694,7 +718,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
           }
           uint32_t v[16], lo[16];
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) split2<T>(e[c], e[c + 1], v[c / 2], lo[c / 2]);
+          for (int c = 0; c < 32; c += 2) {
+            if (!kBf16) most = max3(most, fabsf(e[c]), fabsf(e[c + 1]));
+            split2<T>(e[c], e[c + 1], v[c / 2], lo[c / 2]);
+          }
           tmem_st16(tm_r + lanes + b * 64 + half * 32, v);
           tmem_st16(tm_s + lanes + b * 64 + half * 32 + 16, lo);
         }
@@ -714,6 +741,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
           fine = put_acc<T, D>(tm_acc0 + lanes, kBf16 ? 1.f : 0x1p-12f, x.a.dv, row, head, live);
           fine = put_acc<T, D>(tm_acc1 + lanes, down, x.a.dk, row, head, live) && fine;
         }
+        // fp16 parts are within 2^-25, 2^-13 of the largest at kLeast; below, the row is done again (dv: where 2^-37 of dout, from each of
+        // the streamed rows, could be seen in it)
+        constexpr float kLeast = 0x1p-12f;
+        if (most > 0.f && most < kLeast) fine = false;
+        if (most_p > 0.f && most_p < kLeast && dout_top * ((float)iters * kTileCols) > 2048.f) fine = false;
         const uint32_t bad = __ballot_sync(0xffffffffu, live && !fine);
         if (bad) redo<T, D, M>(x, row0 + 32 * warp, head, bad);
       } else if (ok && live) {
@@ -770,7 +802,7 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const __grid_consta
   if (__any_sync(0xffffffffu, !fine)) redo<T, D, kFwd>(x, row, h, 1u);
 }
 
-// delta0_i = dout_i . out_i of each row and head, a warp each (fp16: and the largest finite |dout|).
+// delta0_i = dout_i . out_i of each row and head, a warp each (fp16: and the largest finite |dout|, [heads][rows]).
 template <class T, int D>
 __global__ void __launch_bounds__(256) attn_delta_kernel(int64_t rows, const AttnArgs a, uint32_t *dout_max) {
   const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
@@ -792,7 +824,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(int64_t rows, const Att
   if (lane == 0) a.delta[item] = s;
   if (std::is_same<T, __half>::value) {
     const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-    if (lane == 0 && bits > *(volatile uint32_t *)dout_max) atomicMax(dout_max, bits);  // a maximum does not depend on the order
+    if (lane == 0) dout_max[h * rows + row] = bits;
   }
 }
 
@@ -877,9 +909,6 @@ int forward(const dsp_pattern *p, TileArgs x, cudaStream_t s) {
 
 template <class T, int D>
 int gradients(const dsp_pattern *p, TileArgs x, uint32_t *dout_max, cudaStream_t s) {
-  cudaError_t e = cudaSuccess;
-  if (std::is_same<T, __half>::value) e = cudaMemsetAsync(dout_max, 0, 4, s);
-  if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_attn_grad: %s", cudaGetErrorString(e));
   attn_delta_kernel<T, D><<<(unsigned)((p->rows * x.a.heads + 7) / 8), 256, 0, s>>>(p->rows, x.a, dout_max);
   x.a.dout_max = dout_max;
   const int rc = launch<T, D, kDq>(p, x, s);
@@ -916,7 +945,9 @@ int tile_forward(const dsp_pattern *p, const AttnArgs &a, int dtype, void *ws, c
   return a.dim == 64 ? forward<__half, 64>(p, x, s) : forward<__half, 128>(p, x, s);
 }
 
-int64_t tile_grad_bytes(const dsp_pattern *p, const dsp_attn_desc *d) { return up256(4 * p->rows * d->heads) + 256; }
+int64_t tile_grad_bytes(const dsp_pattern *p, const dsp_attn_desc *d) {
+  return up256(4 * p->rows * d->heads) * (d->dtype == DSP_F16 ? 2 : 1);  // delta, and the largest |dout| of each row
+}
 
 int tile_gradients(const dsp_pattern *p, const AttnArgs &a, int dtype, void *ws, cudaStream_t s) {
   TileArgs x = {};

@@ -107,7 +107,7 @@ def test_fp16_gradients_with_large_values(gpu, form, heads, kv, dim, size):
         check(form, a, (q.float() / 4).to(F16), k, values, dout)
 
 
-@pytest.mark.parametrize("form", FORMS[1:])
+@pytest.mark.parametrize("form", FORMS)
 @pytest.mark.parametrize("high", [1.0, 2.0 ** 11])
 def test_fp16_gradients_of_different_sizes(gpu, form, high):
     """Rows whose gradient is small beside another's, documents apart and in one: each is right for itself."""
