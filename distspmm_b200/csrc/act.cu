@@ -195,12 +195,12 @@ __device__ __forceinline__ Chunk load_chunk(const DirView &d, int64_t chunk, Chu
   return c;
 }
 
-// One chunk per warp, row by row in steps of G U entries: a row's last step is partly masked. A finished row goes through the
+// One chunk per warp (TB: type of the gathered rows), row by row in steps of G U entries: a row's last step is partly masked. A finished row goes through the
 // epilogue, a cut one to its slot. The residual of the running row is requested when the row begins, so that its end does not
 // wait; rows without entries need no more than act(bias), worked out once.
-template <class T, int VE, int LPR, int VPL, int U, int MINB, bool PERM>
+template <class T, class TB, int VE, int LPR, int VPL, int U, int MINB, bool PERM>
 __global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirView d, const ActArgs a) {
-  using V = RowVec<T, VE>;
+  using V = RowVec<TB, VE>;
   using S = Spread<VE, LPR>;
   constexpr int G = S::G, FE = S::FE;
   using F = RowVec<T, FE>;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirVi
   const char *src[VPL];  // lanes behind the last column read column 0 and store nothing
 #pragma unroll
   for (int w = 0; w < VPL; ++w) {
-    src[w] = (const char *)((const T *)a.B + (col0 + w * LPR * VE < a.N ? col0 + w * LPR * VE : 0));
+    src[w] = (const char *)((const TB *)a.B + (col0 + w * LPR * VE < a.N ? col0 + w * LPR * VE : 0));
     res[w] = F::zero();
 #pragma unroll
     for (int i = 0; i < FE; ++i) {
@@ -244,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirVi
       if (col < a.N) st_f32<FE>(a.slots + slot * a.N + col, z);
     }
   };
-  auto fetch = [&](int32_t c, int w) { return V::ldg((const T *)(src[w] + (uint64_t)(uint32_t)c * a.ldb_bytes)); };
+  auto fetch = [&](int32_t c, int w) { return V::ldg((const TB *)(src[w] + (uint64_t)(uint32_t)c * a.ldb_bytes)); };
   const int2 *entry = list.entry - k.p0;
   request(row);
   int32_t p = k.p0;
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirVi
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int w = 0; w < VPL; ++w) fma_row<T, VE>(acc[w], v[u], b[u][w]);
+        for (int w = 0; w < VPL; ++w) fma_row<TB, VE>(acc[w], v[u], b[u][w]);
     }
     if (p < pe) {  // the last step: entries behind the row's end are read as its last one, and not added
       typename V::Raw b[U][VPL];
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, MINB) act_product_kernel(const DirVi
       for (int u = 0; u < U; ++u)
         if (p + u * G + g < pe) {
 #pragma unroll
-          for (int w = 0; w < VPL; ++w) fma_row<T, VE>(acc[w], v[u], b[u][w]);
+          for (int w = 0; w < VPL; ++w) fma_row<TB, VE>(acc[w], v[u], b[u][w]);
         }
       p = pe;
     }
@@ -392,7 +392,7 @@ struct GradArgs {
   int64_t ldp;
   const void *dout;
   int64_t lddo;
-  void *dz;          // [rows][N] T, or nullptr
+  float *dz;         // [rows][N], or nullptr
   float *dvalues;    // [column blocks][nnz] (one block: the result itself), or nullptr
   float *dbias;      // [gridDim.x][N] partial sums, or nullptr
   int64_t nnz;
@@ -421,9 +421,10 @@ __device__ __forceinline__ float group_sums(float (&s)[U], int lane, uint32_t ma
   return x;
 }
 
-// One pass over A's rows: dz (kept in registers in fp32, so that dvalues and dbias see it unrounded; written in T for the
-// product with A transposed, whose sums over many rows are rounded to T anyway), dvalues, and the block's share of dbias. The
-// walk is the product kernel's; dout and z of the next row are requested when a row begins.
+// One pass over A's rows: dz (fp32, in registers for dvalues and dbias, and written for the product with A transposed: in 16 bits it
+// added an error of the size of dB's own rounding, and in fp16 small gradients were lost; R-MAT 18, N = 128, bf16, silu, training step:
+// 739 us with 16 bits, 794 with fp32, 850 with 24 bits in two planes), dvalues, and the block's share of dbias. The walk is the product
+// kernel's; dout and z of the next row are requested when a row begins.
 template <class T, int VE, int LPR, int VPL, int U, int MINB>
 __global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const DirView d, const GradArgs a) {
   using V = RowVec<T, VE>;
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, MINB) act_grad_rows_kernel(const Dir
           if (row < k.r1) {  // the row ends here: counted and written once
 #pragma unroll
             for (int i = 0; i < FE; ++i) bsum[w][i] += own[w][i];
-            if (a.dz && col < a.N) F::st((T *)a.dz + (int64_t)row * a.N + col, own[w]);
+            if (a.dz && col < a.N) st_f32<FE>(a.dz + (int64_t)row * a.N + col, own[w]);
           }
           if (p < pe) S::gather(own[w], dz[w]);
         }
@@ -585,12 +586,12 @@ Shape shape_of(int N, int ve, int size) {
 // Entries a step and blocks an SM: 4 and 4 measured best (R-MAT 18 forward / R-MAT 16 fp32 training / R-MAT 18 training, us: 4, 4:
 // 275 / 296 / 830; 4, 3: 276 / 377 / 895; 8, 3: 326 / 388 / 1007; 4, 5: 328 / 330 / 1044, spilling).
 constexpr int kSteps = 4, kBlocks = 4;
-template <class T, int VE, int LPR, int VPL, bool PERM>
+template <class T, class TB, int VE, int LPR, int VPL, bool PERM>
 void run_product(const DirView &d, const ActArgs &a, cudaStream_t s) {
   constexpr int U = kSteps, minb = VE * VPL >= 16 ? 2 : kBlocks;  // two vectors a lane take the registers of four blocks
   const dim3 grid((unsigned)((d.n_chunks + kThreads / 32 - 1) / (kThreads / 32)),
                   (unsigned)((a.N + VE * LPR * VPL - 1) / (VE * LPR * VPL)));
-  act_product_kernel<T, VE, LPR, VPL, U, minb, PERM><<<grid, kThreads, 0, s>>>(d, a);
+  act_product_kernel<T, TB, VE, LPR, VPL, U, minb, PERM><<<grid, kThreads, 0, s>>>(d, a);
 }
 
 template <class T, int VE, int LPR, int VPL>
@@ -619,7 +620,8 @@ void with_shape(const Shape &h, F &&f) {
   return h.VPL == 4 ? f.template operator()<1, 32, 4>() : f.template operator()<1, 32, 1>();
 }
 
-template <class T>
+// TB: T, or float (dz of 16-bit operands; vectors of 4 at most).
+template <class T, class TB>
 struct Product {
   const DirView &d;
   const ActArgs &a;
@@ -627,8 +629,12 @@ struct Product {
   cudaStream_t s;
   template <int VE, int LPR, int VPL>
   void operator()() const {
-    if (transposed) run_product<T, VE, LPR, VPL, true>(d, a, s);
-    else run_product<T, VE, LPR, VPL, false>(d, a, s);
+    if constexpr (std::is_same<T, TB>::value) {
+      if (transposed) run_product<T, TB, VE, LPR, VPL, true>(d, a, s);
+      else run_product<T, TB, VE, LPR, VPL, false>(d, a, s);
+    } else if constexpr (VE <= 4) {
+      run_product<T, TB, VE, LPR, VPL, true>(d, a, s);
+    }
   }
 };
 
@@ -644,9 +650,9 @@ struct GradRows {
   }
 };
 
-template <class T>
+template <class T, class TB>
 int product(const DirView &d, const ActArgs &a, bool transposed, int ve, cudaStream_t s) {
-  if (d.n_chunks > 0) with_shape<T>(shape_of(a.N, ve, (int)sizeof(T)), Product<T>{d, a, transposed, s});
+  if (d.n_chunks > 0) with_shape<T>(shape_of(a.N, ve, (int)sizeof(T)), Product<T, TB>{d, a, transposed, s});
   if (d.n_split > 0)
     act_join_kernel<T><<<dim3((unsigned)join_blocks(d), (unsigned)((a.N + 127) / 128)), kThreads, 0, s>>>(d, a);
   const cudaError_t e = cudaGetLastError();
@@ -717,7 +723,7 @@ GradPlan grad_plan(const dsp_pattern *p, const dsp_act_grad_desc *d) {
     at += up256(bytes);
     return o;
   };
-  g.dz = take(d->dB && d->act != DSP_ACT_NONE ? p->rows * d->N * esize(d->dtype) : 0);
+  g.dz = take(d->dB && d->act != DSP_ACT_NONE ? 4 * p->rows * d->N : 0);
   g.slots = take(d->dB ? slot_bytes(p->t, d->N) : 0);
   g.dbias = take(d->dbias ? 4ll * g.blocks * d->N : 0);
   g.dvalues = take(d->dvalues && g.col_blocks > 1 ? 4ll * g.col_blocks * p->nnz : 0);
@@ -733,7 +739,7 @@ int grad(const dsp_pattern *p, const dsp_act_grad_desc *d, char *ws, cudaStream_
     GradArgs a = {};
     a.act = d->act, a.N = d->N, a.B = d->B, a.ldb_bytes = (uint32_t)(d->ldb * sizeof(T)), a.pre = d->pre, a.ldp = d->ldp, a.dout = d->dout;
     a.lddo = d->lddo, a.nnz = p->nnz;
-    a.dz = needs_dz ? ws + g.dz : nullptr;
+    a.dz = needs_dz ? (float *)(ws + g.dz) : nullptr;
     a.dvalues = !d->dvalues || p->nnz == 0 ? nullptr : g.col_blocks > 1 ? (float *)(ws + g.dvalues) : d->dvalues;
     a.dbias = d->dbias ? (float *)(ws + g.dbias) : nullptr;
     const DirView rows = view(p->a);
@@ -747,14 +753,18 @@ int grad(const dsp_pattern *p, const dsp_act_grad_desc *d, char *ws, cudaStream_
   if (d->dB) {
     ActArgs a = {};
     a.act = DSP_ACT_NONE, a.N = d->N, a.values = d->values, a.out = d->dB, a.ldo = d->lddb;
-    a.B = needs_dz ? ws + g.dz : d->dout;
-    const int64_t ldb = needs_dz ? d->N : d->lddo;
-    a.ldb_bytes = (uint32_t)(ldb * sizeof(T));
     a.slots = (float *)(ws + g.slots);
     Align al((int)sizeof(T), d->N);
-    al.row(a.B, ldb);
     al.row(a.out, a.ldo);
-    return product<T>(view(p->t), a, true, al.ve, s);
+    if (needs_dz) {
+      a.B = ws + g.dz;
+      a.ldb_bytes = 4u * (uint32_t)d->N;
+      return product<T, float>(view(p->t), a, true, std::min(al.ve, 4), s);
+    }
+    a.B = d->dout;
+    a.ldb_bytes = (uint32_t)(d->lddo * sizeof(T));
+    al.row(a.B, d->lddo);
+    return product<T, T>(view(p->t), a, true, al.ve, s);
   }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? DSP_OK : fail(DSP_ERR_CUDA, "dsp_spmm_act_grad: %s", cudaGetErrorString(e));
@@ -794,9 +804,9 @@ extern "C" int dsp_spmm_act(const dsp_pattern *p, const dsp_act_desc *d, void *w
   ActArgs a = {d->act, d->N,   d->values, d->B,   (uint32_t)(d->ldb * esize(d->dtype)), d->bias, d->residual,
                d->ldr, d->out, d->ldo,    d->pre, d->ldp, (float *)workspace};
   cudaStream_t s = (cudaStream_t)stream;
-  if (d->dtype == DSP_F32) return product<float>(view(p->a), a, false, al.ve, s);
-  if (d->dtype == DSP_BF16) return product<__nv_bfloat16>(view(p->a), a, false, al.ve, s);
-  return product<__half>(view(p->a), a, false, al.ve, s);
+  if (d->dtype == DSP_F32) return product<float, float>(view(p->a), a, false, al.ve, s);
+  if (d->dtype == DSP_BF16) return product<__nv_bfloat16, __nv_bfloat16>(view(p->a), a, false, al.ve, s);
+  return product<__half, __half>(view(p->a), a, false, al.ve, s);
 }
 
 extern "C" int64_t dsp_spmm_act_grad_workspace(const dsp_pattern *p, const dsp_act_grad_desc *d) {
