@@ -86,7 +86,7 @@ template <int N>
 __device__ __forceinline__ void act_slopes(float (&x)[N], const float (&z)[N], int act) {
   if (act == DSP_ACT_RELU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = z[i] > 0.f ? x[i] : x[i] * 0.f;
+    for (int i = 0; i < N; ++i) x[i] = z[i] <= 0.f ? 0.f : x[i];  // where z <= 0 nothing flows, an infinity neither; NaN lets all through
   } else if (act == DSP_ACT_SILU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {

@@ -52,3 +52,18 @@ def test_small_dz_in_fp16(gpu, n):
     """dz near 1e-7 with values of 100: the products are far above fp16's smallest."""
     a = matrix("rmat")
     check_dB(a, n, F16, "silu", values=torch.full((a.nnz,), 100.0), size=2.0 ** -20)
+
+
+@pytest.mark.parametrize("t", [F32, BF16, F16])
+def test_relu_gradient_of_infinities(gpu, t):
+    """Where z <= 0 nothing flows, not even an infinity."""
+    a = csr_of([[0], [1], [2]], 3, [1.0, 1.0, 1.0])
+    p = d.SparsePattern(a, grad=True)
+    B = torch.tensor([[1.0], [-1.0], [0.0]]).repeat(1, 40).to(t).cuda()
+    _, pre = d.spmm_act_forward(p, B, act="relu", save=True)
+    dy = torch.full((3, 40), float("inf"), dtype=t)
+    dy[:, 1::2] = float("nan")
+    dB, dv, db = d.spmm_act_backward(p, dy.cuda(), B, pre, act="relu")
+    zero = torch.zeros(2, 40)
+    assert torch.equal(dB[1:].cpu().float(), zero) and torch.isinf(dB[0, ::2]).all() and torch.isnan(dB[0, 1::2]).all()
+    assert (dv[1:] == 0).all() and torch.isinf(db[::2]).all() and torch.isnan(db[1::2]).all()
