@@ -67,3 +67,12 @@ def test_relu_gradient_of_infinities(gpu, t):
     zero = torch.zeros(2, 40)
     assert torch.equal(dB[1:].cpu().float(), zero) and torch.isinf(dB[0, ::2]).all() and torch.isnan(dB[0, 1::2]).all()
     assert (dv[1:] == 0).all() and torch.isinf(db[::2]).all() and torch.isnan(db[1::2]).all()
+
+
+def test_gelu_tail(gpu):
+    """gelu keeps its relative accuracy in the negative tail: the exponent z^2 / 2 is rounded (2^-24 of z^2), the rest is 2^-20."""
+    z = torch.linspace(-12, -0.5, 4000)
+    a = csr_of([[i] for i in range(4000)], 4000, np.ones(4000))
+    out = d.spmm_act(d.SparsePattern(a), z[:, None].cuda(), act="gelu")[:, 0].cpu().double()
+    want = 0.5 * z.double() * torch.special.erfc(-z.double() * 0.5 ** 0.5)
+    near(out, want, (z.double() ** 2 * U + 2.0 ** -20) * want.abs(), "gelu")
