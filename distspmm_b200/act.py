@@ -12,7 +12,7 @@ import ctypes
 import torch
 
 from ._lib import call, dsp_act_desc, dsp_act_grad_desc, lib
-from .pattern import DTYPES, SparsePattern, ld, need, on_device, ptr, rows_of, stream_of, wants_grad, workspace
+from .pattern import DTYPES, SparsePattern, ld, need, no_tangents, on_device, ptr, rows_of, stream_of, wants_grad, workspace
 
 ACTS = {None: 0, "none": 0, "relu": 1, "silu": 2, "gelu": 3}
 
@@ -109,7 +109,8 @@ def spmm_act(p: SparsePattern, B: torch.Tensor, values=None, bias=None, residual
     residual (dB needs a pattern with grad=True).
 
     values: [nnz] fp32 in CSR order (None: A's own); bias: [N] fp32; residual: [rows, N] in B's
-    type; act: None, "relu", "silu" or "gelu" (erf form). Runs on the current stream."""
+    type; act: None, "relu", "silu" or "gelu" (erf form). Runs on the current stream. Forward-mode derivatives are refused."""
+    no_tangents(B, values, bias, residual)
     if not wants_grad(B, values, bias, residual):
         return spmm_act_forward(p, B, values, bias, residual, act)[0]
     need(isinstance(p, SparsePattern), "the first argument must be a SparsePattern")

@@ -12,7 +12,7 @@ import math
 import torch
 
 from ._lib import call, dsp_attn_decode_desc, dsp_attn_desc, dsp_attn_grad_desc, lib
-from .pattern import DTYPES, SparsePattern, need, on_device, ptr, stream_of, wants_grad, workspace
+from .pattern import DTYPES, SparsePattern, need, no_tangents, on_device, ptr, stream_of, wants_grad, workspace
 
 
 def _heads(t: torch.Tensor):
@@ -129,8 +129,9 @@ def sparse_attention(p: SparsePattern, q, k, v, scale=None, softcap=0.0, slopes=
 
     scale: of the scores (None: 1 / sqrt(dim)); softcap: scores become softcap tanh(score / softcap); slopes [heads] fp32: a
     bias of -slope |i + row_offset - j|, a constant; heads a multiple of kv_heads. Rows without entries give 0 (lse:
-    -infinity). fp32, bf16 or fp16; dim a multiple of 8 up to 256. return_lse: (out, lse) (lse has no gradient)."""
+    -infinity). fp32, bf16 or fp16; dim a multiple of 8 up to 256. return_lse: (out, lse) (lse has no gradient). Forward-mode derivatives are refused."""
     need(slopes is None or not slopes.requires_grad, "slopes are constants: they get no gradient")
+    no_tangents(q, k, v, slopes)
     if not wants_grad(q, k, v):
         out, lse = sparse_attention_forward(p, q, k, v, scale, softcap, slopes, row_offset)
         return (out, lse) if return_lse else out
@@ -145,7 +146,8 @@ def sparse_attention_decode(q, k_cache, v_cache, indptr, indices, scale=None, so
     graph sees the lists of its replay; their lengths, and so len(indices), are those of the capture at most).
 
     The last listed token is the newest: entry t of n is at distance n - 1 - t for ``slopes``. An entry outside the cache
-    makes its row NaN. No gradient."""
+    makes its row NaN. No gradient (forward-mode derivatives are refused)."""
+    no_tangents(q, k_cache, v_cache, slopes)
     need(isinstance(q, torch.Tensor) and q.is_cuda and q.dim() == 3, "q must be a CUDA tensor [rows, heads, dim]")
     dev, rows = q.get_device(), q.shape[0]
     on_device("indptr", indptr, dev, torch.int64)

@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import c_vp, call, dsp_pattern_info, lib
 from .matrix import Csr
@@ -114,6 +115,14 @@ def workspace(nbytes: int, device: torch.device) -> torch.Tensor | None:
 def stream_of(device: int) -> int:
     """The current stream of the device (cudaStream_t as int)."""
     return torch._C._cuda_getCurrentRawStream(device)
+
+
+def no_tangents(*tensors) -> None:
+    """Refuse dual tensors: only reverse-mode gradients are provided, and a tangent would be lost without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            need(not isinstance(t, torch.Tensor) or forward_ad.unpack_dual(t).tangent is None,
+                 "forward-mode derivatives are not provided")
 
 
 def wants_grad(*tensors) -> bool:
