@@ -257,7 +257,8 @@ extern "C" int dsp_pattern_create(int device, const dsp_csr *a, int flags, dsp_p
               "dsp_pattern_create: flags %d", flags);
   DSP_TRY_ARG(a->num_rows >= 0 && a->num_cols >= 0 && a->nnz >= 0, "dsp_pattern_create: negative size");
   DSP_TRY_ARG(a->nnz == 0 || a->indices, "dsp_pattern_create: null indices");
-  if (a->num_rows >= INT32_MAX || a->num_cols >= INT32_MAX || a->nnz >= INT32_MAX)
+  // kernels step past an entry's place by up to 32 in 32 bits
+  if (a->num_rows >= INT32_MAX || a->num_cols >= INT32_MAX || a->nnz > INT32_MAX - 64)
     return fail(DSP_ERR_UNSUPPORTED, "dsp_pattern_create: %lld x %lld with %lld entries: ids are 32-bit",
                 (long long)a->num_rows, (long long)a->num_cols, (long long)a->nnz);
   dsp_pattern *p = nullptr;

@@ -325,7 +325,7 @@ typedef struct dsp_pattern_info {
   int64_t device_bytes; /* all device memory the pattern holds                    */
 } dsp_pattern_info;
 
-/* rows, cols and nnz < 2^31 - 1 (UNSUPPORTED otherwise); the matrix is validated (FORMAT). Synchronous. Columns need no
+/* rows and cols < 2^31 - 1, nnz < 2^31 - 64 (UNSUPPORTED otherwise); the matrix is validated (FORMAT). Synchronous. Columns need no
  * order; columns listed twice in a row add up in dsp_spmm_act. a->values may be NULL. */
 int dsp_pattern_create(int device, const dsp_csr *a, int flags, dsp_pattern **out);
 /* No call that uses the pattern may still be running on the device. */

@@ -1,9 +1,13 @@
 """More refusals of the sparse-layer entry points that need no GPU: each comes before any CUDA call."""
+import ctypes
+
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import distspmm_b200 as d
+from distspmm_b200._lib import P, c_f32, c_i64, c_vp, dsp_csr
 
 
 def test_forward_mode_is_refused():
@@ -23,3 +27,15 @@ def test_forward_mode_is_refused():
         d.sparse_attention("A", x, x, x)
     with pytest.raises(ValueError, match="forward-mode"):
         torch.func.jvp(lambda y: d.sparse_attention("A", y, x, x), (x,), (x,))
+
+
+@pytest.mark.parametrize("nnz,code", [(2 ** 31 - 64, -6), (2 ** 31 - 40, -6), (2 ** 31 - 2, -6), (2 ** 31 - 65, -3), (5, -3)])
+def test_entries_near_the_32_bit_limit(nnz, code):
+    """A matrix that claims nnz entries: refused for its size where a step from the last ones would pass 2^31, else by validation
+    (its row pointer says 0; nothing behind it is read)."""
+    ptr, ids, val = np.zeros(1, np.int64), np.zeros(1, np.int64), np.zeros(1, np.float32)
+    c = dsp_csr()
+    c.num_rows, c.num_cols, c.nnz = 0, 1, nnz
+    c.indptr, c.indices, c.values = ptr.ctypes.data_as(P(c_i64)), ids.ctypes.data_as(P(c_i64)), val.ctypes.data_as(P(c_f32))
+    h = c_vp()
+    assert d.lib().dsp_pattern_create(0, ctypes.byref(c), 0, ctypes.byref(h)) == code
