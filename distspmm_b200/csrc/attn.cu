@@ -425,6 +425,13 @@ int check_heads(const char *who, const char *name, const void *p, int64_t row, i
   return DSP_OK;
 }
 
+// Grids count warps, one for each chunk and head, in 32 bits; tiles in CTAs.
+int check_grid(const char *who, int64_t chunks, int64_t heads, int64_t tiles) {
+  if (chunks * heads > (1ll << 32) || tiles * heads >= (1ll << 31))
+    return fail(DSP_ERR_UNSUPPORTED, "%s: %lld chunks of entries for %lld heads", who, (long long)chunks, (long long)heads);
+  return DSP_OK;
+}
+
 int check_workspace(const char *who, const void *ws, int64_t have, int64_t need) {
   if (need == 0) return DSP_OK;
   DSP_TRY_ARG(ws && have >= need, "%s: workspace of %lld bytes, %lld needed", who, (long long)(ws ? have : 0), (long long)need);
@@ -473,6 +480,7 @@ extern "C" int dsp_attn(const dsp_pattern *p, const dsp_attn_desc *d, void *work
   int rc = check_attn(who, d, p->rows, p->nnz ? p->cols : 0);
   if (rc) return rc;
   if (p->rows == 0) return DSP_OK;
+  if ((rc = check_grid(who, p->a.n_chunks, d->heads, p->at.n))) return rc;
   rc = check_workspace(who, workspace, workspace_bytes, dsp_attn_workspace(p, d));
   if (rc) return rc;
   DeviceGuard g(p->device);
@@ -510,6 +518,7 @@ extern "C" int dsp_attn_grad(const dsp_pattern *p, const dsp_attn_grad_desc *g, 
   if (p->cols > 0 && ((rc = check_heads(who, "dk", g->dk, g->dk_row, g->dk_head, d->dtype)) ||
                       (rc = check_heads(who, "dv", g->dv, g->dv_row, g->dv_head, d->dtype))))
     return rc;
+  if ((rc = check_grid(who, std::max(p->a.n_chunks, p->t.n_chunks), d->heads, std::max(p->at.n, p->tt.n)))) return rc;
   rc = check_workspace(who, workspace, workspace_bytes, dsp_attn_grad_workspace(p, d));
   if (rc) return rc;
   DeviceGuard dg(p->device);
@@ -536,6 +545,8 @@ extern "C" int dsp_attn_decode(const dsp_attn_decode_desc *g, void *workspace, i
   if (rc) return rc;
   if (g->rows == 0) return DSP_OK;
   DSP_TRY_ARG(g->indptr && (g->indices || g->nnz == 0), "%s: null index list", who);
+  const int64_t units = decode_units(g->rows, g->nnz, g->fwd.heads, g->fwd.kv_heads, decode_on_tensor_cores(g->fwd.dtype, g->fwd.dim));
+  if ((rc = check_grid(who, (row_start(g->rows, g->nnz) + units - 1) / units, g->fwd.heads, 0))) return rc;
   rc = check_workspace(who, workspace, workspace_bytes, dsp_attn_decode_workspace(g));
   if (rc) return rc;
   DeviceGuard dg(g->device);

@@ -39,3 +39,12 @@ def test_entries_near_the_32_bit_limit(nnz, code):
     c.indptr, c.indices, c.values = ptr.ctypes.data_as(P(c_i64)), ids.ctypes.data_as(P(c_i64)), val.ctypes.data_as(P(c_f32))
     h = c_vp()
     assert d.lib().dsp_pattern_create(0, ctypes.byref(c), 0, ctypes.byref(h)) == code
+
+
+@pytest.mark.parametrize("heads,kv,code", [(65535, 65535, -6), (4096, 1, -6), (1024, 1024, -1)])
+def test_more_warps_than_a_grid_has(heads, kv, code):
+    """2^21 chunks of 1024 entries for 4096 heads are 2^33 warps: refused, where the count would have been cut to 32 bits. (The last one
+    fits, and is refused for its missing workspace.)"""
+    from test_sparse_layers import decode_desc, status
+    g = decode_desc(heads=heads, kv_heads=kv, nnz=2 ** 31 - 2, keys=5)
+    assert status("dsp_attn_decode", ctypes.byref(g), None, 0, None) == code
