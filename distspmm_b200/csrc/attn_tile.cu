@@ -64,6 +64,7 @@ struct TileArgs {
   int splits;           // pieces of a row tile's list (forward)
   float *part, *part_ml;  // their partial results: [splits][rows][heads][dim], [splits][rows][heads][2]
   int *err;
+  long long wait_cycles;  // limit of a wait; 0: no copies are started, so that waits run out (tests)
 };
 
 template <int D, Mode M>
@@ -84,7 +85,7 @@ struct Cfg {
 };
 
 // Bounded wait; gives up at once where another thread of the CTA has.
-__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *dead, int *err, int code) {
+__device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile int *dead, const TileArgs &x, int code) {
   const long long t0 = clock64();
   while (true) {
     uint32_t done;
@@ -95,34 +96,34 @@ __device__ __noinline__ bool wait_slow(uint32_t bar, uint32_t parity, volatile i
         : "memory");
     if (done) return true;
     if (*dead) return false;
-    if (clock64() - t0 > kMbarWaitCycles) {
+    if (clock64() - t0 > x.wait_cycles) {
       *dead = 1;
-      atomicExch(err, code);
+      atomicExch(x.err, code);
       return false;
     }
   }
 }
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *dead, int *err, int code) {
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *dead, const TileArgs &x, int code) {
   uint32_t done;
   asm volatile(
       "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
       : "r"(bar), "r"(parity)
       : "memory");
-  return done ? true : wait_slow(bar, parity, dead, err, code);
+  return done ? true : wait_slow(bar, parity, dead, x, code);
 }
 
 // The same by a whole warp, which leaves it together.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *dead, int *err, int code) {
-  return __all_sync(0xffffffffu, wait(bar, parity, dead, err, code));
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *dead, const TileArgs &x, int code) {
+  return __all_sync(0xffffffffu, wait(bar, parity, dead, x, code));
 }
 
 // The second products of iterations 0, 1, ... complete on kAccBars barriers in turn. A thread waits for some of them only, and a
 // wait tells two phases of a barrier apart by their parity alone: with one barrier, a late thread would take phase n for phase
 // n - 2. On these, the phase before the awaited one is four iterations old and the one after it four ahead.
 constexpr int kAccBars = 4;
-__device__ __forceinline__ bool wait_acc(uint32_t bars, int it, volatile int *dead, int *err, int code) {
-  return warp_wait(bars + 8 * (it % kAccBars), (it / kAccBars) & 1, dead, err, code);
+__device__ __forceinline__ bool wait_acc(uint32_t bars, int it, volatile int *dead, const TileArgs &x, int code) {
+  return warp_wait(bars + 8 * (it % kAccBars), (it / kAccBars) & 1, dead, x, code);
 }
 
 // s -> cap tanh(k s), k = scale / cap, of N columns of this thread's row. Where no score of the warp's rows is above half the cap, as
@@ -230,6 +231,14 @@ __device__ __noinline__ void redo(const TileArgs &x, int64_t row0, int head, uin
   }
 }
 
+// A row of NaN: what a wait that gave up leaves.
+template <class T, int D>
+__device__ __forceinline__ void put_nan(const HeadsOut &o, int64_t row, int head) {
+  T *dst = (T *)o.p + row * o.row + (int64_t)head * o.head;
+#pragma unroll 1
+  for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0x7fff7fff, 0x7fff7fff, 0x7fff7fff, 0x7fff7fff);
+}
+
 // D columns of this thread's row at `addr`, times f (TWO: plus those at `addr2` times f2), to the row's place in global memory; whether
 // all were finite.
 template <class T, int D, bool TWO = false>
@@ -325,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
   const uint32_t tm_s = tm, tm_r = tm + NB * 64, tm_acc0 = tm + C::kAcc, tm_acc1 = tm_acc0 + D;
 
   if (warp == 4) {  // ------------------------------------------------------------------ loads
-    if ((threadIdx.x & 31) == 0 && iters > 0) {
+    if ((threadIdx.x & 31) == 0 && iters > 0 && x.wait_cycles > 0) {
       mbar_arrive_expect_tx(bar_static, C::kStatic * C::kStaticBytes);
       for (int c = 0; c < D / 64; ++c) {
         tma_load3(sm_a0 + c * 16384, &map_a0, c * 64, head_a, (int)row0, bar_static);
@@ -335,11 +344,11 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         const int s = it % ST, col = __ldg(x.t.col + (M == kFwd ? t1 - 1 - it : t0 + it % nt)) * kTileCols;
         const uint32_t parity = ((it / ST) & 1) ^ 1;
         const int hx = M == kDkv ? head * x.a.group + it / nt : head / x.a.group;
-        if (!wait(bar_x0_free + 8 * s, parity, dead, x.err, 1)) break;
+        if (!wait(bar_x0_free + 8 * s, parity, dead, x, 1)) break;
         mbar_arrive_expect_tx(bar_x0_full + 8 * s, C::kStreamBytes);
         for (int c = 0; c < D / 64; ++c)
           tma_load3(sm_x0 + s * C::kStreamBytes + c * 8192, &map_x0, c * 64, hx, col, bar_x0_full + 8 * s);
-        if (!wait(bar_x1_free + 8 * s, parity, dead, x.err, 2)) break;
+        if (!wait(bar_x1_free + 8 * s, parity, dead, x, 2)) break;
         mbar_arrive_expect_tx(bar_x1_full + 8 * s, C::kStreamBytes);
         for (int c = 0; c < D / 64; ++c)
           tma_load3(sm_x1 + s * C::kStreamBytes + c * 8192, &map_x1, c * 64, hx, col, bar_x1_full + 8 * s);
@@ -353,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
       auto first = [&](int it) {
         const int s = it % ST, b = it % NB;
         const uint32_t parity = (it / ST) & 1;
-        if (!wait(bar_x0_full + 8 * s, parity, dead, x.err, 3)) return false;
+        if (!wait(bar_x0_full + 8 * s, parity, dead, x, 3)) return false;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
@@ -363,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         }
         if (M == kFwd) mma_commit(bar_x0_free + 8 * s);  // K is not needed again
         if (M != kFwd) {
-          if (!wait(bar_x1_full + 8 * s, parity, dead, x.err, 4)) return false;
+          if (!wait(bar_x1_full + 8 * s, parity, dead, x, 4)) return false;
           tc_fence_after();
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
@@ -378,8 +387,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
       };
       auto second = [&](int it) {
         const int s = it % ST, b = it % NB;
-        if (!wait(bar_weights + 8 * b, (it / NB) & 1, dead, x.err, 5)) return false;
-        if (M == kFwd && !wait(bar_x1_full + 8 * s, (it / ST) & 1, dead, x.err, 6)) return false;
+        if (!wait(bar_weights + 8 * b, (it / NB) & 1, dead, x, 5)) return false;
+        if (M == kFwd && !wait(bar_x1_full + 8 * s, (it / ST) & 1, dead, x, 6)) return false;
         tc_fence_after();
         const uint32_t x0 = sm_x0 + s * C::kStreamBytes, x1 = sm_x1 + s * C::kStreamBytes;
         // 16 streamed rows each: 8 columns of weights, 2048 bytes of the stream's image
@@ -414,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         mma_commit(bar_acc + 8 * (it % kAccBars));
         return true;
       };
-      bool ok = wait(bar_static, 0, dead, x.err, 7);
+      bool ok = wait(bar_static, 0, dead, x, 7);
       tc_fence_after();
       ok = ok && first(0);
       for (int it = 0; ok && it < iters; ++it) {
@@ -445,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         const int b = it % NB;
         const int now_mask = walk.mask, now_col = walk.col;
         const uint64_t now_bits = walk.bits;
-        if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x.err, 8))) break;
+        if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x, 8))) break;
         tc_fence_after();
         float u[64];
         {
@@ -501,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
           m = m2;
           l *= less;
           if (it > 0) {  // the sum so far, once the previous product has been added to it
-            if (!(ok = wait_acc(bar_acc, it - 1, dead, x.err, 9))) break;
+            if (!(ok = wait_acc(bar_acc, it - 1, dead, x, 9))) break;
             tc_fence_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
@@ -536,7 +545,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         tc_fence_before();
         mbar_arrive(bar_weights + 8 * b);
       }
-      if (ok && iters > 0) ok = wait_acc(bar_acc, iters - 1, dead, x.err, 10);
+      if (ok && iters > 0) ok = wait_acc(bar_acc, iters - 1, dead, x, 10);
       tc_fence_after();
       const bool live = row < n_rows;
       if (ok && x.splits > 1) {
@@ -565,6 +574,13 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         T *dst = (T *)x.a.out.p + row * x.a.out.row + (int64_t)head * x.a.out.head;
         for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(0, 0, 0, 0);
         if (x.a.lse) x.a.lse[row * x.a.heads + head] = -INFINITY;
+      } else if (!ok && live) {  // a wait gave up
+        if (x.splits > 1) {
+          x.part_ml[2 * (((int64_t)blockIdx.y * n_rows + row) * x.a.heads + head)] = NAN;
+        } else {
+          put_nan<T, D>(x.a.out, row, head);
+          if (x.a.lse) x.a.lse[row * x.a.heads + head] = NAN;
+        }
       }
     } else {
       const bool live = row < n_rows;
@@ -627,8 +643,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         const int64_t col = (int64_t)now_col * kTileCols;
         const float k0 = slope2 * (M == kDq ? -(float)(row + x.a.row_offset - col) : (float)(col + x.a.row_offset - row));
         const float sign = slope2 < 0.f ? 1.f : -1.f;
-        if (M == kDkv && !(ok = warp_wait(bar_stats, it & 1, dead, x.err, 13))) break;
-        if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x.err, 11))) break;
+        if (M == kDkv && !(ok = warp_wait(bar_stats, it & 1, dead, x, 13))) break;
+        if (!(ok = warp_wait(bar_scores + 8 * b, (it / NB) & 1, dead, x, 11))) break;
         tc_fence_after();
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
@@ -729,7 +745,7 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
         tc_fence_before();
         mbar_arrive(bar_weights + 8 * b);
       }
-      if (ok && iters > 0) ok = wait_acc(bar_acc, iters - 1, dead, x.err, 12);
+      if (ok && iters > 0) ok = wait_acc(bar_acc, iters - 1, dead, x, 12);
       tc_fence_after();
       if (ok && iters > 0) {
         bool fine;
@@ -758,6 +774,10 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
             *reinterpret_cast<uint4 *>((T *)x.a.dv.p + row * x.a.dv.row + (int64_t)head * x.a.dv.head + c) = zero;
           }
         }
+      } else if (!ok && live) {  // a wait gave up
+        put_nan<T, D>(M == kDq ? x.a.dq : x.a.dk, row, head);
+        if (M == kDkv) put_nan<T, D>(x.a.dv, row, head);
+        if (M == kDq) x.a.delta[row * x.a.heads + head] = NAN;
       }
     }
   }
@@ -777,11 +797,16 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const __grid_consta
   const int64_t row = item / x.a.heads;
   const int h = (int)(item - row * x.a.heads), lane = threadIdx.x & 31;
   float m = -INFINITY, l = 0.f, acc[D / 32];
+  bool lost = false;  // a piece's wait gave up
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) acc[i] = 0.f;
   for (int z = 0; z < x.splits; ++z) {
     const int64_t at = z * n + item;
     const float m2 = x.part_ml[2 * at], l2 = x.part_ml[2 * at + 1];
+    if (m2 != m2) {
+      lost = true;
+      break;
+    }
     const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
     const float f1 = exp2_approx(m - base), f2 = exp2_approx(m2 - base);
     l = l * f1 + l2 * f2;
@@ -789,7 +814,7 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const __grid_consta
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) acc[i] = acc[i] * f1 + x.part[at * D + lane + 32 * i] * f2;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = lost ? NAN : l == 0.f ? 0.f : 1.f / l;
   bool fine = l == l;
   T *dst = (T *)x.a.out.p + row * x.a.out.row + (int64_t)h * x.a.out.head;
 #pragma unroll
@@ -798,8 +823,8 @@ __global__ void __launch_bounds__(256) attn_tile_join_kernel(const __grid_consta
     fine &= isfinite(o);
     dst[lane + 32 * i] = T(o);
   }
-  if (x.a.lse && lane == 0) x.a.lse[item] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-  if (__any_sync(0xffffffffu, !fine)) redo<T, D, kFwd>(x, row, h, 1u);
+  if (x.a.lse && lane == 0) x.a.lse[item] = lost ? NAN : l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+  if (!lost && __any_sync(0xffffffffu, !fine)) redo<T, D, kFwd>(x, row, h, 1u);
 }
 
 // delta0_i = dout_i . out_i of each row and head, a warp each (fp16: and the largest finite |dout|, [heads][rows]).
@@ -876,6 +901,7 @@ int launch(const dsp_pattern *p, TileArgs x, cudaStream_t s) {
   x.rows = {view(M == kDkv ? p->t : p->a)};
   x.n_heads = M == kDkv ? kv_heads : x.a.heads;
   x.err = p->d_err;
+  x.wait_cycles = p->wait_cycles;
   // an operand without rows is never loaded: any valid map will do
   const Heads q = x.a.q, k = p->cols ? x.a.k : q, v = p->cols ? x.a.v : q, o = M == kFwd ? q : x.a.dout;
   const int64_t nq = p->rows, nk = p->cols ? p->cols : p->rows;

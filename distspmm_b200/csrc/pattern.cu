@@ -1,9 +1,11 @@
 // pattern.cu — dsp_pattern: a CSR matrix prepared once for the fused product (act.cu) and for attention (attn.cu).
+#include <stdlib.h>
 #include <string.h>
 
 #include <algorithm>
 #include <new>
 
+#include "mbar.cuh"
 #include "pattern.h"
 
 namespace dsp {
@@ -203,6 +205,8 @@ int create(int device, const dsp_csr *a, int flags, dsp_pattern *p) {
   p->rows = M;
   p->cols = K;
   p->nnz = a->nnz;
+  const char *limit = getenv("DSP_ATTN_WAIT_CYCLES");  // of the tile kernels' waits; 0: they start no copies and so run out at once (tests)
+  p->wait_cycles = limit ? std::max(0ll, atoll(limit)) : kMbarWaitCycles;
   HostDir h;
   h.ptr.resize(M + 1);
   h.cols.resize(a->nnz);

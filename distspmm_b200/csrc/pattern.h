@@ -109,6 +109,7 @@ struct dsp_pattern {
   bool tiled = false;  // the tile form of a (and of t) exists
   dsp::PatternTiles at, tt;
   int *d_err = nullptr;  // set by a kernel whose bounded wait gave up
+  long long wait_cycles = 0;  // their limit
   int64_t device_bytes = 0;
   std::vector<void *> allocs;
 };

@@ -57,7 +57,7 @@ class SparsePattern:
 
     def check_error(self) -> None:
         """After the streams were synchronised: raise DspError if an attention kernel's bounded wait
-        gave up (the flag is cleared)."""
+        gave up (its rows are NaN; the flag is cleared)."""
         call("dsp_pattern_check_error", self._h)
 
     def close(self) -> None:

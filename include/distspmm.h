@@ -332,7 +332,7 @@ int dsp_pattern_create(int device, const dsp_csr *a, int flags, dsp_pattern **ou
 void dsp_pattern_destroy(dsp_pattern *p);
 int dsp_pattern_info_get(const dsp_pattern *p, dsp_pattern_info *info);
 /* After the streams of earlier calls were synchronised: DSP_OK, or DSP_ERR_TIMEOUT if an attention kernel's bounded wait on
- * its own copies or products gave up; the flag is cleared. */
+ * its own copies or products gave up (the rows it was to write are NaN); the flag is cleared. */
 int dsp_pattern_check_error(dsp_pattern *p);
 
 /* ---------------------------------------------------------------- sparse layers: product with an epilogue */
