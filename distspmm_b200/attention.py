@@ -109,16 +109,17 @@ class _SparseAttention(torch.autograd.Function):
     def forward(ctx, p, q, k, v, scale, softcap, slopes, row_offset):
         _pattern(p, grad=any(ctx.needs_input_grad))
         out, lse = sparse_attention_forward(p, q, k, v, scale, softcap, slopes, row_offset)
-        ctx.p, ctx.opt = p, (scale, softcap, slopes, row_offset)
-        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.p, ctx.opt = p, (scale, softcap)
+        ctx.row_offset = row_offset
+        ctx.save_for_backward(q, k, v, out, lse, slopes)  # slopes too: a change in place before the backward pass is noticed
         ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _):
-        q, k, v, out, lse = ctx.saved_tensors
-        dq, dk, dv = sparse_attention_backward(ctx.p, dout, q, k, v, out, lse, *ctx.opt)
+        q, k, v, out, lse, slopes = ctx.saved_tensors
+        dq, dk, dv = sparse_attention_backward(ctx.p, dout, q, k, v, out, lse, *ctx.opt, slopes, ctx.row_offset)
         return None, dq, dk, dv, None, None, None, None
 
 

@@ -230,3 +230,16 @@ def test_infinite_values_in_a_cache(gpu, t, dim):
         if (at == idx[500]).any():
             o[:, :, 4] = -math.inf
         near(got[r:r + 1], o, tol["out"], "out")
+
+
+def test_slopes_changed_before_the_backward_pass(gpu):
+    """The gradient of other slopes than the forward's is no gradient: autograd refuses, as for q, k and v."""
+    a = positional("window", 40, window=9)
+    p = d.SparsePattern(a, grad=True, attention=True)
+    q, k, v, dout = (x.cuda() for x in inputs(40, 40, 2, 1, 64, BF16, 1))
+    slopes = slopes_of(2).cuda()
+    out = d.sparse_attention(p, q.requires_grad_(), k, v, slopes=slopes)
+    out.backward(dout, retain_graph=True)
+    slopes.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward(dout)
