@@ -39,7 +39,7 @@ class SparsePattern:
         call("dsp_pattern_create", device, ctypes.byref(c), self.GRAD * self.grad + self.ATTENTION * self.attention +
              self.FORMS[form], ctypes.byref(h))
         self._h = h
-        self._host_values = a.values
+        self._host_values = a.values.copy()  # those of now, whatever becomes of a
         self._values = None
 
     @property
@@ -48,6 +48,7 @@ class SparsePattern:
         before capturing a graph that relies on it)."""
         if self._values is None:
             self._values = torch.from_numpy(self._host_values).to(torch.device("cuda", self.device))
+            self._host_values = None
         return self._values
 
     def info(self) -> dict:

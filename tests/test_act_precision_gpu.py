@@ -76,3 +76,12 @@ def test_gelu_tail(gpu):
     out = d.spmm_act(d.SparsePattern(a), z[:, None].cuda(), act="gelu")[:, 0].cpu().double()
     want = 0.5 * z.double() * torch.special.erfc(-z.double() * 0.5 ** 0.5)
     near(out, want, (z.double() ** 2 * U + 2.0 ** -20) * want.abs(), "gelu")
+
+
+def test_a_pattern_keeps_the_values_it_was_made_with(gpu):
+    a = csr_of([[0], [1]], 2, [1.0, 2.0])
+    p = d.SparsePattern(a)
+    a.values[:] = 5
+    B = torch.ones(2, 4, device="cuda")
+    assert torch.equal(d.spmm_act(p, B).cpu(), torch.tensor([[1.0] * 4, [2.0] * 4]))
+    assert torch.equal(p.values.cpu(), torch.tensor([1.0, 2.0]))
