@@ -31,7 +31,6 @@ struct ListRows {
   __device__ int64_t col(int64_t p) const { return __ldg(indices + p); }
   __device__ float distance(const AttnArgs &, int64_t, int64_t end, int64_t p, int64_t) const { return (float)(end - 1 - p); }
   __device__ bool in_range(int64_t c) const { return c >= 0 && c < keys; }
-  __device__ int32_t units() const { return L; }
 };
 
 // Whether attn_decode.cu's kernel takes a call (else the gather kernel of attn.cu).

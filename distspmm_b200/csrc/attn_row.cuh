@@ -20,7 +20,6 @@ struct PlanRows {
     return fabsf((float)(row + a.row_offset - col));
   }
   __device__ bool in_range(int64_t) const { return true; }
-  __device__ int32_t units() const { return d.L; }
 };
 
 // A chunk of a prepared pattern with its lists in shared memory: one coalesced read instead of a wait for each step.

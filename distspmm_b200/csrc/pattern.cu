@@ -157,7 +157,7 @@ int put_dir(dsp_pattern *p, int32_t n, const HostDir &h, PatternDir *d) {
   d->n_split = (int32_t)h.split_row.size();
   d->n_long = h.n_long;
   int rc;
-  if ((rc = put(p, h.ptr, &d->ptr)) || (rc = put(p, h.row_of, &d->row_of)) || (rc = put(p, h.cols, &d->cols)) ||
+  if ((rc = put(p, h.ptr, &d->ptr)) || (rc = put(p, h.cols, &d->cols)) ||
       (rc = put(p, h.row0, &d->row0)) || (rc = put(p, h.nz0, &d->nz0)) || (rc = put(p, h.split_row, &d->split_row)))
     return rc;
   if (!h.perm.empty() && (rc = put(p, h.perm, &d->perm))) return rc;

@@ -29,7 +29,6 @@ struct PatternDir {
   int32_t L = 0;          // units of a chunk
   int32_t n_split = 0, n_long = 0;
   int32_t *ptr = nullptr;        // [n + 1]
-  int32_t *row_of = nullptr;     // [nnz]
   int32_t *cols = nullptr;       // [nnz]
   int32_t *perm = nullptr;       // [nnz] place of the entry in A's own order (transposed orientation only)
   int32_t *row0 = nullptr;       // [n_chunks + 1]
@@ -40,11 +39,11 @@ struct PatternDir {
 // Kernel-side view (passed by value).
 struct DirView {
   int32_t n, n_chunks, L, n_split, n_long;
-  const int32_t *ptr, *row_of, *cols, *perm, *row0, *nz0, *split_row;
+  const int32_t *ptr, *cols, *perm, *row0, *nz0, *split_row;
 };
 
 inline DirView view(const PatternDir &d) {
-  return {d.n, d.n_chunks, d.L, d.n_split, d.n_long, d.ptr, d.row_of, d.cols, d.perm, d.row0, d.nz0, d.split_row};
+  return {d.n, d.n_chunks, d.L, d.n_split, d.n_long, d.ptr, d.cols, d.perm, d.row0, d.nz0, d.split_row};
 }
 
 // Blocks of 8 warps that join the cut rows: a block for each long one, a warp for each other.
@@ -56,7 +55,7 @@ struct HostDir {
   int32_t L = 0, n_chunks = 0, n_long = 0;
 };
 
-// Fill row_of, chunks and cut rows from ptr.
+// Fill row_of (which stays on the host), chunks and cut rows from ptr.
 void pattern_chunks(int32_t n, HostDir *d);
 
 // The tile form: tiles of kTileRows x kTileCols entries that hold at least one entry, by row tiles, columns rising. A tile

@@ -48,7 +48,6 @@ class SparsePattern:
         before capturing a graph that relies on it)."""
         if self._values is None:
             self._values = torch.from_numpy(self._host_values).to(torch.device("cuda", self.device))
-            self._host_values = None
         return self._values
 
     def info(self) -> dict:
