@@ -78,7 +78,9 @@ struct Cfg {
   static constexpr int kCols = kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
   static constexpr int kStaticBytes = 128 * D * 2, kStreamBytes = 64 * D * 2;
   static constexpr int kSmemUsed = kStatic * kStaticBytes + 2 * ST * kStreamBytes + 1024;
-  // no more CTAs on an SM than tensor memory has room for: an allocation never waits for another CTA's end
+  // no more CTAs of a launch on an SM than tensor memory has room for: their allocations do not wait for one another. CTAs of
+  // different launches (another stream's forward of 256 columns beside a backward of 512) may still meet on an SM: the later one's
+  // allocation then waits until the earlier one ends, as it will, since all its own waits have limits.
   static constexpr int kCtas = 512 / kCols;
   static constexpr int kSmemLeast = 232448 / (kCtas + 1) + 1024;
   static constexpr int kSmem = kSmemUsed > kSmemLeast ? kSmemUsed : kSmemLeast;
@@ -298,7 +300,6 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
     t0 = t0 + (int)((int64_t)n * z / x.splits);
   }
   const int nt = t1 - t0, iters = M == kDkv ? nt * x.a.group : nt;
-  const int head_a = M == kDkv ? head : head;                      // head of the stationary operands
   const int64_t row0 = (int64_t)rt * kTileRows;
 
   const uint32_t sm = (smem_addr(raw_smem) + 1023u) & ~1023u;
@@ -337,8 +338,8 @@ __global__ void __launch_bounds__(kThreads, Cfg<D, M>::kCtas > 2 ? 2 : Cfg<D, M>
     if ((threadIdx.x & 31) == 0 && iters > 0 && x.wait_cycles > 0) {
       mbar_arrive_expect_tx(bar_static, C::kStatic * C::kStaticBytes);
       for (int c = 0; c < D / 64; ++c) {
-        tma_load3(sm_a0 + c * 16384, &map_a0, c * 64, head_a, (int)row0, bar_static);
-        if (C::kStatic == 2) tma_load3(sm_a1 + c * 16384, &map_a1, c * 64, head_a, (int)row0, bar_static);
+        tma_load3(sm_a0 + c * 16384, &map_a0, c * 64, head, (int)row0, bar_static);
+        if (C::kStatic == 2) tma_load3(sm_a1 + c * 16384, &map_a1, c * 64, head, (int)row0, bar_static);
       }
       for (int it = 0; it < iters; ++it) {
         const int s = it % ST, col = __ldg(x.t.col + (M == kFwd ? t1 - 1 - it : t0 + it % nt)) * kTileCols;
@@ -902,18 +903,16 @@ int launch(const dsp_pattern *p, TileArgs x, cudaStream_t s) {
   x.n_heads = M == kDkv ? kv_heads : x.a.heads;
   x.err = p->d_err;
   x.wait_cycles = p->wait_cycles;
-  // an operand without rows is never loaded: any valid map will do
-  const Heads q = x.a.q, k = p->cols ? x.a.k : q, v = p->cols ? x.a.v : q, o = M == kFwd ? q : x.a.dout;
-  const int64_t nq = p->rows, nk = p->cols ? p->cols : p->rows;
-  const int hk = p->cols ? kv_heads : x.a.heads;
+  const Heads q = x.a.q, k = x.a.k, v = x.a.v, o = M == kFwd ? q : x.a.dout;  // the forward has no second stationary operand
+  const int64_t nq = p->rows, nk = p->cols;
   CUtensorMap a0, a1, x0, x1;
   bool ok;
   if (M == kDkv)
-    ok = encode(&a0, k, nk, hk, D, bf16, 128) && encode(&a1, v, nk, hk, D, bf16, 128) &&
-         (nq == 0 || (encode(&x0, q, nq, x.a.heads, D, bf16, 64) && encode(&x1, o, nq, x.a.heads, D, bf16, 64)));
+    ok = encode(&a0, k, nk, kv_heads, D, bf16, kTileRows) && encode(&a1, v, nk, kv_heads, D, bf16, kTileRows) &&
+         encode(&x0, q, nq, x.a.heads, D, bf16, kTileCols) && encode(&x1, o, nq, x.a.heads, D, bf16, kTileCols);
   else
-    ok = encode(&a0, q, nq, x.a.heads, D, bf16, 128) && encode(&a1, o, nq, x.a.heads, D, bf16, 128) &&
-         encode(&x0, k, nk, hk, D, bf16, 64) && encode(&x1, v, nk, hk, D, bf16, 64);
+    ok = encode(&a0, q, nq, x.a.heads, D, bf16, kTileRows) && encode(&a1, o, nq, x.a.heads, D, bf16, kTileRows) &&
+         encode(&x0, k, nk, kv_heads, D, bf16, kTileCols) && encode(&x1, v, nk, kv_heads, D, bf16, kTileCols);
   if (!ok) return fail(DSP_ERR_CUDA, "dsp_attn: a tensor map was refused");
   const cudaError_t e = cudaFuncSetAttribute((const void *)attn_tile_kernel<T, D, M>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
   if (e != cudaSuccess) return fail(DSP_ERR_CUDA, "dsp_attn: %s", cudaGetErrorString(e));
