@@ -205,8 +205,12 @@ int create(int device, const dsp_csr *a, int flags, dsp_pattern *p) {
   p->rows = M;
   p->cols = K;
   p->nnz = a->nnz;
-  const char *limit = getenv("DSP_ATTN_WAIT_CYCLES");  // of the tile kernels' waits; 0: they start no copies and so run out at once (tests)
-  p->wait_cycles = limit ? std::max(0ll, atoll(limit)) : kMbarWaitCycles;
+  p->wait_cycles = kMbarWaitCycles;
+  if (const char *limit = getenv("DSP_ATTN_WAIT_CYCLES")) {  // of the tile kernels' waits; 0: they start no copies and so run out at once (tests)
+    char *end = nullptr;
+    const long long n = strtoll(limit, &end, 10);
+    if (end != limit && *end == 0 && n >= 0) p->wait_cycles = n;
+  }
   HostDir h;
   h.ptr.resize(M + 1);
   h.cols.resize(a->nnz);

@@ -69,3 +69,13 @@ def test_forward_beside_backward_of_another_stream(gpu):
     want = [sets[0][2], sets[1][2], sets[0][1], sets[1][1]]
     for i, g in enumerate(got):
         assert all(torch.equal(y, z) for y, z in zip(g, want[i % 4]))
+
+
+@pytest.mark.parametrize("text", ["", "fast", "-1", "10 s"])
+def test_limits_that_are_no_number_are_ignored(gpu, monkeypatch, text):
+    monkeypatch.setenv("DSP_ATTN_WAIT_CYCLES", text)
+    a = positional("window", 200, window=50)
+    p = d.SparsePattern(a, attention=True, form="tiles")
+    q, k, v, _ = (x.cuda() for x in inputs(200, 200, 2, 1, 64, torch.bfloat16, 3))
+    assert torch.isfinite(d.sparse_attention(p, q, k, v)).all()
+    p.check_error()
