@@ -75,10 +75,14 @@ struct HostTiles {
   std::vector<uint64_t> words;
   int32_t max_tiles = 0;
 };
-// Entries per tile from which the tile form is built and used. A tile costs the same however many entries it has, a row's entry
-// by itself; 8 heads of 64, training step, tiles / rows in us: R-MAT 11 (92 entries a tile) 176 / 150, 4096 rows of 60 random
-// columns (120) 371 / 463, R-MAT 10 (167) 108 / 100, 2048 rows of 60 (240) 176 / 252, a window of 8 over 4096 rows (345) 72 / 119.
-constexpr int64_t kTileFill = 160;
+// Entries per tile, on average over the matrix, from which the tile form is built and used. A tile costs the same however many entries it
+// has, a row's entry by itself. Measured with 8 heads of 64, bf16, training step (forward), tiles / rows in us, by entries a tile:
+//   uniform rows     120: 448 / 488 (103 / 125)   160: 201 / 183 (47 / 49)   200: 448 / 670 (102 / 163)   240: 201 / 253 (47 / 68)
+//   R-MAT 11, 10, 9   92: 203 / 146 (47 / 43)     165: 111 / 93 (27 / 27)    300: 66 / 58 (17 / 19)
+//   a window of 8    345: 47 / 119 (12 / 35)
+// One threshold cannot be right for all: skewed graphs leave many thin tiles beside full ones. 180 costs the two it misses (uniform 120,
+// R-MAT 9) 9 and 14 %.
+constexpr int64_t kTileFill = 180;
 // False (and out untouched) where tiles would hold fewer than kTileFill entries on average.
 bool build_tiles(int32_t n, int32_t n_cols, const HostDir &d, bool always, HostTiles *out);
 
