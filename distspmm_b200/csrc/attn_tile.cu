@@ -19,7 +19,7 @@
 //
 // Rounding: weights enter the second products as hi + lo, two parts of the operands' 16-bit type, and so do the score gradients (2^-16
 // of a value is lost at most). One part alone put a second rounding of the result's size into out and dv (window case below: 218
-// instead of 257 us forward; documents: 115 instead of 126 us dk and dv). The first delta0 = dout . out has a rounded
+// instead of 260 us forward; documents: 115 instead of 126 us dk and dv). The first delta0 = dout . out has a rounded
 // out; so dq = sum p c (dp - delta0) k - g sum p c k with g = sum p (dp - delta0) = delta - delta0, whose weights p c may be rounded once, as g is
 // but a rounding itself; delta0 + g is what dk takes. fp16 has few exponents:
 // weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is scaled by a power of two that brings the
@@ -34,7 +34,7 @@
 // first 384 since 128 x 64 x 16 steps read shared memory 1.5 times as fast as it delivers; its exponentials take 512 on the special
 // function units. The forward takes some 1900 cycles a tile and SM: neither of the two bounds it, but the chain of waits from scores
 // to weights to products, which two CTAs on an SM (tensor memory and registers allow no third) overlap only in part. Measured: 8192
-// rows, window 1024 with 64 first keys, 32 query heads over 8 of 128, distance bias: 257 us, 531 TFLOP/s of listed entries; documents,
+// rows, window 1024 with 64 first keys, 32 query heads over 8 of 128, distance bias: 260 us, 525 TFLOP/s of listed entries; documents,
 // 6001 rows, 16 heads of 64, cap: 67 us forward, 106 dq, 126 dk and dv.
 #include <algorithm>
 #include <type_traits>
