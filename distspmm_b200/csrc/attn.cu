@@ -83,8 +83,8 @@ __global__ void __launch_bounds__(kThreads, VPL == 1 ? 3 : 2) attn_dq_kernel(con
   for (int32_t row = r0; row <= r1; ++row) {
     if (row == r1 && p >= p1) break;
     const int32_t pe = row < r1 ? d.ptr(row + 1) : p1;
-    float delta, x[VPL][VE], y[VPL][VE];
-    attend_dq<H, LPR>(d, a, row, h, p, pe, delta, x, y);
+    float gap, delta0, x[VPL][VE], y[VPL][VE];
+    attend_dq<H, LPR>(d, a, row, h, p, pe, gap, delta0, x, y);
     const bool cut_head = row == r0 && head_cut;
     if (cut_head || row == r1) {
       const int64_t slot = (cut_head ? 2 * chunk : 2 * chunk + 1) * a.heads + h;
@@ -92,14 +92,14 @@ __global__ void __launch_bounds__(kThreads, VPL == 1 ? 3 : 2) attn_dq_kernel(con
         H::store_f32(a.slots + slot * 2 * a.dim, lane, a.dim, x);
         H::store_f32(a.slots + slot * 2 * a.dim + a.dim, lane, a.dim, y);
       }
-      if ((threadIdx.x & 31) == 0) a.slot_ml[2 * slot] = delta, a.slot_ml[2 * slot + 1] = 0.f;
+      if ((threadIdx.x & 31) == 0) a.slot_ml[2 * slot] = gap, a.slot_ml[2 * slot + 1] = delta0;
     } else {
 #pragma unroll
       for (int w = 0; w < VPL; ++w)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) x[w][i] = (x[w][i] - delta * y[w][i]) * a.scale;
+        for (int i = 0; i < VE; ++i) x[w][i] = (x[w][i] - gap * y[w][i]) * a.scale;
       if (g == 0) H::store(a.dq, row, h, lane, a.dim, x);
-      if ((threadIdx.x & 31) == 0) a.delta[(int64_t)row * a.heads + h] = delta;
+      if ((threadIdx.x & 31) == 0) a.delta[(int64_t)row * a.heads + h] = delta0 + gap;
     }
     p = pe;
   }
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 5) attn_join_kernel(const __grid_con
 }
 
 // Partials of cut rows (gradients), 2 dim floats per slot and head, summed in a fixed order. DQ: the sums x and y of a row, its
-// delta - delta0 and delta0 (attn_graph.cu; attend_dq: 0); else dk and dv of a key.
+// delta - delta0 and delta0 (attend_dq); else dk and dv of a key.
 template <class T, bool DQ>
 __global__ void __launch_bounds__(kThreads, 4) attn_sum_kernel(const __grid_constant__ DirView d, int n_heads, const __grid_constant__ AttnArgs a) {
   __shared__ float part[8][512], part_delta[8];

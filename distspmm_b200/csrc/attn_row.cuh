@@ -192,12 +192,13 @@ __device__ __noinline__ void attend_again(const Rows &d, const AttnArgs &a, int6
   put_row<H, D / 8>(a, row, h, m, l, y);
 }
 
-// The entries [p, pe) of a row for head h, for dq. With c = 1 - tanh^2: delta = sum p dp, x = sum p c dp k, y = sum p c k, so
-// that dq = scale (x - delta y) needs one pass, and delta is not that of a rounded out (in a row of one entry the two parts
-// cancel exactly, as they should).
+// The entries [p, pe) of a row for head h, for dq. With c = 1 - tanh^2 and delta0 = dout . out (out may be rounded): gap = sum p (dp -
+// delta0) = delta - delta0, x = sum p c (dp - delta0) k, y = sum p c k, so that dq = scale (x - gap y) needs one pass. Differences from
+// delta0 are as small as ds itself: what the weights are off together (lse is rounded, by 2^-24 of its size) scales dq, and
+// leaves nothing of delta in it.
 template <class H, int LPR, class Rows, int VPL, int VE>
 __device__ __forceinline__ void attend_dq(const Rows &d, const AttnArgs &a, int64_t row, int h, int32_t p, int32_t pe,
-                                          float &delta, float (&x)[VPL][VE], float (&y)[VPL][VE]) {
+                                          float &gap, float &delta0, float (&x)[VPL][VE], float (&y)[VPL][VE]) {
   constexpr int G = 32 / LPR, U = 4;
   const int lane = threadIdx.x % LPR, g = (threadIdx.x & 31) / LPR;
   const float slope = a.slopes ? __ldg(a.slopes + h) : 0.f, inv_cap = a.cap > 0.f ? 1.f / a.cap : 0.f;
@@ -207,8 +208,10 @@ __device__ __forceinline__ void attend_dq(const Rows &d, const AttnArgs &a, int6
   H::widen(raw, q);
   H::fetch(a.dout, row, h, lane, a.dim, true, raw);
   H::widen(raw, dout);
+  H::fetch(a.o, row, h, lane, a.dim, true, raw);
+  delta0 = group_sum<LPR>(H::dot(dout, raw));
   const float lse2 = a.lse[row * a.heads + h] * kLog2e;
-  delta = 0.f;
+  gap = 0.f;
 #pragma unroll
   for (int w = 0; w < VPL; ++w)
 #pragma unroll
@@ -227,10 +230,10 @@ __device__ __forceinline__ void attend_dq(const Rows &d, const AttnArgs &a, int6
     for (int u = 0; u < U; ++u) {
       float th = 0.f;
       const float s = score2(a, group_sum<LPR>(H::dot(q, k[u])), inv_cap, slope, d.distance(a, row, 0, 0, c[u]), th);
-      const float dp = group_sum<LPR>(H::dot(dout, v[u]));
+      const float dp = group_sum<LPR>(H::dot(dout, v[u])) - delta0;
       if (b + u * G + g < pe) {
         const float w = lse2 == -INFINITY ? 0.f : exp2_approx(s - lse2), wc = w * (1.f - th * th);
-        delta = fmaf(w, dp, delta);
+        gap = fmaf(w, dp, gap);
         H::add(x, wc * dp, k[u]);
         H::add(y, wc, k[u]);
       }
@@ -238,7 +241,7 @@ __device__ __forceinline__ void attend_dq(const Rows &d, const AttnArgs &a, int6
   }
 #pragma unroll
   for (int o = LPR; o < 32; o <<= 1) {
-    delta += __shfl_xor_sync(0xffffffffu, delta, o);
+    gap += __shfl_xor_sync(0xffffffffu, gap, o);
 #pragma unroll
     for (int w = 0; w < VPL; ++w)
 #pragma unroll

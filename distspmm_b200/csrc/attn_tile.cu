@@ -213,16 +213,16 @@ __device__ __noinline__ void redo(const TileArgs &x, int64_t row0, int head, uin
     const int64_t row = row0 + __ffs(bad) - 1;
     bad &= bad - 1;
     const int64_t p = x.rows.ptr(row), pe = x.rows.ptr(row + 1);
-    float y[1][8], z[1][8], m, l;
+    float y[1][8], z[1][8], m, l;  // dq: m is delta - delta0, l is delta0
     if constexpr (M == kFwd) {
       attend<H, D / 8>(x.rows, x.a, row, head, p, pe, pe, m, l, y);
       put_row<H, D / 8>(x.a, row, head, m, l, y);
     } else if constexpr (M == kDq) {
-      attend_dq<H, D / 8>(x.rows, x.a, row, head, p, pe, m, y, z);
+      attend_dq<H, D / 8>(x.rows, x.a, row, head, p, pe, m, l, y, z);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[0][i] = (y[0][i] - m * z[0][i]) * x.a.scale;
       if (g == 0) H::store(x.a.dq, row, head, lane, D, y);
-      if ((threadIdx.x & 31) == 0) x.a.delta[row * x.a.heads + head] = m;
+      if ((threadIdx.x & 31) == 0) x.a.delta[row * x.a.heads + head] = l + m;
     } else {
       attend_dkv<H, D / 8>(x.rows, x.a, row, head, p, pe, y, z);
       if (g == 0) {

@@ -14,10 +14,10 @@ pytestmark = pytest.mark.gpu
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
-def check(form, a, q, k, v, dout, cap=0.0, scale=None, slopes=None, names=("out", "lse", "dq", "dk", "dv"), depth=None):
+def check(form, a, q, k, v, dout, cap=0.0, scale=None, slopes=None, names=("out", "lse", "dq", "dk", "dv"), depth=None, offset=0):
     t, dim = q.dtype, q.shape[2]
     p = d.SparsePattern(a, grad=True, attention=True, form=form)
-    opt = dict(scale=scale, softcap=cap, slopes=None if slopes is None else slopes.cuda())
+    opt = dict(scale=scale, softcap=cap, slopes=None if slopes is None else slopes.cuda(), row_offset=offset)
     qc, kc, vc, dc = (x.cuda() for x in (q, k, v, dout))
     out, lse = d.sparse_attention_forward(p, qc, kc, vc, **opt)
     got = dict(out=out, lse=lse)
@@ -25,10 +25,10 @@ def check(form, a, q, k, v, dout, cap=0.0, scale=None, slopes=None, names=("out"
     w = [x.double().requires_grad_() for x in (q, k, v)]
     s = dim ** -0.5 if scale is None else scale
     mask = mask_of(a)
-    o, l, pr = attention64(mask, *w, s, cap, slopes)
+    o, l, pr = attention64(mask, *w, s, cap, slopes, offset)
     grads = torch.autograd.grad(o, w, dout.double())
     want = dict(out=o.detach(), lse=l.detach(), **dict(zip(("dq", "dk", "dv"), grads)))
-    tol = bounds(mask, *(x.detach() for x in (*w, o, l, pr)), t, s, cap, slopes, dout=dout.double(), grads=grads, depth=depth, once=form == "tiles")
+    tol = bounds(mask, *(x.detach() for x in (*w, o, l, pr)), t, s, cap, slopes, offset, dout=dout.double(), grads=grads, depth=depth, once=form == "tiles")
     for name in names:
         near(got[name], want[name], tol[name], name)
     p.check_error()
@@ -243,3 +243,13 @@ def test_slopes_changed_before_the_backward_pass(gpu):
     slopes.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         out.backward(dout)
+
+
+@pytest.mark.parametrize("offset", [0, 100_000])
+@pytest.mark.parametrize("form,t,dim", [("tiles", BF16, 64), ("tiles", F16, 128), ("rows", BF16, 64), ("rows", F16, 32), ("rows", F16, 8), ("rows", BF16, 96),
+                                        ("rows", F32, 64), ("rows", F32, 8)])
+def test_gradients_under_a_far_distance_bias(gpu, form, t, dim, offset):
+    """lse is some -50000 there and rounded by 2^-9: the weights' sum is off by as much, and no share of delta may come into dq and dk."""
+    a = positional("docs", 300, cuts=[0, 1, 2, 40, 41, 200, 290])
+    q, k, v, dout = inputs(300, 300, 4, 2, dim, t, 14)
+    check(form, a, q, k, v, dout, slopes=slopes_of(4), offset=offset)
