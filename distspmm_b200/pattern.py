@@ -119,7 +119,7 @@ def stream_of(device: int) -> int:
 
 def no_tangents(*tensors) -> None:
     """Refuse dual tensors: only reverse-mode gradients are provided, and a tangent would be lost without a word."""
-    if forward_ad._current_level >= 0:
+    if getattr(forward_ad, "_current_level", 0) >= 0:
         for t in tensors:
             need(not isinstance(t, torch.Tensor) or forward_ad.unpack_dual(t).tangent is None,
                  "forward-mode derivatives are not provided")
