@@ -6,7 +6,8 @@
 //   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i
 //
 // These kernels gather: for each entry and head one row of k and one of v (or of q and dout, by columns) come out of L2, two
-// operations per element read, so L2's rate bounds them. A warp owns one chunk of entries (pattern.h) and one head; LPR lanes
+// operations per element read. What bounds them is issue (68 % of the slots in the forward of R-MAT 14, fp32, 4 heads of 32; L1 31 %): dot
+// products by shuffles, and the ends of short rows. A warp owns one chunk of entries (pattern.h) and one head; LPR lanes
 // hold a head's row in vectors of VE elements, so 32 / LPR entries are in work side by side, each with its own running
 // maximum and sum, merged when the row ends. Only listed entries are read: what other rows of k and v hold, NaN included,
 // cannot reach a row that does not list them.

@@ -7,6 +7,7 @@
 //   forward   Q            K, V      S = Q K^T                 P = exp(u - m)                       O += P V
 //   dq        Q, dO        K, V      S = Q K^T, R = dO V^T     dS = P (R - delta0) c, P c           dQ += dS K, Y += P c K
 //   dk, dv    K, V         Q, dO     S^T = K Q^T, R^T = V dO^T P^T, dS^T                            dV += P^T dO, dK += dS^T Q
+//
 // All weights but P c are in two parts.
 //
 // A CTA: four warps of weights (a thread owns one of the 128 rows: the running maximum, sum and all masks are its own
@@ -17,14 +18,15 @@
 // the result the same (weights and their sum share the stale maximum). It takes the tiles from the last to the first: under a
 // causal mask with a distance bias scores fall along that way, and the maximum stands after one tile.
 //
-// Rounding: weights enter the second products as hi + lo, two parts of the operands' 16-bit type, and so do the score gradients (2^-16
-// of a value is lost at most). One part alone put a second rounding of the result's size into out and dv (window case below: 218
-// instead of 260 us forward; documents: 115 instead of 126 us dk and dv). The first delta0 = dout . out has a rounded
-// out; so dq = sum p c (dp - delta0) k - g sum p c k with g = sum p (dp - delta0) = delta - delta0, whose weights p c may be rounded once, as g is
-// but a rounding itself; delta0 + g is what dk takes. fp16 has few exponents:
-// weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is scaled by a power of two that brings the
-// largest |dout| (of the row for dq, of the streamed rows for dk and dv) near 16; both come off in the epilogue. Rows whose largest dS
-// still leaves fp16's range, or comes so low that its parts lose bits, are computed again as below.
+// Rounding: weights enter the second products as hi + lo, two parts of the operands' 16-bit type, and so do the score gradients
+// (2^-16 of a value is lost at most). One part alone put a second rounding of the result's size into out and dv (window case below:
+// 218 instead of 260 us forward; documents: 115 instead of 126 us dk and dv). The first delta0 = dout . out has a rounded out in it; so
+// dq = scale (sum p c (dp - delta0) k - g sum p c k) with g = sum p (dp - delta0) = delta - delta0. The weights p c of the last sum may be
+// rounded once, since g is of a rounding's size itself. dk and dv read delta0 + g.
+//
+// fp16 has few exponents: weights are carried 2^6 above (forward) or 2^12 above (backward) their value, and dS is scaled by a power of
+// two that brings the largest |dout| (of the row for dq, of the streamed rows for dk and dv) near 16; both come off in the epilogue.
+// Rows whose largest dS still leaves fp16's range, or comes so low that its parts lose bits, are computed again as below.
 //
 // Masks and values that are not finite: an entry that is not listed has weight 0, but 0 x NaN in the product is NaN. So a row
 // whose result is not finite is computed again by attn_row.cuh's gather, which reads listed entries only. A NaN that belongs
